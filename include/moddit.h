@@ -278,6 +278,15 @@ int moddit_select_topk_blocks(const void* map_f16, int H, int n, int count, cons
  */
 int moddit_tile_lists(const uint8_t* mask, int Hm, int nbq, int nbk, int block_size, int N,
                       int kv_block_limit, int32_t* counts, int32_t* entries, int32_t* order, void* stream);
+/* The lists of the backward pass: for each (mask head, key tile of 128) the query tiles that attend to it, ascending, each
+ * as (query_tile << 8) | flags, flag bit (2*row_half + col_half) as above.  No reference counterpart (the reference has no
+ * backward pass).
+ *   counts : (Hm, ntiles) int32      entries : (Hm, ntiles, ntiles) int32
+ *   order  : NULL or Hm*ntiles int32, as moddit_tile_lists makes it for pairs: order[pos] = head*ntiles + tile
+ * N up to 6,553,600 (51,200 tiles).
+ */
+int moddit_key_lists(const uint8_t* mask, int Hm, int nbq, int nbk, int block_size, int N, int kv_block_limit,
+                     int32_t* counts, int32_t* entries, int32_t* order, void* stream);
 /* The start order alone, for launches over groups of heads: heads [g*heads_per_group, (g+1)*heads_per_group) form
  * group g, whose part of `order` starts at g*heads_per_group*npairs, is laid out like the order of a launch with
  * that many heads and holds indices relative to the group's first head.  heads_per_group = Hm gives the order
@@ -319,6 +328,27 @@ int moddit_sparse_attn_fwd(const void* q, const void* k, const void* v, int dtyp
                            const int32_t* counts, const int32_t* entries, const int32_t* order, int Hm,
                            float softmax_scale, int q_split, int kv_len_lo, int kv_len_hi, void* out,
                            float* lse, int32_t* status, void* stream);
+
+/* Gradients of the block-sparse attention: with s = softmax_scale * q.k over the pairs that the forward kept and
+ * P = exp(s - lse), computed again tile by tile, and delta = sum(dout * out) per row,
+ *   dv = P^T dout,  ds = P * (dout v^T - delta),  dq = softmax_scale * ds k,  dk = softmax_scale * ds^T q.
+ * No reference counterpart (the reference runs inference only).  Results do not depend on the order in which blocks run.
+ *   q,k,v, Hm, softmax_scale, q_split, kv_len_lo, kv_len_hi : as in the forward;  out, lse : what it gave
+ *   dout, dq, dk, dv : (BH, N, D) like q;  none of the outputs may overlap an input
+ *   q_counts, q_entries, q_order : lists of moddit_tile_lists;  k_counts, k_entries, k_order : lists of moddit_key_lists for
+ *               the same mask (the orders may be NULL)
+ *   workspace : moddit_sparse_attn_bwd_workspace_bytes(BH, N) bytes of scratch, 16-byte aligned
+ *   status    : as in the forward
+ * Rows that attend to nothing (lse = -inf) and keys that no row attends to get zeros.  Keys at and past the larger limit are
+ * never read; all other rows have to be finite, because a tile is multiplied whole where its mask keeps any of it.
+ */
+size_t moddit_sparse_attn_bwd_workspace_bytes(int BH, int N);
+int moddit_sparse_attn_bwd(const void* q, const void* k, const void* v, const void* out, const void* dout, const float* lse,
+                           int dtype, int BH, int N, int D, const int32_t* q_counts, const int32_t* q_entries,
+                           const int32_t* q_order, const int32_t* k_counts, const int32_t* k_entries,
+                           const int32_t* k_order, int Hm, float softmax_scale, int q_split, int kv_len_lo,
+                           int kv_len_hi, void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
+                           int32_t* status, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
  * Strided row copy: `rows` rows of `width_bytes` bytes from src (pitch src_pitch) to dst (pitch dst_pitch).
@@ -407,6 +437,27 @@ int moddit_qkv_prologue(const void* q_in, const void* k_in, const void* v_in, in
                         const float* rope_sin, int rope_form, int rope_lo, int rope_hi, void* q_out, void* k_out,
                         void* v_out, int N_out, int dst_row0, float* q_pool, float* k_pool, int block_size,
                         void* workspace, size_t ws_bytes, void* stream);
+
+/* Gradients of the prologue: the rotation turned back, then the normalisation's gradient, from head-major to token-major, and
+ * the gradients of its weight and bias.  (No reference counterpart: the reference runs inference only.)  With g a row's
+ * gradient before the rotation, r and xhat the row's factor and its normalised values, computed again in float32 from x:
+ *   rms:   dx = r * (g*w - xhat * mean(g*w*xhat))      layer:  dx = r * (g*w - mean(g*w) - xhat * mean(g*w*xhat))
+ *   dweight = sum over tokens (and heads, where they share the weight) of g*xhat,   dbias = sum of g
+ * the forward's roundings of intermediate values counting as the identity; float32 sums, each result rounded once.
+ *   dq,dk,dv  : (B, H, N_out, D) head-major gradients; token s is row src_row0 + s.  Any may be null and is then skipped
+ *   q_in,k_in : the forward's inputs ((B, S, >= H*D), token_stride elements between tokens); not read for MODDIT_NORM_NONE
+ *   dq_in,dk_in,dv_in : (B, S, H*D) results, out_stride elements between tokens (slices of one buffer are fine)
+ *   dq_weight..dk_bias: null, or where the parameter's gradient goes (D values, H*D for MODDIT_NORM_RMS_ALL_HEADS), of `dtype`
+ *   workspace : moddit_qkv_prologue_bwd_workspace_bytes(...) bytes, 16-byte aligned, only for parameter gradients
+ * MODDIT_NORM_RMS_ALL_HEADS covers up to 49,152 values a token.  All other arguments as in moddit_qkv_prologue.
+ */
+size_t moddit_qkv_prologue_bwd_workspace_bytes(int B, int S, int H, int D, int norm_kind);
+int moddit_qkv_prologue_bwd(const void* dq, const void* dk, const void* dv, const void* q_in, const void* k_in, int dtype,
+                            int B, int S, int H, int D, int64_t token_stride, int norm_kind, const void* q_weight,
+                            const void* k_weight, float eps, const float* rope_cos, const float* rope_sin, int rope_form,
+                            int rope_lo, int rope_hi, int N_out, int src_row0, void* dq_in, void* dk_in, void* dv_in,
+                            int64_t out_stride, void* dq_weight, void* dq_bias, void* dk_weight, void* dk_bias,
+                            void* workspace, size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }

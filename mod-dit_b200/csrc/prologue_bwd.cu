@@ -1,0 +1,485 @@
+// Gradients of the attention prologue (prologue.cu): the rotary embedding turned back, the normalisation's gradient, the
+// move from the head-major to the token-major layout and the gradients of the norm's weight and bias, in one pass over the
+// data.  With g the gradient of a row after the rotation is turned back, x the projection, w the weight, r the row's factor:
+//   rms    r = rsqrt(mean(x^2) + eps)          dx = r g w - x r^3 mean(g w x)
+//   layer  xhat = (x - mean) r                 dx = r (g w - mean(g w) - xhat mean(g w xhat))
+//   dw = sum over rows of g xhat (xhat = x r for rms),   db = sum of g
+// The forward's intermediate roundings to the 16-bit type count as the identity; the factors are computed again in float32
+// from x, so the forward keeps nothing for this pass but its inputs.
+//
+// Bound: HBM.  Algorithmic bytes per token: q and k 3 * 2 * H * D each (g and x in, dx out), v 2 * 2 * H * D; the rotary
+// tables are fetched once for all heads and shared through L2.
+//
+// Weight gradients are sums over all tokens.  Blocks are persistent: a thread keeps float32 sums for the eight columns it
+// always has, a block adds its threads' sums in shared memory and writes one row of partial sums, and a second kernel adds
+// the rows in index order: the results are the same bits on every run.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+
+namespace moddit {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kRows = 4;                // rows per thread of an item of the per-head kernel
+
+template <typename T>
+struct Pair;
+template <>
+struct Pair<__nv_bfloat16> {
+  static __device__ __forceinline__ float2 floats(uint32_t w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  static __device__ __forceinline__ __nv_bfloat16 round(float a) { return __float2bfloat16_rn(a); }
+};
+template <>
+struct Pair<__half> {
+  static __device__ __forceinline__ float2 floats(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  static __device__ __forceinline__ __half round(float a) { return __float2half_rn(a); }
+};
+
+template <typename T>
+__device__ __forceinline__ void unpack(const uint4& v, float (&f)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 p = Pair<T>::floats(w[i]);
+    f[2 * i] = p.x;
+    f[2 * i + 1] = p.y;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
+  return make_uint4(Pair<T>::pack(f[0], f[1]), Pair<T>::pack(f[2], f[3]), Pair<T>::pack(f[4], f[5]), Pair<T>::pack(f[6], f[7]));
+}
+
+// Sum over an aligned group of kLanes lanes of a warp.
+template <int kLanes>
+__device__ __forceinline__ float lane_sum(float x) {
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+
+struct BwdArgs {
+  const void* g[3];        // (B, H, N_out, D)
+  const void* x[2];        // token-major, token_stride elements between tokens; null without a norm
+  void* dx[3];             // token-major, out_stride elements between tokens
+  const void* weight[2];
+  float* part[2];          // partial sums: gridDim.x rows of dw, then as many of db
+  const float* cos;
+  const float* sin;
+  int64_t token_stride, out_stride;
+  int B, S, H, N_out, src_row0, rope_form, rope_lo, rope_hi;
+  float eps;
+};
+
+// Turns eight gradients of token s (columns 8 c to 8 c + 7 of a head) back through the rotation.
+template <int D>
+__device__ __forceinline__ void unrotate(const BwdArgs& a, int s, int c, float (&g)[8]) {
+  if (a.cos == nullptr || s < a.rope_lo || s >= a.rope_hi) return;
+  float cs[8], sn[8];
+  if (a.rope_form == MODDIT_ROPE_PAIR) {
+    const int64_t at = static_cast<int64_t>(s - a.rope_lo) * (D / 2) + c * 4;
+    const float4 c4 = __ldg(reinterpret_cast<const float4*>(a.cos + at)), s4 = __ldg(reinterpret_cast<const float4*>(a.sin + at));
+    const float cv[4] = {c4.x, c4.y, c4.z, c4.w}, sv[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      cs[2 * i] = cs[2 * i + 1] = cv[i];
+      sn[2 * i] = sn[2 * i + 1] = sv[i];
+    }
+  } else {
+    const int64_t at = static_cast<int64_t>(s - a.rope_lo) * D + c * 8;
+#pragma unroll
+    for (int i = 0; i < 8; i += 4) {
+      *reinterpret_cast<float4*>(cs + i) = __ldg(reinterpret_cast<const float4*>(a.cos + at + i));
+      *reinterpret_cast<float4*>(sn + i) = __ldg(reinterpret_cast<const float4*>(a.sin + at + i));
+    }
+    if (a.rope_form == MODDIT_ROPE_EVEN_COS_ODD_SIN) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        cs[2 * i + 1] = cs[2 * i];
+        sn[2 * i] = sn[2 * i + 1];
+      }
+    }
+  }
+  // out0 = y0 cs0 - y1 sn0, out1 = y0 sn1 + y1 cs1
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float g0 = g[2 * i], g1 = g[2 * i + 1];
+    g[2 * i] = g0 * cs[2 * i] + g1 * sn[2 * i + 1];
+    g[2 * i + 1] = g1 * cs[2 * i + 1] - g0 * sn[2 * i];
+  }
+}
+
+// Grid: x = persistent blocks, y = tensor.  An item is kRows rows per thread of one head; neighbouring items are the heads of
+// the same tokens, so the table rows are shared.
+template <typename T, int D, int kNorm>
+__global__ void __launch_bounds__(kThreads) prologue_bwd_kernel(const __grid_constant__ BwdArgs a) {
+  constexpr int kTpr = D / 8;                     // threads per row
+  constexpr int kRpp = kThreads / kTpr;           // rows per pass
+  constexpr float kInvD = 1.0f / D;
+  __shared__ float red[kRpp][D];
+  const int which = blockIdx.y;
+  const T* __restrict__ g_in = static_cast<const T*>(a.g[which]);
+  if (g_in == nullptr) return;
+  T* __restrict__ dx = static_cast<T*>(a.dx[which]);
+  const int c = threadIdx.x % kTpr, rg = threadIdx.x / kTpr;
+  const bool normed = kNorm != MODDIT_NORM_NONE && which < 2;
+  float w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = 1.f;
+  if (normed && a.weight[which] != nullptr) unpack<T>(__ldg(static_cast<const uint4*>(a.weight[which]) + c), w);
+  float dw[8] = {}, db[8] = {};
+  const int blocks = (a.S + kRows * kRpp - 1) / (kRows * kRpp);
+  const int64_t items = static_cast<int64_t>(a.B) * blocks * a.H;
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int h = static_cast<int>(item % a.H);
+    const int64_t bt = item / a.H;
+    const int b = static_cast<int>(bt / blocks);
+    const int s0 = static_cast<int>(bt - static_cast<int64_t>(b) * blocks) * kRows * kRpp + rg;
+    const T* gp = g_in + ((static_cast<int64_t>(b) * a.H + h) * a.N_out + a.src_row0) * D + c * 8;
+    const int64_t tok0 = static_cast<int64_t>(b) * a.S;
+    uint4 gv[kRows], xv[kRows];
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) {
+      const int s = s0 + u * kRpp;
+      const bool in = s < a.S;
+      gv[u] = in ? __ldg(reinterpret_cast<const uint4*>(gp + static_cast<int64_t>(s) * D)) : make_uint4(0, 0, 0, 0);
+      if (normed)
+        xv[u] = in ? __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.x[which]) + (tok0 + s) * a.token_stride + h * D + c * 8))
+                   : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) {
+      const int s = s0 + u * kRpp;
+      uint4 res = gv[u];
+      if (which < 2 && (normed || a.cos != nullptr)) {
+        float g[8];
+        unpack<T>(gv[u], g);
+        if (s < a.S) unrotate<D>(a, s, c, g);
+        if (normed) {
+          float x[8];
+          unpack<T>(xv[u], x);
+          if constexpr (kNorm == MODDIT_NORM_RMS_HEAD) {
+            float ss = 0.f, sg = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              ss = fmaf(x[i], x[i], ss);
+              sg = fmaf(g[i] * w[i], x[i], sg);
+            }
+            const float ms = lane_sum<kTpr>(ss) * kInvD;
+            const float r = s < a.S ? rsqrtf(ms + a.eps) : 0.f;     // rows past the end add nothing, eps = 0 included
+            const float f = -r * r * (lane_sum<kTpr>(sg) * kInvD);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              dw[i] = fmaf(g[i], x[i] * r, dw[i]);
+              g[i] = r * fmaf(x[i], f, g[i] * w[i]);
+            }
+          } else if constexpr (kNorm == MODDIT_NORM_LAYER) {
+            float sx = 0.f, sg = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              sx += x[i];
+              sg = fmaf(g[i], w[i], sg);
+            }
+            const float mean = lane_sum<kTpr>(sx) * kInvD, mg = lane_sum<kTpr>(sg) * kInvD;
+            float ss = 0.f, sgx = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              x[i] -= mean;
+              ss = fmaf(x[i], x[i], ss);
+              sgx = fmaf(g[i] * w[i], x[i], sgx);
+            }
+            const float ms = lane_sum<kTpr>(ss) * kInvD;
+            const float r = s < a.S ? rsqrtf(ms + a.eps) : 0.f;     // rows past the end add nothing, eps = 0 included
+            const float f = -r * r * (lane_sum<kTpr>(sgx) * kInvD);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              dw[i] = fmaf(g[i], x[i] * r, dw[i]);
+              db[i] += g[i];
+              g[i] = r * (fmaf(x[i], f, g[i] * w[i]) - mg);
+            }
+          }
+        }
+        res = pack8<T>(g);
+      }
+      if (s < a.S) *reinterpret_cast<uint4*>(dx + (tok0 + s) * a.out_stride + h * D + c * 8) = res;
+    }
+  }
+  if (normed && a.part[which] != nullptr) {
+    for (int k = 0; k < (kNorm == MODDIT_NORM_LAYER ? 2 : 1); ++k) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) red[rg][c * 8 + i] = k ? db[i] : dw[i];
+      __syncthreads();
+      if (threadIdx.x < D) {
+        float t = 0.f;
+        for (int j = 0; j < kRpp; ++j) t += red[j][threadIdx.x];
+        a.part[which][(static_cast<int64_t>(k) * gridDim.x + blockIdx.x) * D + threadIdx.x] = t;
+      }
+    }
+  }
+}
+
+// Normalisation over all heads of a token.  A block has one token per warp at a time.  First every warp sums x^2 and g w x
+// over its token; then a thread takes fixed pieces of eight columns through the block's tokens, whose rows it reads again
+// (they are in the L2), writes dx and adds to its columns' weight gradient, which lives in shared memory.
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) prologue_bwd_all_heads_kernel(const __grid_constant__ BwdArgs a) {
+  constexpr int kTpr = D / 8;
+  constexpr int kTokens = kThreads / 32;
+  extern __shared__ float dw_s[];                 // H * D
+  __shared__ float r_s[kTokens], f_s[kTokens];
+  const int which = blockIdx.y;
+  const T* __restrict__ g_in = static_cast<const T*>(a.g[which]);
+  if (g_in == nullptr) return;
+  const T* __restrict__ x_in = which < 2 ? static_cast<const T*>(a.x[which]) : nullptr;
+  T* __restrict__ dx = static_cast<T*>(a.dx[which]);
+  const uint4* wp = which < 2 ? static_cast<const uint4*>(a.weight[which]) : nullptr;
+  const int W = a.H * D, pieces = W / 8;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const bool sums = which < 2 && a.part[which] != nullptr;
+  if (sums)
+    for (int i = threadIdx.x; i < W; i += kThreads) dw_s[i] = 0.f;
+  const float inv_w = 1.f / static_cast<float>(W);
+  const int groups = (a.S + kTokens - 1) / kTokens;
+  auto g_at = [&](int b, int s, int p) {
+    return reinterpret_cast<const uint4*>(g_in + ((static_cast<int64_t>(b) * a.H + p / kTpr) * a.N_out + a.src_row0 + s) * D) + p % kTpr;
+  };
+  auto x_at = [&](int b, int s, int p) {
+    return reinterpret_cast<const uint4*>(x_in + (static_cast<int64_t>(b) * a.S + s) * a.token_stride) + p;
+  };
+  for (int64_t grp = blockIdx.x; grp < static_cast<int64_t>(a.B) * groups; grp += gridDim.x) {
+    const int b = static_cast<int>(grp / groups);
+    const int s0 = static_cast<int>(grp - static_cast<int64_t>(b) * groups) * kTokens;
+    if (which < 2) {
+      const int s = s0 + warp;
+      float ss = 0.f, sg = 0.f;
+      if (s < a.S) {
+#pragma unroll 4
+        for (int p = lane; p < pieces; p += 32) {
+          float g[8], x[8], w[8];
+          unpack<T>(__ldg(g_at(b, s, p)), g);
+          unpack<T>(__ldg(x_at(b, s, p)), x);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w[i] = 1.f;
+          if (wp != nullptr) unpack<T>(__ldg(wp + p), w);
+          unrotate<D>(a, s, p % kTpr, g);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            ss = fmaf(x[i], x[i], ss);
+            sg = fmaf(g[i] * w[i], x[i], sg);
+          }
+        }
+      }
+      ss = lane_sum<32>(ss);
+      sg = lane_sum<32>(sg);
+      __syncthreads();                            // the previous group's factors have been read
+      if (lane == 0) {
+        const float r = rsqrtf(ss * inv_w + a.eps);
+        r_s[warp] = r;
+        f_s[warp] = -r * r * (sg * inv_w);
+      }
+      __syncthreads();
+    }
+    for (int p = threadIdx.x; p < pieces; p += kThreads) {
+      float w[8], dw[8] = {};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = 1.f;
+      if (wp != nullptr) unpack<T>(__ldg(wp + p), w);
+#pragma unroll
+      for (int t = 0; t < kTokens; ++t) {
+        const int s = s0 + t;
+        if (s >= a.S) break;
+        uint4 res = __ldg(g_at(b, s, p));
+        if (which < 2) {
+          float g[8], x[8];
+          unpack<T>(res, g);
+          unpack<T>(__ldg(x_at(b, s, p)), x);
+          unrotate<D>(a, s, p % kTpr, g);
+          const float r = r_s[t], f = f_s[t];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            dw[i] = fmaf(g[i], x[i] * r, dw[i]);
+            g[i] = r * fmaf(x[i], f, g[i] * w[i]);
+          }
+          res = pack8<T>(g);
+        }
+        *(reinterpret_cast<uint4*>(dx + (static_cast<int64_t>(b) * a.S + s) * a.out_stride) + p) = res;
+      }
+      if (sums)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dw_s[p * 8 + i] += dw[i];
+    }
+  }
+  if (sums) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < W; i += kThreads) a.part[which][static_cast<int64_t>(blockIdx.x) * W + i] = dw_s[i];
+  }
+}
+
+// Adds the rows of partial sums in index order: 32 columns a block, eight groups of rows.  y = tensor, z = weight, bias.
+struct SumArgs {
+  const float* part[2];
+  void* out[2][2];
+};
+template <typename T>
+__global__ void __launch_bounds__(kThreads) prologue_bwd_sums_kernel(const __grid_constant__ SumArgs a, int rows, int width) {
+  __shared__ float red[8][32];
+  T* out = static_cast<T*>(a.out[blockIdx.y][blockIdx.z]);
+  if (out == nullptr) return;
+  const int col = blockIdx.x * 32 + threadIdx.x % 32, grp = threadIdx.x / 32;
+  const float* p = a.part[blockIdx.y] + static_cast<int64_t>(blockIdx.z) * rows * width;
+  float t = 0.f;
+#pragma unroll 8
+  for (int j = grp; j < rows; j += 8) t += p[static_cast<int64_t>(j) * width + col];
+  red[grp][threadIdx.x % 32] = t;
+  __syncthreads();
+  if (grp == 0) {
+#pragma unroll
+    for (int j = 1; j < 8; ++j) t += red[j][threadIdx.x];
+    out[col] = Pair<T>::round(t);
+  }
+}
+
+// Persistent blocks per tensor: a fixed number, whatever the GPU, so that the order of the sums does not depend on it; more
+// than the items of a tensor would only add rows of zeros.
+constexpr int kBlocksPerHead = 592;      // per-head kernel
+constexpr int kBlocksAllHeads = 296;
+int blocks_for(int B, int S, int H, int D, int norm_kind) {
+  if (norm_kind == MODDIT_NORM_RMS_ALL_HEADS)
+    return static_cast<int>(std::min<int64_t>(kBlocksAllHeads, static_cast<int64_t>(B) * ceil_div(S, kThreads / 32)));
+  return static_cast<int>(std::min<int64_t>(kBlocksPerHead, static_cast<int64_t>(B) * ceil_div(S, kRows * kThreads / (D / 8)) * H));
+}
+
+template <typename T, int D>
+int launch_bwd(const BwdArgs& a, int norm_kind, int blocks, const SumArgs& sums, cudaStream_t st) {
+  const dim3 grid(blocks, 3);
+  switch (norm_kind) {
+    case MODDIT_NORM_NONE:
+      prologue_bwd_kernel<T, D, MODDIT_NORM_NONE><<<grid, kThreads, 0, st>>>(a);
+      break;
+    case MODDIT_NORM_RMS_HEAD:
+      prologue_bwd_kernel<T, D, MODDIT_NORM_RMS_HEAD><<<grid, kThreads, 0, st>>>(a);
+      break;
+    case MODDIT_NORM_LAYER:
+      prologue_bwd_kernel<T, D, MODDIT_NORM_LAYER><<<grid, kThreads, 0, st>>>(a);
+      break;
+    default: {
+      auto kernel = prologue_bwd_all_heads_kernel<T, D>;
+      const size_t smem = sizeof(float) * a.H * D;
+      if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem)) return rc;
+      kernel<<<grid, kThreads, smem, st>>>(a);
+    }
+  }
+  MODDIT_CHECK_LAUNCH("prologue_bwd_kernel");
+  if (sums.out[0][0] || sums.out[0][1] || sums.out[1][0] || sums.out[1][1]) {
+    const int width = norm_kind == MODDIT_NORM_RMS_ALL_HEADS ? a.H * D : D;
+    prologue_bwd_sums_kernel<T><<<dim3(width / 32, 2, norm_kind == MODDIT_NORM_LAYER ? 2 : 1), kThreads, 0, st>>>(sums, blocks, width);
+    MODDIT_CHECK_LAUNCH("prologue_bwd_sums_kernel");
+  }
+  return MODDIT_OK;
+}
+
+}  // namespace
+}  // namespace moddit
+
+using namespace moddit;
+
+extern "C" size_t moddit_qkv_prologue_bwd_workspace_bytes(int B, int S, int H, int D, int norm_kind) {
+  if (B <= 0 || S <= 0 || H <= 0 || (D != 64 && D != 128) || norm_kind <= MODDIT_NORM_NONE || norm_kind > MODDIT_NORM_LAYER) return 0;
+  const size_t width = norm_kind == MODDIT_NORM_RMS_ALL_HEADS ? static_cast<size_t>(H) * D : 2 * D;
+  return 2 * width * blocks_for(B, S, H, D, norm_kind) * sizeof(float);
+}
+
+extern "C" int moddit_qkv_prologue_bwd(const void* dq, const void* dk, const void* dv, const void* q_in, const void* k_in,
+                                       int dtype, int B, int S, int H, int D, int64_t token_stride, int norm_kind,
+                                       const void* q_weight, const void* k_weight, float eps, const float* rope_cos,
+                                       const float* rope_sin, int rope_form, int rope_lo, int rope_hi, int N_out, int src_row0,
+                                       void* dq_in, void* dk_in, void* dv_in, int64_t out_stride, void* dq_weight,
+                                       void* dq_bias, void* dk_weight, void* dk_bias, void* workspace, size_t ws_bytes,
+                                       void* stream) {
+  clear_error();
+  MODDIT_CHECK_ARG(dtype == MODDIT_BF16 || dtype == MODDIT_FP16, "dtype must be MODDIT_BF16 or MODDIT_FP16");
+  MODDIT_CHECK_ARG(D == 64 || D == 128, "head_dim %d not supported (64 or 128)", D);
+  MODDIT_CHECK_ARG(B > 0 && S > 0 && H > 0, "B, S and H must be positive (got %d, %d, %d)", B, S, H);
+  MODDIT_CHECK_ARG(norm_kind >= MODDIT_NORM_NONE && norm_kind <= MODDIT_NORM_LAYER, "unknown norm_kind %d", norm_kind);
+  MODDIT_CHECK_ARG(dq != nullptr || dk != nullptr || dv != nullptr, "no gradient given");
+  MODDIT_CHECK_ARG(src_row0 >= 0 && static_cast<int64_t>(src_row0) + S <= N_out, "rows %d..%lld are not in tensors of %d rows",
+                   src_row0, static_cast<long long>(src_row0) + S, N_out);
+  const int64_t width = static_cast<int64_t>(H) * D;
+  MODDIT_CHECK_ARG(out_stride >= width && out_stride % 8 == 0, "out_stride %lld must be a multiple of 8 elements and at least H*D",
+                   static_cast<long long>(out_stride));
+  const void* g[3] = {dq, dk, dv};
+  const void* x[2] = {q_in, k_in};
+  void* dx[3] = {dq_in, dk_in, dv_in};
+  for (int i = 0; i < 3; ++i) {
+    if (g[i] == nullptr) continue;
+    MODDIT_CHECK_ARG(dx[i] != nullptr, "gradient %d has no output buffer", i);
+    MODDIT_CHECK_ARG(aligned16(g[i]) && aligned16(dx[i]), "tensor %d is not 16-byte aligned", i);
+    if (i < 2 && norm_kind != MODDIT_NORM_NONE) {
+      MODDIT_CHECK_ARG(x[i] != nullptr && aligned16(x[i]), "input %d of the normalisation is null or not 16-byte aligned", i);
+      MODDIT_CHECK_ARG(token_stride >= width && token_stride % 8 == 0,
+                       "token_stride %lld must be a multiple of 8 elements and at least H*D", static_cast<long long>(token_stride));
+    }
+  }
+  MODDIT_CHECK_ARG(aligned16(q_weight) && aligned16(k_weight), "norm parameters must be 16-byte aligned");
+  void* grads[2][2] = {{dq_weight, dq_bias}, {dk_weight, dk_bias}};
+  bool any = false;
+  for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < 2; ++j) {
+      if (grads[i][j] == nullptr) continue;
+      any = true;
+      MODDIT_CHECK_ARG(g[i] != nullptr, "parameter gradient of tensor %d without its gradient", i);
+      MODDIT_CHECK_ARG(norm_kind != MODDIT_NORM_NONE && (j == 0 || norm_kind == MODDIT_NORM_LAYER),
+                       "norm_kind %d has no such parameter", norm_kind);
+    }
+  MODDIT_CHECK_ARG((rope_cos == nullptr) == (rope_sin == nullptr), "rope_cos and rope_sin go together");
+  if (rope_cos != nullptr) {
+    MODDIT_CHECK_ARG(aligned16(rope_cos) && aligned16(rope_sin), "rotary tables must be 16-byte aligned");
+    MODDIT_CHECK_ARG(0 <= rope_lo && rope_lo <= rope_hi && rope_hi <= S, "rotary range [%d, %d) outside 0..%d", rope_lo, rope_hi, S);
+    MODDIT_CHECK_ARG(rope_form >= MODDIT_ROPE_ELEMENTWISE && rope_form <= MODDIT_ROPE_PAIR, "unknown rope_form %d", rope_form);
+  }
+  if (norm_kind == MODDIT_NORM_RMS_ALL_HEADS && width > 48 * 1024)
+    return fail(MODDIT_E_UNSUPPORTED, "a normalisation over all heads covers at most 49,152 values, got %lld", static_cast<long long>(width));
+  if (any && (workspace == nullptr || !aligned16(workspace) || ws_bytes < moddit_qkv_prologue_bwd_workspace_bytes(B, S, H, D, norm_kind)))
+    return fail(MODDIT_E_WORKSPACE, "parameter gradients need a 16-byte aligned workspace of %zu bytes",
+                moddit_qkv_prologue_bwd_workspace_bytes(B, S, H, D, norm_kind));
+  if (int rc = require_sm100()) return rc;
+
+  const int blocks = blocks_for(B, S, H, D, norm_kind);
+  const int64_t per = static_cast<int64_t>(blocks) * (norm_kind == MODDIT_NORM_RMS_ALL_HEADS ? width : 2 * D);
+  BwdArgs a{};
+  SumArgs sums{};
+  for (int i = 0; i < 3; ++i) { a.g[i] = g[i]; a.dx[i] = dx[i]; }
+  for (int i = 0; i < 2; ++i) {
+    a.x[i] = x[i];
+    a.part[i] = grads[i][0] || grads[i][1] ? static_cast<float*>(workspace) + i * per : nullptr;
+    sums.part[i] = a.part[i];
+    sums.out[i][0] = grads[i][0];
+    sums.out[i][1] = grads[i][1];
+  }
+  a.weight[0] = q_weight; a.weight[1] = k_weight;
+  a.cos = rope_cos; a.sin = rope_sin;
+  a.token_stride = token_stride; a.out_stride = out_stride;
+  a.B = B; a.S = S; a.H = H; a.N_out = N_out; a.src_row0 = src_row0;
+  a.rope_form = rope_form; a.rope_lo = rope_lo; a.rope_hi = rope_hi;
+  a.eps = eps;
+  cudaStream_t st = as_stream(stream);
+  if (dtype == MODDIT_BF16)
+    return D == 128 ? launch_bwd<__nv_bfloat16, 128>(a, norm_kind, blocks, sums, st) : launch_bwd<__nv_bfloat16, 64>(a, norm_kind, blocks, sums, st);
+  return D == 128 ? launch_bwd<__half, 128>(a, norm_kind, blocks, sums, st) : launch_bwd<__half, 64>(a, norm_kind, blocks, sums, st);
+}

@@ -405,6 +405,58 @@ __global__ void __launch_bounds__(kListThreads) tile_lists_kernel(const uint8_t*
   if (lane == 0) counts[static_cast<int64_t>(h) * npairs + p] = base;
 }
 
+// The lists of the backward pass: for every key tile the query tiles that attend to it.  One CTA has 32 neighbouring key
+// tiles of a mask head.  It reads the mask rows of kKeyChunk query tiles at a time, a warp a row (32 neighbouring bytes, 64
+// at block size 64), leaves the four flags of every (query tile, key tile) in shared memory, and compacts them key tile by
+// key tile with ballots: each warp has four key tiles and writes their lists in increasing query-tile order.
+// A warp that walked a mask column by itself would fetch a 32-byte sector for every byte.
+constexpr int kKeyChunk = 128;
+__global__ void __launch_bounds__(kListThreads) key_lists_kernel(const uint8_t* __restrict__ mask, int nbq, int nbk, int sub,
+                                                                 int nt, int kv_block_limit, int32_t* __restrict__ counts,
+                                                                 int32_t* __restrict__ entries) {
+  __shared__ uint8_t flags[kKeyChunk][33];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int k0 = blockIdx.x * 32, h = blockIdx.y;
+  const uint8_t* mh = mask + static_cast<int64_t>(h) * nbq * nbk;
+  const int lim = min(nbk, kv_block_limit);
+  int base[4] = {0, 0, 0, 0};
+  for (int q0 = 0; q0 < nt; q0 += kKeyChunk) {
+#pragma unroll 8
+    for (int u = 0; u < kKeyChunk / 8; ++u) {
+      const int qt = q0 + 8 * u + warp, kt = k0 + lane;
+      int fl = 0;
+      if (qt < nt && kt < nt) {
+        if (sub == 1) {
+          fl = (qt < nbq && kt < lim && mh[static_cast<int64_t>(qt) * nbk + kt]) ? 0xf : 0;
+        } else {
+          for (int rh = 0; rh < 2; ++rh)
+            for (int ch = 0; ch < 2; ++ch) {
+              const int bi = 2 * qt + rh, bj = 2 * kt + ch;
+              if (bi < nbq && bj < lim && mh[static_cast<int64_t>(bi) * nbk + bj]) fl |= 1 << (2 * rh + ch);
+            }
+        }
+      }
+      flags[8 * u + warp][lane] = static_cast<uint8_t>(fl);
+    }
+    __syncthreads();
+    for (int j = 0; j < 4; ++j) {
+      const int kt = k0 + 4 * warp + j;
+      if (kt >= nt) continue;
+      int32_t* out = entries + (static_cast<int64_t>(h) * nt + kt) * nt;
+      for (int c = 0; c < kKeyChunk; c += 32) {
+        const int fl = flags[c + lane][4 * warp + j];
+        const unsigned bal = __ballot_sync(0xffffffffu, fl != 0);
+        if (fl) out[base[j] + __popc(bal & ((1u << lane) - 1))] = ((q0 + c + lane) << 8) | fl;
+        base[j] += __popc(bal);
+      }
+    }
+    __syncthreads();
+  }
+  if (lane < 4 && k0 + 4 * warp + lane < nt)
+    counts[static_cast<int64_t>(h) * nt + k0 + 4 * warp + lane] =
+        lane == 0 ? base[0] : lane == 1 ? base[1] : lane == 2 ? base[2] : base[3];
+}
+
 // Start order of the (head, query-tile pair) work items of the sparse forward: order[pos] = head * npairs + pair.
 // Pairs are ranked by list length inside their head (rank by counting; ties by index, so the result is
 // deterministic).  The kLongFirst longest pairs of EVERY head come first (a pair of text rows keeps every key
@@ -630,6 +682,29 @@ extern "C" int moddit_tile_lists(const uint8_t* mask, int Hm, int nbq, int nbk, 
   MODDIT_CHECK_LAUNCH("tile_lists_kernel");
   if (order != nullptr) {
     order_pairs_kernel<<<dim3(Hm, kOrderSplit), 256, sizeof(int32_t) * npairs, as_stream(stream)>>>(counts, npairs, Hm, order);
+    MODDIT_CHECK_LAUNCH("order_pairs_kernel");
+  }
+  return MODDIT_OK;
+}
+
+extern "C" int moddit_key_lists(const uint8_t* mask, int Hm, int nbq, int nbk, int block_size, int N, int kv_block_limit,
+                                int32_t* counts, int32_t* entries, int32_t* order, void* stream) {
+  clear_error();
+  MODDIT_CHECK_ARG(mask && counts && entries, "key_lists: null pointer");
+  MODDIT_CHECK_ARG(Hm > 0 && Hm <= 65535 && nbq > 0 && nbk > 0 && N > 0 && kv_block_limit >= 0, "key_lists: bad sizes");
+  if (block_size != 64 && block_size != 128)
+    return fail(MODDIT_E_UNSUPPORTED, "key_lists: block_size must be 64 or 128, got %d", block_size);
+  const int nt = ceil_div(N, 128);
+  if (sizeof(int32_t) * static_cast<size_t>(nt) > 200 * 1024)
+    return fail(MODDIT_E_UNSUPPORTED, "key_lists: N=%d too large", N);
+  if (int rc = require_sm100()) return rc;
+  key_lists_kernel<<<dim3(ceil_div(nt, 32), Hm), kListThreads, 0, as_stream(stream)>>>(mask, nbq, nbk, 128 / block_size, nt,
+                                                                                       kv_block_limit, counts, entries);
+  MODDIT_CHECK_LAUNCH("key_lists_kernel");
+  if (order != nullptr) {
+    const size_t smem = sizeof(int32_t) * nt;
+    if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(order_pairs_kernel), smem)) return rc;
+    order_pairs_kernel<<<dim3(Hm, kOrderSplit), 256, smem, as_stream(stream)>>>(counts, nt, Hm, order);
     MODDIT_CHECK_LAUNCH("order_pairs_kernel");
   }
   return MODDIT_OK;

@@ -25,7 +25,7 @@ static void lookup_encode() {
 namespace {
 struct CachedMap {
   const void* base;
-  int dtype, BH, N, D, box_rows;
+  int dtype, BH, N, rows, D, box_rows;
   CUtensorMap map;
 };
 constexpr int kCachedMaps = 16;
@@ -34,9 +34,13 @@ thread_local int t_maps_used = 0, t_maps_next = 0;
 }  // namespace
 
 int make_tmap_rows(CUtensorMap* map, const void* base, int dtype, int BH, int N, int D, int box_rows) {
+  return make_tmap_first_rows(map, base, dtype, BH, N, N, D, box_rows);
+}
+
+int make_tmap_first_rows(CUtensorMap* map, const void* base, int dtype, int BH, int N, int rows, int D, int box_rows) {
   for (int i = 0; i < t_maps_used; ++i) {
     const CachedMap& c = t_maps[i];
-    if (c.base == base && c.dtype == dtype && c.BH == BH && c.N == N && c.D == D && c.box_rows == box_rows) {
+    if (c.base == base && c.dtype == dtype && c.BH == BH && c.N == N && c.rows == rows && c.D == D && c.box_rows == box_rows) {
       *map = c.map;
       return MODDIT_OK;
     }
@@ -44,7 +48,12 @@ int make_tmap_rows(CUtensorMap* map, const void* base, int dtype, int BH, int N,
   std::call_once(g_once, lookup_encode);
   if (!g_encode) return fail(MODDIT_E_CUDA, "cuTensorMapEncodeTiled is not available from the driver (%s)",
                              cudaGetErrorString(g_lookup_error));
-  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(N), static_cast<cuuint64_t>(BH)};
+  // The driver wants a current context.  A thread that has made no runtime call that needs one (a backward pass runs on a
+  // thread of the autograd engine) has none yet; cudaSetDevice on the current device gives it one, also during a capture.
+  int dev = 0;
+  MODDIT_CHECK_CUDA(cudaGetDevice(&dev));
+  MODDIT_CHECK_CUDA(cudaSetDevice(dev));
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(BH)};
   const cuuint64_t strides[2] = {static_cast<cuuint64_t>(D) * 2, static_cast<cuuint64_t>(N) * D * 2};
   const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_rows), 1};
   const cuuint32_t estr[3] = {1, 1, 1};
@@ -54,7 +63,7 @@ int make_tmap_rows(CUtensorMap* map, const void* base, int dtype, int BH, int N,
                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (res != CUDA_SUCCESS) return fail(MODDIT_E_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", static_cast<int>(res));
   CachedMap& slot = t_maps[t_maps_next];
-  slot = CachedMap{base, dtype, BH, N, D, box_rows, *map};
+  slot = CachedMap{base, dtype, BH, N, rows, D, box_rows, *map};
   t_maps_next = (t_maps_next + 1) % kCachedMaps;
   if (t_maps_used < kCachedMaps) ++t_maps_used;
   return MODDIT_OK;

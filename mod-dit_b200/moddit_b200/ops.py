@@ -28,10 +28,12 @@ KERNELS_PER_CALL = {"moddit_pool_blocks": 1, "moddit_pooled_map": 1, "moddit_poo
                     "moddit_mts": 2,
                     "moddit_mtm": 1, "moddit_solve": 3, "moddit_select_lines": 1, "moddit_head_modes": 1,
                     "moddit_mask_from_lines": 1, "moddit_select_mass": 1, "moddit_tile_lists": 2,
-                    "moddit_sparse_attn_fwd": 1, "moddit_replay_status": 0,
+                    "moddit_sparse_attn_fwd": 1, "moddit_replay_status": 0, "moddit_key_lists": 2,
+                    "moddit_sparse_attn_bwd": 3,
                     # the stages of a prediction in one call: 3 + 2 + 3 (1 with the small solve) + 1 + 1 + 2
                     "moddit_predict_lines": 12, "moddit_predict_lines (small)": 10,
-                    "moddit_mts_noalloc": 2, "moddit_copy_rows_dma": 0, "moddit_qkv_prologue": 1}
+                    "moddit_mts_noalloc": 2, "moddit_copy_rows_dma": 0, "moddit_qkv_prologue": 1,
+                    "moddit_qkv_prologue_bwd": 2}
 
 
 def stage_timing(enable: bool, only=None, by_stage: bool = True) -> None:
@@ -256,6 +258,94 @@ def qkv_prologue(q_in: Optional[torch.Tensor], k_in: Optional[torch.Tensor], v_i
             _ptr(pools[1] if pools is not None and k_in is not None else None), pool_block_size, _ptr(ws),
             ws_bytes, _stream(dev)), "moddit_qkv_prologue")
     return out, pools
+
+
+def _token_stride(tensors, shape, dtype: torch.dtype, dev: torch.device, what: str) -> int:
+    """The elements between tokens that (B, S, W) tensors share; raises where they are not laid out alike."""
+    B, S, W = shape
+    stride = W
+    if tensors:
+        stride = tensors[0].stride(1) if S > 1 else tensors[0].stride(0) if B > 1 else W
+    for t in tensors:
+        if tuple(t.shape) != shape or t.dtype != dtype or t.device != dev or t.stride(2) != 1 or \
+                (S > 1 and t.stride(1) != stride) or (B > 1 and t.stride(0) != S * stride):
+            raise ValueError(f"{what} must be {shape} {dtype} tensors on {dev} with a contiguous last dimension and one "
+                             "token stride")
+    return stride
+
+
+def qkv_prologue_bwd(dq: Optional[torch.Tensor], dk: Optional[torch.Tensor], dv: Optional[torch.Tensor],
+                     q_in: Optional[torch.Tensor] = None, k_in: Optional[torch.Tensor] = None, *, num_heads: int,
+                     norm: Optional[str] = None, q_weight: Optional[torch.Tensor] = None,
+                     q_bias: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+                     k_bias: Optional[torch.Tensor] = None, eps: float = 1e-6, rope_cos: Optional[torch.Tensor] = None,
+                     rope_sin: Optional[torch.Tensor] = None, rope_form: str = "elementwise",
+                     rope_range: Optional[Tuple[int, int]] = None, src_row0: int = 0, n_tokens: Optional[int] = None,
+                     out: Optional[Tuple[Optional[torch.Tensor], ...]] = None):
+    """Gradients of `qkv_prologue` (`moddit_qkv_prologue_bwd`).
+
+    dq/dk/dv: (B, H, N, D) gradients of its outputs, any may be None; the tokens of this call are rows src_row0 to
+    src_row0 + S (`dst_row0` of the forward).  q_in/k_in, the norm's parameters, eps and the rotary arguments are the
+    forward's; q_in/k_in are needed where there is a norm.  S is that of q_in/k_in, else `n_tokens`, else the rest of the rows.
+    `out`: buffers for the gradients of q_in, k_in and v_in (B, S, H*D), slices of one fused gradient included.
+    Returns ((dq_in, dk_in, dv_in), {"q_weight", "q_bias", "k_weight", "k_bias"}): gradients of the parameters given
+    (each in its own dtype), None for the others."""
+    grads = (dq, dk, dv)
+    given = [t for t in grads if t is not None]
+    if not given:
+        raise ValueError("qkv_prologue_bwd: no gradient")
+    dev = _need_cuda(*given)
+    ref = given[0]
+    if ref.dim() != 4 or ref.shape[1] != num_heads:
+        raise ValueError(f"gradients must be (B, {num_heads}, N, D) tensors")
+    B, H, N, D = ref.shape
+    dt = _qkv_dtype(ref)
+    for t in given:
+        if t.shape != ref.shape or t.dtype != ref.dtype or not t.is_contiguous():
+            raise ValueError("dq, dk and dv must be contiguous tensors of one shape and dtype")
+    kind = _lib.NORM_KIND[norm]
+    inputs = [x if kind and g is not None else None for x, g in ((q_in, dq), (k_in, dk))]
+    if kind and any(x is None and g is not None for x, g in zip(inputs, grads)):
+        raise ValueError("the gradient of a norm needs its input (q_in, k_in)")
+    present = [x for x in inputs if x is not None]
+    if n_tokens is None:
+        n_tokens = next((x.shape[1] for x in (q_in, k_in) if x is not None), N - src_row0)
+    S = int(n_tokens)
+    stride = _token_stride(present, (B, S, H * D), ref.dtype, dev, "inputs")
+    width = H * D if norm == "rms_all_heads" else D
+    for name, p in (("q_weight", q_weight), ("q_bias", q_bias), ("k_weight", k_weight), ("k_bias", k_bias)):
+        if p is not None and (p.dtype != ref.dtype or not p.is_contiguous() or p.device != dev or p.numel() != width):
+            raise ValueError(f"{name} must be a contiguous {ref.dtype} tensor of {width} values on {dev}")
+    if (rope_cos is None) != (rope_sin is None):
+        raise ValueError("rope_cos and rope_sin go together")
+    lo, hi = (0, S) if rope_range is None else rope_range
+    if rope_cos is not None:
+        cols = D // 2 if rope_form == "pair" else D
+        for t in (rope_cos, rope_sin):
+            if t.dtype != torch.float32 or not t.is_contiguous() or t.shape != (hi - lo, cols) or t.device != dev:
+                raise ValueError(f"rotary tables must be contiguous float32 ({hi - lo}, {cols}) tensors on {dev}")
+    if out is None:
+        out = tuple(None if g is None else torch.empty(B, S, H * D, device=dev, dtype=ref.dtype) for g in grads)
+    stores = [o for o, g in zip(out, grads) if g is not None]
+    if any(o is None for o in stores):
+        raise ValueError("every gradient given needs an output buffer")
+    out_stride = _token_stride(stores, (B, S, H * D), ref.dtype, dev, "output buffers")
+    params = {"q_weight": q_weight if dq is not None else None, "k_weight": k_weight if dk is not None else None,
+              "q_bias": q_bias if dq is not None else None, "k_bias": k_bias if dk is not None else None}
+    res = {name: None if p is None or not kind else torch.empty_like(p) for name, p in params.items()}
+    ws = None
+    wsb = 0
+    if any(r is not None for r in res.values()):
+        wsb = lib.moddit_qkv_prologue_bwd_workspace_bytes(B, S, H, D, kind)
+        ws = torch.empty(wsb, device=dev, dtype=torch.uint8)
+    with torch.cuda.device(dev), _timed("moddit_qkv_prologue_bwd", dev):
+        check(lib.moddit_qkv_prologue_bwd(
+            _ptr(dq), _ptr(dk), _ptr(dv), _ptr(inputs[0]), _ptr(inputs[1]), dt, B, S, H, D, stride, kind, _ptr(q_weight),
+            _ptr(k_weight), float(eps), _ptr(rope_cos), _ptr(rope_sin), _lib.ROPE_FORM[rope_form], lo, hi, N, int(src_row0),
+            _ptr(out[0] if dq is not None else None), _ptr(out[1] if dk is not None else None),
+            _ptr(out[2] if dv is not None else None), out_stride, _ptr(res["q_weight"]), _ptr(res["q_bias"]),
+            _ptr(res["k_weight"]), _ptr(res["k_bias"]), _ptr(ws), wsb, _stream(dev)), "moddit_qkv_prologue_bwd")
+    return tuple(out), res
 
 
 def pooled_map(qbar: torch.Tensor, kbar: torch.Tensor, *, q_block_offset: int, k_block_offset: int,
@@ -666,6 +756,29 @@ def tile_lists(mask: torch.Tensor, block_size: int, n_tokens: int, kv_block_limi
     return TileLists(counts, entries, order)
 
 
+class KeyLists(TileLists):
+    """(counts, entries, order) produced by `key_lists`."""
+
+
+def key_lists(mask: torch.Tensor, block_size: int, n_tokens: int, kv_block_limit: Optional[int] = None) -> KeyLists:
+    """Work lists of the backward pass for a bool (H, nbq, nbk) block mask: for every key tile the query tiles that
+    attend to it, plus the start order of the (head, key tile) work items (long lists first)."""
+    dev = _need_cuda(mask)
+    if mask.dtype != torch.bool or mask.dim() != 3:
+        raise ValueError("mask must be a bool (H, nbq, nbk) tensor")
+    mask = mask.contiguous()
+    Hm, nbq, nbk = mask.shape
+    nt = (n_tokens + 127) // 128
+    counts = torch.empty(Hm, nt, device=dev, dtype=torch.int32)
+    entries = torch.empty(Hm, nt, nt, device=dev, dtype=torch.int32)
+    order = torch.empty(Hm, nt, device=dev, dtype=torch.int32)
+    lim = nbk if kv_block_limit is None else int(kv_block_limit)
+    with torch.cuda.device(dev), _timed("moddit_key_lists", dev):
+        check(lib.moddit_key_lists(_ptr(mask), Hm, nbq, nbk, block_size, n_tokens, lim, _ptr(counts), _ptr(entries),
+                                   _ptr(order), _stream(dev)), "moddit_key_lists")
+    return KeyLists(counts, entries, order)
+
+
 def predict_lines(q: torch.Tensor, k: torch.Tensor, block_size: int, *, first: int, n: int, blocks_per_frame: int,
                   model_type: str, last: Dict[str, torch.Tensor], top_k: int, predict_T: float, threshold: float = 1.0):
     """The mask prediction of a step in one call (`moddit_predict_lines`): block means of (1,H,N,D) q and k, pooled map,
@@ -771,7 +884,7 @@ def _status_words(dev: torch.device) -> torch.Tensor:
 
 def _status_error(vals) -> "_lib.ModditError":
     return _lib.ModditError(
-        f"sparse_attn_fwd: a bounded wait expired inside the kernel (code={vals[0]} block={vals[1]} "
+        f"sparse attention: a bounded wait expired inside the kernel (code={vals[0]} block={vals[1]} "
         f"role={vals[2]} position={vals[3]}); the output is invalid")
 
 
@@ -887,3 +1000,55 @@ def sparse_attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, counts: t
             check(lib.moddit_sparse_attn_fwd(*args, _ptr(out), _ptr(lse), _ptr(st), _stream(dev)), "moddit_sparse_attn_fwd")
     _after_launch(dev, check_status)
     return (out, lse) if return_lse else out
+
+
+# ---------------------------------------------------------------------------------------------
+# sparse backward
+# ---------------------------------------------------------------------------------------------
+
+def _need_lists(lists, rows: int, tiles: int, dev: torch.device, what: str) -> None:
+    Hm = lists.counts.shape[0]
+    for t, shape in ((lists.counts, (Hm, rows)), (lists.entries, (Hm, rows, tiles)), (lists.order, (Hm, rows))):
+        if t.dtype != torch.int32 or tuple(t.shape) != shape or t.device != dev or not t.is_contiguous():
+            raise ValueError(f"the work lists do not match the sequence length and device (see {what})")
+
+
+def sparse_attn_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+                    lse: torch.Tensor, lists: TileLists, key_lists: KeyLists, *, softmax_scale: Optional[float] = None,
+                    q_split: Optional[int] = None, kv_len_lo: Optional[int] = None, kv_len_hi: Optional[int] = None,
+                    check_status=True) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Gradients (dq, dk, dv) of `sparse_attn_fwd` from the gradient `dout` of its output.
+
+    q, k, v, the limits and the scale are the forward's, `out` and `lse` what it returned (`return_lse=True`), `lists`
+    and `key_lists` the results of `tile_lists` and `key_lists` for its mask.  The probabilities are computed again tile
+    by tile; the results are the same bits on every run.  check_status: as in `sparse_attn_fwd`."""
+    dev = _need_cuda(dout, q, k, v, out, lse)
+    if q.dim() != 4:
+        raise ValueError("query, key, value, output and its gradient must be (B, H, N, D) tensors")
+    dt = _qkv_dtype(q)
+    for t in (k, v, out, dout):
+        if t.shape != q.shape or t.dtype != q.dtype:
+            raise ValueError("query, key, value, output and its gradient must have identical shapes and dtypes")
+    B, H, N, D = q.shape
+    if tuple(lse.shape) != (B, H, N) or lse.dtype != torch.float32:
+        raise ValueError("lse must be the float32 (B, H, N) tensor that the forward returned")
+    _need_contig(dout=dout, q=q, k=k, v=v, out=out, lse=lse)
+    nt = (N + 127) // 128
+    _need_lists(lists, (nt + 1) // 2, nt, dev, "tile_lists")
+    _need_lists(key_lists, nt, nt, dev, "key_lists")
+    Hm = lists.counts.shape[0]
+    if key_lists.counts.shape[0] != Hm:
+        raise ValueError("tile_lists and key_lists must come from one mask")
+    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    wsb = lib.moddit_sparse_attn_bwd_workspace_bytes(B * H, N)
+    ws = torch.empty(max(wsb, 16), device=dev, dtype=torch.uint8)
+    st = _status_words(dev)
+    with torch.cuda.device(dev), _timed("moddit_sparse_attn_bwd", dev):
+        check(lib.moddit_sparse_attn_bwd(
+            _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(dout), _ptr(lse), dt, B * H, N, D, _ptr(lists.counts),
+            _ptr(lists.entries), _ptr(lists.order), _ptr(key_lists.counts), _ptr(key_lists.entries), _ptr(key_lists.order),
+            Hm, float(D ** -0.5 if softmax_scale is None else softmax_scale), N if q_split is None else int(q_split),
+            N if kv_len_lo is None else int(kv_len_lo), N if kv_len_hi is None else int(kv_len_hi), _ptr(dq), _ptr(dk),
+            _ptr(dv), _ptr(ws), wsb, _ptr(st), _stream(dev)), "moddit_sparse_attn_bwd")
+    _after_launch(dev, check_status)
+    return dq, dk, dv
