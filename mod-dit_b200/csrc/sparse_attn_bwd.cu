@@ -38,51 +38,89 @@ namespace moddit {
 namespace {
 
 constexpr int kThreads = 384;
-constexpr int kTile = 128;
-constexpr int kStages = 2;
+constexpr int kTile = 128;             // rows of a work item
+constexpr int kBlock = 64;             // streamed rows that are kept or left out together
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kHalfShift = 8.f;      // float16: P is held 2^kHalfShift times larger
+constexpr int kLongKeys = 2, kLongQueries = 4;      // items of every head that start first (the order lists put long ones there)
 
-enum BarrierIndex {
-  kFixed = 0,                         // F0, F1 have landed
-  kFull,                              // [kStages] X0, X1 (and the row statistics of a key item) have landed
-  kEmpty = kFull + kStages,           // [kStages] all products of an entry are done
-  kSFull = kEmpty + kStages,          // scores are ready
-  kDPFull,                            // dP is ready
-  kPDone,                             // S has been read and P stored
-  kDSDone,                            // dP has been read and dS stored
-  kFinal,
-  kNumBarriers
+struct Lists {
+  const int32_t *counts, *entries, *order;
 };
-
-struct __align__(16) Control {
-  float stats[kStages][2][kTile];     // key items: -lse * log2 e and -delta of the streamed query rows
-  unsigned long long bars[kNumBarriers];
-  uint32_t tmem_base;
-  int abort_flag;
-};
-
-template <int D>
-constexpr size_t smem_bytes() {
-  return static_cast<size_t>(2 + 2 * kStages) * kTile * D * 2 + 1024 + sizeof(Control);
-}
 
 struct BwdArgs {
-  const int32_t* counts;
-  const int32_t* entries;
-  const int32_t* order;
+  Lists key_lists, query_lists;       // of the key items (by key tile) and of the query items (by pair of query tiles)
+  const void *q, *k, *v, *dout;
   const float* nlse;                  // (BH, npad): -lse * log2 e (+ kHalfShift), -inf for rows that attend to nothing
   const float* ndelta;                // (BH, npad): -delta (* 2^-kHalfShift)
-  void* g0;                           // dK or dQ
-  void* g1;                           // dV
+  void *dq, *dk, *dv;
   int32_t* status;
-  int Hm, N, ntiles, npad, q_split, kvl_lo, kvl_hi;
+  int Hm, batches, N, ntiles, npad, q_split, kvl_lo, kvl_hi;
   float scale, scale_log2;
+};
+
+// Which work item a block has: `keys`, position in the kind's start order and batch.  The longest items of every head and
+// batch come first, then batch after batch the key items and the (shorter) query items.
+struct Item {
+  bool keys;
+  int pos, batch;
+};
+__device__ __forceinline__ Item item_of(const BwdArgs& a) {
+  const int n_keys = a.ntiles * a.Hm, n_queries = (a.ntiles + (a.ntiles & 1)) * a.Hm;
+  const int lk = min(n_keys, kLongKeys * a.Hm), lq = min(n_queries, kLongQueries * a.Hm);
+  const int first = (lk + lq) * a.batches;
+  int b = static_cast<int>(blockIdx.x);
+  Item it;
+  if (b < first) {
+    const int p = b / a.batches;
+    it.batch = b - p * a.batches;
+    it.keys = p < lk;
+    it.pos = it.keys ? p : p - lk;
+  } else {
+    b -= first;
+    const int rest = n_keys - lk + n_queries - lq;
+    it.batch = b / rest;
+    const int p = b - it.batch * rest;
+    it.keys = p < n_keys - lk;
+    it.pos = it.keys ? lk + p : lq + p - (n_keys - lk);
+  }
+  return it;
+}
+
+// The streamed 64-row blocks of a work item in list order, with the halves of the item's rows that keep each.
+// An entry of a list names a streamed tile of 128 rows and its kept quarters; blocks past `limit` are left out.
+template <bool kKeys>
+struct Walk {
+  const int32_t* ent;
+  int left, shift, limit;
+  int en, next_en, half;
+  int x0, bits;                       // first row of the block, bit i: rows [64 i, 64 i + 64) of the item keep it
+  __device__ __forceinline__ Walk(const int32_t* entries, int count, int flag_shift, int row_limit)
+      : ent(entries), left(count), shift(flag_shift), limit(row_limit), en(0), half(2), x0(0), bits(0) {
+    next_en = left > 0 ? __ldg(ent) : 0;
+  }
+  __device__ __forceinline__ bool next() {
+    while (true) {
+      if (half == 2) {
+        if (left == 0) return false;
+        en = next_en;
+        --left;
+        ++ent;
+        if (left > 0) next_en = __ldg(ent);
+        half = 0;
+      }
+      const int fl = en >> shift;
+      bits = kKeys ? (fl >> (2 * half)) & 3 : ((fl >> half) & 1) | ((fl >> (1 + half)) & 2);
+      x0 = (en >> 8) * kTile + kBlock * half;
+      ++half;
+      if (bits != 0 && x0 < limit) return true;
+    }
+  }
 };
 
 __device__ __forceinline__ void report(int32_t* status, int code, int role, int where) {
   if (atomicCAS(status, 0, code) == 0) {
-    status[1] = static_cast<int32_t>(blockIdx.y * gridDim.x + blockIdx.x);
+    status[1] = static_cast<int32_t>(blockIdx.x);
     status[2] = role;
     status[3] = where;
   }
@@ -96,6 +134,700 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   } else {
     const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+
+// dP - delta for a pair of values (float16: both 2^-kHalfShift times, which undoes the factor that P carries)
+template <bool kBF16>
+__device__ __forceinline__ uint64_t minus_delta(uint64_t dp, uint64_t nd) {
+  if constexpr (kBF16) return ptx::add_f32x2(dp, nd);
+  const float down = 1.f / 256.f;
+  return ptx::fma_f32x2(dp, ptx::pack_f32x2(down, down), nd);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Elementwise work on one 64-column block: P = 2^(S scale + nlse) and dS = P (dP - delta).
+//
+// Query items: a thread has one row and all 64 columns, so the row's statistics are two registers.
+template <bool kBF16>
+struct QueryRows {
+  float p[64];
+  __device__ __forceinline__ void load(uint32_t tS) {
+    ptx::tmem_ld32(tS, reinterpret_cast<uint32_t*>(p));
+    ptx::tmem_ld32(tS + 32, reinterpret_cast<uint32_t*>(p) + 32);
+    ptx::tmem_ld_wait();
+  }
+  __device__ __forceinline__ void probabilities(uint64_t scale2, float nl, int below) {      // columns >= below are masked
+    const uint64_t nl2 = ptx::pack_f32x2(nl, nl);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      float x0, x1;
+      ptx::unpack_f32x2(ptx::fma_f32x2(ptx::pack_f32x2(p[2 * i], p[2 * i + 1]), scale2, nl2), x0, x1);
+      p[2 * i] = ptx::ex2(x0);
+      p[2 * i + 1] = ptx::ex2(x1);
+    }
+    if (__any_sync(0xffffffffu, below < kBlock)) {
+#pragma unroll
+      for (int c = 0; c < 64; ++c) p[c] = c < below ? p[c] : 0.f;
+    }
+  }
+  // reads dP, stores dS over it
+  __device__ __forceinline__ void scores_gradient(uint32_t tP, float nd, int below) {
+    const uint64_t nd2 = ptx::pack_f32x2(nd, nd);
+    const bool masked = __any_sync(0xffffffffu, below < kBlock);
+    float d[64];
+    ptx::tmem_ld32(tP, reinterpret_cast<uint32_t*>(d));
+    ptx::tmem_ld32(tP + 32, reinterpret_cast<uint32_t*>(d) + 32);
+    ptx::tmem_ld_wait();
+    if (masked) {                     // what lies in a masked place may be anything
+#pragma unroll
+      for (int c = 0; c < 64; ++c) d[c] = c < below ? d[c] : 0.f;
+    }
+    uint32_t pk[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const uint64_t t = ptx::mul_f32x2(minus_delta<kBF16>(ptx::pack_f32x2(d[2 * i], d[2 * i + 1]), nd2),
+                                        ptx::pack_f32x2(p[2 * i], p[2 * i + 1]));
+      float y0, y1;
+      ptx::unpack_f32x2(t, y0, y1);
+      pk[i] = pack2<kBF16>(y0, y1);
+    }
+    ptx::tmem_st32(tP, pk);
+  }
+};
+
+// Key items: columns are queries, so every column has statistics of its own.  A thread has four rows and sixteen columns
+// (fragments of tcgen05.ld.16x256b): it reads 16 column statistics from shared memory for 64 values.  With one row and 64
+// columns a thread it would read all 64, a warp-wide shared-memory access each - as many cycles of the shared memory as the
+// products of a tile take from it.
+template <bool kBF16>
+struct KeyRows {
+  float p[2][32];
+  // which places are masked: rows by `lo`, `hi` (bit j: row i / 4 + 8 j may see queries before / from `split` on)
+  struct Mask {
+    bool on;
+    int split, lo, hi;
+  };
+  __device__ __forceinline__ bool kept(const Mask& m, int lh, int g, int i) const {
+    const int c = 8 * g + 2 * (threadIdx.x % 4) + (i & 1), row = 2 * lh + (i >> 1);
+    return (((c < m.split) ? m.lo : m.hi) >> row) & 1;
+  }
+  __device__ __forceinline__ void load(uint32_t tS) {
+    ptx::tmem_ld_16x64(tS, reinterpret_cast<uint32_t*>(p[0]));
+    ptx::tmem_ld_16x64(tS + (16u << 16), reinterpret_cast<uint32_t*>(p[1]));
+    ptx::tmem_ld_wait();
+  }
+  // column groups [4 part, 4 part + 4): computes P and stores it over the first columns of S
+  __device__ __forceinline__ void probabilities(int part, uint32_t tS, uint64_t scale2, const float* nl, const Mask& m) {
+    uint32_t pk[2][8];
+#pragma unroll
+    for (int gg = 0; gg < 4; ++gg) {
+      const int g = 4 * part + gg;
+      const uint64_t nl2 = *reinterpret_cast<const uint64_t*>(nl + 8 * g + 2 * (threadIdx.x % 4));
+#pragma unroll
+      for (int lh = 0; lh < 2; ++lh)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float* v = p[lh] + 4 * g + 2 * j;
+          float x0, x1;
+          ptx::unpack_f32x2(ptx::fma_f32x2(ptx::pack_f32x2(v[0], v[1]), scale2, nl2), x0, x1);
+          v[0] = ptx::ex2(x0);
+          v[1] = ptx::ex2(x1);
+          if (m.on) {
+            v[0] = kept(m, lh, g, 2 * j) ? v[0] : 0.f;
+            v[1] = kept(m, lh, g, 2 * j + 1) ? v[1] : 0.f;
+          }
+          pk[lh][2 * gg + j] = pack2<kBF16>(v[0], v[1]);
+        }
+    }
+    ptx::tmem_st_16x4g(tS + 16 * part, pk[0]);
+    ptx::tmem_st_16x4g(tS + (16u << 16) + 16 * part, pk[1]);
+  }
+  __device__ __forceinline__ void scores_gradient(uint32_t tP, const float* nd, const Mask& m) {
+    float d[2][32];
+    ptx::tmem_ld_16x64(tP, reinterpret_cast<uint32_t*>(d[0]));
+    ptx::tmem_ld_16x64(tP + (16u << 16), reinterpret_cast<uint32_t*>(d[1]));
+    ptx::tmem_ld_wait();
+    uint32_t pk[2][16];
+#pragma unroll
+    for (int g = 0; g < 8; ++g) {
+      const uint64_t nd2 = *reinterpret_cast<const uint64_t*>(nd + 8 * g + 2 * (threadIdx.x % 4));
+#pragma unroll
+      for (int lh = 0; lh < 2; ++lh)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float* v = d[lh] + 4 * g + 2 * j;
+          if (m.on) {                 // what lies in a masked place may be anything
+            v[0] = kept(m, lh, g, 2 * j) ? v[0] : 0.f;
+            v[1] = kept(m, lh, g, 2 * j + 1) ? v[1] : 0.f;
+          }
+          const uint64_t t = ptx::mul_f32x2(minus_delta<kBF16>(ptx::pack_f32x2(v[0], v[1]), nd2),
+                                            ptx::pack_f32x2(p[lh][4 * g + 2 * j], p[lh][4 * g + 2 * j + 1]));
+          float y0, y1;
+          ptx::unpack_f32x2(t, y0, y1);
+          pk[lh][2 * g + j] = pack2<kBF16>(y0, y1);
+        }
+    }
+    ptx::tmem_st_16x8g(tP, pk[0]);
+    ptx::tmem_st_16x8g(tP + (16u << 16), pk[1]);
+  }
+};
+
+// 32 packed columns of zeros (P or dS of rows that keep nothing of a block)
+__device__ __forceinline__ void store_zeros(uint32_t t) {
+  uint32_t z[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) z[i] = 0u;
+  ptx::tmem_st32(t, z);
+}
+
+__device__ __forceinline__ void hand_over(uint32_t bar) {
+  ptx::tmem_st_wait();
+  ptx::tc_fence_before();
+  ptx::mbar_arrive(bar);
+}
+
+// kCols accumulator columns of this thread's row, times f, as 16-bit values to dst; zeros where nothing was accumulated
+template <bool kBF16, int kCols>
+__device__ __forceinline__ void store_rows(uint32_t t, bool any, bool in, float f, uint4* dst) {
+#pragma unroll
+  for (int c = 0; c < kCols / 32; ++c) {
+    float o[32];
+    if (any) {
+      ptx::tmem_ld32(t + c * 32, reinterpret_cast<uint32_t*>(o));
+      ptx::tmem_ld_wait();
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) o[i] = 0.f;
+    }
+    if (in) {
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) {
+        uint4 w;
+        w.x = pack2<kBF16>(o[q4 * 8 + 0] * f, o[q4 * 8 + 1] * f);
+        w.y = pack2<kBF16>(o[q4 * 8 + 2] * f, o[q4 * 8 + 3] * f);
+        w.z = pack2<kBF16>(o[q4 * 8 + 4] * f, o[q4 * 8 + 5] * f);
+        w.w = pack2<kBF16>(o[q4 * 8 + 6] * f, o[q4 * 8 + 7] * f);
+        dst[c * 4 + q4] = w;
+      }
+    }
+  }
+}
+
+struct Block {                        // what all roles of a block know
+  unsigned char* smem;                // 1024-byte aligned
+  uint32_t tmem;
+  volatile int* abort_flag;
+  uint32_t bar0;
+  int row0, bh, count, shift, limit;
+  const int32_t* ent;
+  __device__ __forceinline__ uint32_t bar(int i) const { return bar0 + 8u * static_cast<uint32_t>(i); }
+  template <bool kKeys>
+  __device__ __forceinline__ Walk<kKeys> walk() const { return Walk<kKeys>(ent, count, shift, limit); }
+};
+
+__device__ __forceinline__ uint64_t advance(uint64_t desc, uint32_t bytes) {
+  // the start-address field (bits 0-13, units of 16 bytes) never carries out for shared-memory addresses
+  return (desc & 0xffffffff00000000ull) | static_cast<uint32_t>(static_cast<uint32_t>(desc) + (bytes >> 4));
+}
+
+constexpr int kMaxStages = 8;
+constexpr int kNumBarriers = 2 * kMaxStages + 10;
+struct __align__(16) Control {
+  float stats[kMaxStages][2][kBlock]; // key items: -lse * log2 e and -delta of the streamed query rows
+  unsigned long long bars[kNumBarriers];
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+// bytes of tiles in shared memory; behind them the control block, before them up to 1024 bytes of alignment
+template <int D>
+constexpr size_t kTilesBytes = static_cast<size_t>(D == 128 ? 192 : 128) * 1024;
+
+// ---------------------------------------------------------------------------------------------------------------
+// Two chains: warpgroup c takes the streamed blocks c, c + 2, c + 4, ... through scores, dP and dS of its own, half a step
+// behind the other one, so that one has exponentials to do while the other one waits or packs.  The fixed tiles live in
+// tensor memory as A operands, which halves what the products read from shared memory.
+// Tensor memory: S_c [64 c, 64 c + 64), dP_c 128 + the same, acc0 [256, 256 + D), acc1 behind it (D = 64), F0, F1 from 384 on.
+template <int D, bool kBF16, bool kKeys>
+struct Chains {
+  static constexpr int kStages = D == 128 ? 6 : 8;
+  static constexpr int kBlockBytes = kBlock * D * 2;
+  static constexpr int kChunks = D / 64;
+  static constexpr int kChunkBytes = kBlock * 128;
+  static constexpr int kAcc0 = 256, kAcc1 = 320, kF = 384;
+  static_assert(!kKeys || D == 64, "tensor memory holds two accumulators and the fixed tiles at D = 64 only");
+  enum { kFixed = 0, kSFull = 1, kDPFull = 3, kPDone = 5, kDSDone = 7, kFinal = 9, kFull = 10, kEmpty = kFull + kStages };
+
+  static __device__ __forceinline__ int arrivals(int i) {
+    return i == kFixed ? 256 : (i >= kPDone && i < kFinal) ? 128 : 1;
+  }
+
+  static __device__ __forceinline__ void produce(const Block& b, const BwdArgs& a, const Control* ctl, const CUtensorMap* tx0,
+                                                 const CUtensorMap* tx1) {
+    auto w = b.walk<kKeys>();
+    const uint32_t sX = ptx::smem_u32(b.smem);
+    bool ok = true;
+    int k = 0;
+    for (; w.next(); ++k) {
+      const int s = k % kStages;
+      ok = ptx::mbar_wait(b.bar(kEmpty + s), ((k / kStages) & 1) ^ 1, b.abort_flag);
+      if (!ok) { report(a.status, 1, 0, k); break; }
+      const uint32_t to = sX + 2 * s * kBlockBytes;
+      ptx::mbar_expect_tx(b.bar(kFull + s), 2 * kBlockBytes + (kKeys ? 2 * kBlock * 4 : 0));
+      for (int c = 0; c < kChunks; ++c) {
+        ptx::tma_load_3d(to + c * kChunkBytes, tx0, b.bar(kFull + s), c * 64, w.x0, b.bh);
+        ptx::tma_load_3d(to + kBlockBytes + c * kChunkBytes, tx1, b.bar(kFull + s), c * 64, w.x0, b.bh);
+      }
+      if (kKeys) {
+        const int64_t at = static_cast<int64_t>(b.bh) * a.npad + w.x0;
+        ptx::bulk_load(ptx::smem_u32(ctl->stats[s][0]), a.nlse + at, kBlock * 4, b.bar(kFull + s));
+        ptx::bulk_load(ptx::smem_u32(ctl->stats[s][1]), a.ndelta + at, kBlock * 4, b.bar(kFull + s));
+      }
+    }
+    if (!ok)        // give copies in flight a bounded time to land (their barriers may never be consumed)
+      for (int m = max(0, k - kStages); m < k; ++m)
+        for (int i = 0; i < 4096 && !ptx::mbar_try_wait(b.bar(kFull + m % kStages), (m / kStages) & 1); ++i) {}
+  }
+
+  static __device__ __forceinline__ void issue(const Block& b, const BwdArgs& a) {
+    constexpr uint32_t kIdescS = ptx::idesc_f16(128, kBlock, kBF16, false);
+    constexpr uint32_t kIdescG = ptx::idesc_f16(128, D, kBF16, true);
+    const uint32_t sX = ptx::smem_u32(b.smem);
+    const uint64_t dx = ptx::smem_desc_sw128(sX, 16, 1024);                // K-major
+    const uint64_t dg = ptx::smem_desc_sw128(sX, kChunkBytes, 1024);       // MN-major
+    // which = 0: S = F0 X0^T, 1: dP = F1 X1^T
+    auto first = [&](int which, int k) {
+      const int c = k & 1;
+      const uint64_t b0 = advance(dx, (2 * (k % kStages) + which) * kBlockBytes);
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk)
+        ptx::mma_ts(b.tmem + which * 128 + c * 64, b.tmem + kF + which * (D / 2) + kk * 8,
+                    advance(b0, (kk / 4) * kChunkBytes + (kk % 4) * 32), kIdescS, kk > 0 ? 1u : 0u);
+      ptx::tc_commit(b.bar((which ? kDPFull : kSFull) + c));
+    };
+    // which = 0: acc1 += P X1, 1: acc0 += dS X0
+    auto second = [&](int which, int k) {
+      const uint64_t b0 = advance(dg, (2 * (k % kStages) + 1 - which) * kBlockBytes);
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+        ptx::mma_ts(b.tmem + (which ? kAcc0 : kAcc1), b.tmem + which * 128 + (k & 1) * 64 + kk * 8, advance(b0, kk * 2048),
+                    kIdescG, (k > 0 || kk > 0) ? 1u : 0u);
+    };
+    auto landed = [&](int k) {
+      const bool ok = ptx::mbar_wait(b.bar(kFull + k % kStages), (k / kStages) & 1, b.abort_flag);
+      if (!ok) report(a.status, 2, 1, k);
+      ptx::tc_fence_after();
+      return ok;
+    };
+    auto w = b.walk<kKeys>();
+    int known = 0;                    // blocks found so far
+    bool more = true;
+    auto have = [&](int k) {          // whether there is a block k (asked in order)
+      if (more && known <= k) {
+        more = w.next();
+        known += more;
+      }
+      return k < known;
+    };
+    if (have(0)) {
+      bool ok = ptx::mbar_wait(b.bar(kFixed), 0, b.abort_flag);
+      if (!ok) report(a.status, 2, 1, -1);
+      ptx::tc_fence_after();
+      for (int k = 0; k < 2 && ok && have(k); ++k) {
+        ok = landed(k);
+        if (ok) { first(0, k); first(1, k); }
+      }
+      for (int k = 0; ok && k <= known; ++k) {
+        if (k < known) {
+          ok = ptx::mbar_wait(b.bar(kPDone + (k & 1)), (k >> 1) & 1, b.abort_flag);
+          if (!ok) { report(a.status, 3, 1, k); break; }
+          ptx::tc_fence_after();
+          if (kKeys) second(0, k);
+          if (have(k + 2)) {
+            ok = landed(k + 2);
+            if (!ok) break;
+            first(0, k + 2);
+          }
+        }
+        if (k > 0) {
+          ok = ptx::mbar_wait(b.bar(kDSDone + ((k - 1) & 1)), ((k - 1) >> 1) & 1, b.abort_flag);
+          if (!ok) { report(a.status, 4, 1, k); break; }
+          ptx::tc_fence_after();
+          second(1, k - 1);
+          ptx::tc_commit(b.bar(kEmpty + (k - 1) % kStages));
+          if (k + 1 < known && k + 1 >= 2) first(1, k + 1);
+        }
+      }
+    }
+    ptx::tc_commit(b.bar(kFinal));
+  }
+
+  // This thread's row of F0 (chain 0) or F1 (chain 1) into tensor memory; rows at and past `rows` are zero.
+  static __device__ __forceinline__ void load_fixed(const Block& b, const BwdArgs& a, const void* f, int c, uint32_t lane_base,
+                                                    int grow, int rows) {
+    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(f) +
+                                                      (static_cast<int64_t>(b.bh) * a.N + grow) * D * 2);
+#pragma unroll
+    for (int j = 0; j < D / 64; ++j) {
+      uint32_t v[32];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint4 x = grow < rows ? __ldg(src + 8 * j + i) : make_uint4(0, 0, 0, 0);
+        v[4 * i] = x.x; v[4 * i + 1] = x.y; v[4 * i + 2] = x.z; v[4 * i + 3] = x.w;
+      }
+      ptx::tmem_st32(b.tmem + lane_base + kF + c * (D / 2) + 32 * j, v);
+    }
+    hand_over(b.bar(kFixed));
+  }
+
+  static __device__ __forceinline__ void compute(const Block& b, const BwdArgs& a, const Control* ctl, int warp, int lane) {
+    const int c = (warp - 4) / 4;                 // chain
+    const int wq = warp % 4;                      // tensor-memory lane quarter
+    const int grow = b.row0 + wq * 32 + lane;
+    const uint32_t lane_base = static_cast<uint32_t>(wq * 32) << 16;
+    const uint32_t tS = b.tmem + lane_base + c * 64, tP = tS + 128;
+    const int kv_min = min(a.kvl_lo, a.kvl_hi), kv_max = max(a.kvl_lo, a.kvl_hi);
+    load_fixed(b, a, kKeys ? (c ? a.v : a.k) : (c ? a.dout : a.q), c, lane_base, grow, kKeys ? kv_max : a.N);
+    float nl = 0.f, nd = 0.f;
+    if (!kKeys) {
+      nl = a.nlse[static_cast<int64_t>(b.bh) * a.npad + grow];
+      nd = a.ndelta[static_cast<int64_t>(b.bh) * a.npad + grow];
+    }
+    const int lim = grow < a.q_split ? a.kvl_lo : a.kvl_hi;
+    int rows_lo = 0, rows_hi = 0;                 // key items: which of this thread's four rows lie below the limits
+    if (kKeys)
+      for (int j = 0; j < 4; ++j) {
+        const int key = b.row0 + wq * 32 + 8 * j + lane / 4;
+        rows_lo |= (key < a.kvl_lo) << j;
+        rows_hi |= (key < a.kvl_hi) << j;
+      }
+    const uint64_t scale2 = ptx::pack_f32x2(a.scale_log2, a.scale_log2);
+    auto w = b.walk<kKeys>();
+    bool ok = true;
+    int k = 0;
+    for (; w.next(); ++k) {
+      if ((k & 1) != c) continue;
+      const uint32_t par = (k >> 1) & 1;
+      const int s = k % kStages;
+      if (kKeys) ok = ptx::mbar_wait(b.bar(kFull + s), (k / kStages) & 1, b.abort_flag);      // the statistics
+      ok = ok && ptx::mbar_wait(b.bar(kSFull + c), par, b.abort_flag);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) { if (lane == 0) report(a.status, 5, 2 + c, k); break; }
+      ptx::tc_fence_after();
+      const bool mine = (w.bits >> (wq >> 1)) & 1;
+      if (!mine) {                                // these rows keep nothing of the block
+        if (kKeys) store_zeros(tS);
+        hand_over(b.bar(kPDone + c));
+        ok = __all_sync(0xffffffffu, ptx::mbar_wait(b.bar(kDPFull + c), par, b.abort_flag));
+        if (!ok) { if (lane == 0) report(a.status, 6, 2 + c, k); break; }
+        ptx::tc_fence_after();
+        store_zeros(tP);
+        hand_over(b.bar(kDSDone + c));
+        continue;
+      }
+      if constexpr (kKeys) {
+        KeyRows<kBF16> x;
+        const typename KeyRows<kBF16>::Mask m{b.row0 + kTile > kv_min, a.q_split - w.x0, rows_lo, rows_hi};
+        x.load(tS);
+        x.probabilities(0, tS, scale2, ctl->stats[s][0], m);
+        x.probabilities(1, tS, scale2, ctl->stats[s][0], m);
+        hand_over(b.bar(kPDone + c));
+        ok = __all_sync(0xffffffffu, ptx::mbar_wait(b.bar(kDPFull + c), par, b.abort_flag));
+        if (!ok) { if (lane == 0) report(a.status, 6, 2 + c, k); break; }
+        ptx::tc_fence_after();
+        x.scores_gradient(tP, ctl->stats[s][1], m);
+      } else {
+        QueryRows<kBF16> x;
+        const int below = lim - w.x0;
+        x.load(tS);
+        ptx::tc_fence_before();
+        ptx::mbar_arrive(b.bar(kPDone + c));      // P stays in registers: the next scores may overwrite these
+        x.probabilities(scale2, nl, below);
+        ok = __all_sync(0xffffffffu, ptx::mbar_wait(b.bar(kDPFull + c), par, b.abort_flag));
+        if (!ok) { if (lane == 0) report(a.status, 6, 2 + c, k); break; }
+        ptx::tc_fence_after();
+        x.scores_gradient(tP, nd, below);
+      }
+      hand_over(b.bar(kDSDone + c));
+    }
+    if (ok) {
+      ok = __all_sync(0xffffffffu, ptx::mbar_wait(b.bar(kFinal), 0, b.abort_flag));
+      if (!ok && lane == 0) report(a.status, 7, 2 + c, -1);
+    }
+    if (!ok) return;
+    ptx::tc_fence_after();
+    const int64_t at = (static_cast<int64_t>(b.bh) * a.N + grow) * D * 2;
+    auto to = [&](void* g) { return reinterpret_cast<uint4*>(static_cast<unsigned char*>(g) + at) + c * (D / 16); };
+    const bool in = grow < a.N;
+    const uint32_t t = b.tmem + lane_base + c * (D / 2);
+    store_rows<kBF16, D / 2>(t + kAcc0, k > 0, in, a.scale, to(kKeys ? a.dk : a.dq));
+    if (kKeys) store_rows<kBF16, D / 2>(t + kAcc1, k > 0, in, kBF16 ? 1.f : exp2f(-kHalfShift), to(a.dv));
+  }
+};
+
+// ---------------------------------------------------------------------------------------------------------------
+// Key items at D = 128: the four 128-column regions fill tensor memory, so the fixed tiles stay in shared memory and both
+// warpgroups work on one pair of streamed blocks.  A product with both operands in shared memory reads it at its full rate,
+// and at N = 64 it would take 52 clocks of the pipe for 32 of work: hence 128 columns at a time.
+// Tensor memory: S [0, 128) dP [128, 256) acc0 [256, 384) acc1 [384, 512).
+template <bool kBF16>
+struct Pairs {
+  static constexpr int D = 128;
+  static constexpr int kStages = 2;
+  static constexpr int kTileBytes = kTile * D * 2;
+  static constexpr int kChunkBytes = kTile * 128;
+  static constexpr int kHalfBytes = kBlock * 128;       // a block's rows of one 64-element chunk
+  enum { kFixed = 0, kSFull, kDPFull, kPLo, kPHi, kDSDone, kFinal, kFull, kEmpty = kFull + kStages, kUsed = kEmpty + kStages };
+
+  static __device__ __forceinline__ int arrivals(int i) { return (i >= kPLo && i <= kDSDone) ? 256 : 1; }
+
+  static __device__ __forceinline__ void produce(const Block& b, const BwdArgs& a, const Control* ctl, const CUtensorMap* tf0,
+                                                 const CUtensorMap* tf1, const CUtensorMap* tx0, const CUtensorMap* tx1) {
+    auto w = b.walk<true>();
+    const uint32_t sF = ptx::smem_u32(b.smem), sX = sF + 2 * kTileBytes;
+    bool more = w.next();
+    if (!more) return;
+    ptx::mbar_expect_tx(b.bar(kFixed), 2 * kTileBytes);
+    for (int c = 0; c < 2; ++c)
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t to = sF + c * kChunkBytes + h * kHalfBytes;
+        ptx::tma_load_3d(to, tf0, b.bar(kFixed), c * 64, b.row0 + h * kBlock, b.bh);
+        ptx::tma_load_3d(to + kTileBytes, tf1, b.bar(kFixed), c * 64, b.row0 + h * kBlock, b.bh);
+      }
+    bool ok = true;
+    int n = 0;
+    for (; more; ++n) {
+      const int s = n % kStages;
+      ok = ptx::mbar_wait(b.bar(kEmpty + s), ((n / kStages) & 1) ^ 1, b.abort_flag);
+      if (!ok) { report(a.status, 1, 0, n); break; }
+      ptx::mbar_expect_tx(b.bar(kFull + s), 2 * kTileBytes + 4 * kBlock * 4);
+      int x0 = w.x0;
+      for (int h = 0; h < 2; ++h) {
+        if (h == 1) {                 // an odd last block is there twice: its second copy is masked
+          more = w.next();
+          if (more) x0 = w.x0;
+        }
+        const uint32_t to = sX + 2 * s * kTileBytes + h * kHalfBytes;
+        for (int c = 0; c < 2; ++c) {
+          ptx::tma_load_3d(to + c * kChunkBytes, tx0, b.bar(kFull + s), c * 64, x0, b.bh);
+          ptx::tma_load_3d(to + kTileBytes + c * kChunkBytes, tx1, b.bar(kFull + s), c * 64, x0, b.bh);
+        }
+        const int64_t at = static_cast<int64_t>(b.bh) * a.npad + x0;
+        ptx::bulk_load(ptx::smem_u32(ctl->stats[2 * s + h][0]), a.nlse + at, kBlock * 4, b.bar(kFull + s));
+        ptx::bulk_load(ptx::smem_u32(ctl->stats[2 * s + h][1]), a.ndelta + at, kBlock * 4, b.bar(kFull + s));
+      }
+      if (more) more = w.next();
+    }
+    if (!ok) {
+      for (int i = 0; i < 4096 && !ptx::mbar_try_wait(b.bar(kFixed), 0); ++i) {}
+      for (int m = max(0, n - kStages); m < n; ++m)
+        for (int i = 0; i < 4096 && !ptx::mbar_try_wait(b.bar(kFull + m % kStages), (m / kStages) & 1); ++i) {}
+    }
+  }
+
+  static __device__ __forceinline__ void issue(const Block& b, const BwdArgs& a) {
+    constexpr uint32_t kIdescS = ptx::idesc_f16(128, 128, kBF16, false);
+    constexpr uint32_t kIdescG = ptx::idesc_f16(128, D, kBF16, true);
+    const uint32_t sF = ptx::smem_u32(b.smem), sX = sF + 2 * kTileBytes;
+    const uint64_t df = ptx::smem_desc_sw128(sF, 16, 1024);                // K-major: F0, F1 and the X tiles
+    const uint64_t dx = advance(df, sX - sF);
+    const uint64_t dg = ptx::smem_desc_sw128(sX, kChunkBytes, 1024);       // MN-major: the X tiles
+    auto first = [&](int which, int s) {
+      const uint64_t a0 = advance(df, which * kTileBytes), b0 = advance(dx, (2 * s + which) * kTileBytes);
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        const uint32_t off = (kk / 4) * kChunkBytes + (kk % 4) * 32;
+        ptx::mma_ss(b.tmem + which * 128, advance(a0, off), advance(b0, off), kIdescS, kk > 0 ? 1u : 0u);
+      }
+      ptx::tc_commit(b.bar(kSFull + which));
+    };
+    // acc += A X over 16-query steps: kk = 4 h + j has its A operand at 64 h + 8 j
+    auto second = [&](int which, int s, int kk, uint32_t acc) {
+      const uint64_t b0 = advance(dg, (2 * s + 1 - which) * kTileBytes);
+      ptx::mma_ts(b.tmem + (which ? 256 : 384), b.tmem + which * 128 + (kk / 4) * 64 + (kk % 4) * 8, advance(b0, kk * 2048),
+                  kIdescG, acc);
+    };
+    auto w = b.walk<true>();
+    bool next = w.next();
+    bool ok = true;
+    if (next) {
+      ok = ptx::mbar_wait(b.bar(kFixed), 0, b.abort_flag) && ptx::mbar_wait(b.bar(kFull), 0, b.abort_flag);
+      if (!ok) report(a.status, 2, 1, -1);
+      ptx::tc_fence_after();
+      if (ok) { first(0, 0); first(1, 0); }
+    }
+    for (int n = 0; next && ok; ++n) {
+      const int s = n % kStages, s1 = (n + 1) % kStages;
+      next = w.next() && w.next();              // whether there is a step n + 1
+      for (int part = 0; part < 2; ++part) {
+        ok = ptx::mbar_wait(b.bar(kPLo + part), n & 1, b.abort_flag);
+        if (!ok) { report(a.status, 3, 1, n); break; }
+        ptx::tc_fence_after();
+        second(0, s, 2 * part, (n > 0 || part > 0) ? 1u : 0u);
+        second(0, s, 2 * part + 1, 1u);
+        second(0, s, 2 * part + 4, 1u);
+        second(0, s, 2 * part + 5, 1u);
+      }
+      if (!ok) break;
+      if (next) {
+        ok = ptx::mbar_wait(b.bar(kFull + s1), ((n + 1) / kStages) & 1, b.abort_flag);
+        if (!ok) { report(a.status, 2, 1, n); break; }
+        ptx::tc_fence_after();
+        first(0, s1);
+      }
+      ok = ptx::mbar_wait(b.bar(kDSDone), n & 1, b.abort_flag);
+      if (!ok) { report(a.status, 4, 1, n); break; }
+      ptx::tc_fence_after();
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk) second(1, s, kk, (n > 0 || kk > 0) ? 1u : 0u);
+      ptx::tc_commit(b.bar(kEmpty + s));
+      if (next) first(1, s1);
+    }
+    ptx::tc_commit(b.bar(kFinal));
+  }
+
+  static __device__ __forceinline__ void compute(const Block& b, const BwdArgs& a, const Control* ctl, int warp, int lane) {
+    const int h = (warp - 4) / 4;                 // which of the two streamed blocks
+    const int wq = warp % 4;
+    const uint32_t lane_base = static_cast<uint32_t>(wq * 32) << 16;
+    const uint32_t tS = b.tmem + lane_base + h * 64, tP = tS + 128;
+    const int kv_min = min(a.kvl_lo, a.kvl_hi);
+    int rows_lo = 0, rows_hi = 0;
+    for (int j = 0; j < 4; ++j) {
+      const int key = b.row0 + wq * 32 + 8 * j + lane / 4;
+      rows_lo |= (key < a.kvl_lo) << j;
+      rows_hi |= (key < a.kvl_hi) << j;
+    }
+    const uint64_t scale2 = ptx::pack_f32x2(a.scale_log2, a.scale_log2);
+    auto w = b.walk<true>();
+    bool ok = true;
+    int n = 0;
+    for (bool more = w.next(); more; ++n) {
+      int x0 = w.x0, bits = w.bits;
+      more = w.next();
+      if (h == 1) {
+        x0 = w.x0;
+        bits = more ? w.bits : 0;
+      }
+      if (more) more = w.next();
+      const int s = n % kStages;
+      ok = ptx::mbar_wait(b.bar(kFull + s), (n / kStages) & 1, b.abort_flag) &&        // the statistics
+           ptx::mbar_wait(b.bar(kSFull), n & 1, b.abort_flag);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) { if (lane == 0) report(a.status, 5, 2 + h, n); break; }
+      ptx::tc_fence_after();
+      const bool mine = (bits >> (wq >> 1)) & 1;
+      KeyRows<kBF16> x;
+      const typename KeyRows<kBF16>::Mask m{b.row0 + kTile > kv_min, a.q_split - x0, rows_lo, rows_hi};
+      if (mine) {
+        x.load(tS);
+        x.probabilities(0, tS, scale2, ctl->stats[2 * s + h][0], m);
+        hand_over(b.bar(kPLo));
+        x.probabilities(1, tS, scale2, ctl->stats[2 * s + h][0], m);
+        hand_over(b.bar(kPHi));
+      } else {
+        store_zeros(tS);
+        hand_over(b.bar(kPLo));
+        ptx::mbar_arrive(b.bar(kPHi));
+      }
+      ok = __all_sync(0xffffffffu, ptx::mbar_wait(b.bar(kDPFull), n & 1, b.abort_flag));
+      if (!ok) { if (lane == 0) report(a.status, 6, 2 + h, n); break; }
+      ptx::tc_fence_after();
+      if (mine) x.scores_gradient(tP, ctl->stats[2 * s + h][1], m);
+      else store_zeros(tP);
+      hand_over(b.bar(kDSDone));
+    }
+    if (ok) {
+      ok = __all_sync(0xffffffffu, ptx::mbar_wait(b.bar(kFinal), 0, b.abort_flag));
+      if (!ok && lane == 0) report(a.status, 7, 2 + h, -1);
+    }
+    if (!ok) return;
+    ptx::tc_fence_after();
+    const int grow = b.row0 + wq * 32 + lane;
+    const int64_t at = (static_cast<int64_t>(b.bh) * a.N + grow) * D * 2;
+    auto to = [&](void* g) { return reinterpret_cast<uint4*>(static_cast<unsigned char*>(g) + at) + h * 8; };
+    const uint32_t t = b.tmem + lane_base + h * 64;
+    store_rows<kBF16, 64>(t + 256, n > 0, grow < a.N, a.scale, to(a.dk));
+    store_rows<kBF16, 64>(t + 384, n > 0, grow < a.N, kBF16 ? 1.f : exp2f(-kHalfShift), to(a.dv));
+  }
+};
+
+template <int D, bool kBF16>
+__global__ void __launch_bounds__(kThreads, 1) sparse_attn_bwd_kernel(
+    const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+    const __grid_constant__ CUtensorMap tm_do, const __grid_constant__ BwdArgs a) {
+  using Queries = Chains<D, kBF16, false>;
+  extern __shared__ unsigned char smem_raw[];
+  Block b;
+  b.smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Control* ctl = reinterpret_cast<Control*>(b.smem + kTilesBytes<D>);
+  b.bar0 = ptx::smem_u32(&ctl->bars[0]);
+  b.abort_flag = &ctl->abort_flag;
+
+  const int warp = ptx::warp_index();
+  const int lane = threadIdx.x % 32;
+  const Item it = item_of(a);
+  const Lists& l = it.keys ? a.key_lists : a.query_lists;
+  const int nlist = it.keys ? a.ntiles : (a.ntiles + 1) / 2;
+  const int index = it.keys ? it.pos : it.pos >> 1;
+  const int item = l.order ? __ldg(l.order + index) : index;
+  const int mh = item / nlist;
+  const int tile = it.keys ? item - mh * nlist : 2 * (item - mh * nlist) + (it.pos & 1);
+  if (tile >= a.ntiles) return;                   // the second query tile of a pair that has one only
+  const int kv_max = max(a.kvl_lo, a.kvl_hi);
+  b.bh = it.batch * a.Hm + mh;
+  b.row0 = tile * kTile;
+  b.shift = it.keys ? 0 : 4 * (it.pos & 1);
+  b.limit = it.keys ? a.N : kv_max;
+  b.count = (it.keys && b.row0 >= kv_max) ? 0 : __ldg(l.counts + item);
+  b.ent = l.entries + static_cast<int64_t>(item) * a.ntiles;
+
+  auto with_kind = [&](auto&& f) {
+    if (it.keys) {
+      if constexpr (D == 128) f(Pairs<kBF16>{});
+      else f(Chains<64, kBF16, true>{});
+    } else {
+      f(Queries{});
+    }
+  };
+  if (threadIdx.x == 0) {
+    with_kind([&](auto kind) {
+      for (int i = 0; i < kNumBarriers; ++i) ptx::mbar_init(b.bar(i), kind.arrivals(i));
+    });
+    ctl->abort_flag = 0;
+    ptx::fence_barrier_init();
+    ptx::prefetch_tensormap(&tm_q);
+    ptx::prefetch_tensormap(&tm_k);
+    ptx::prefetch_tensormap(&tm_v);
+    ptx::prefetch_tensormap(&tm_do);
+  }
+  if (warp == 2) {
+    ptx::tmem_alloc(ptx::smem_u32(&ctl->tmem_base), 512);
+    ptx::tmem_relinquish();
+    ptx::tc_fence_before();
+  }
+  __syncthreads();
+  ptx::tc_fence_after();
+  b.tmem = ctl->tmem_base;
+
+  if (warp == 0) {
+    if (ptx::elect_one()) {
+      if (!it.keys) Queries::produce(b, a, ctl, &tm_k, &tm_v);
+      else if constexpr (D == 128) Pairs<kBF16>::produce(b, a, ctl, &tm_k, &tm_v, &tm_q, &tm_do);
+      else Chains<64, kBF16, true>::produce(b, a, ctl, &tm_q, &tm_do);
+    }
+  } else if (warp == 1) {
+    if (ptx::elect_one()) with_kind([&](auto kind) { kind.issue(b, a); });
+  } else if (warp >= 4) {
+    with_kind([&](auto kind) { kind.compute(b, a, ctl, warp, lane); });
+  }
+
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (warp == 2) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(b.tmem, 512);
   }
 }
 
@@ -139,355 +871,24 @@ __global__ void __launch_bounds__(256) bwd_stats_kernel(const void* __restrict__
   }
 }
 
-template <int D, bool kBF16, bool kKeys>
-__global__ void __launch_bounds__(kThreads, 1) sparse_attn_bwd_kernel(
-    const __grid_constant__ CUtensorMap tm_f0, const __grid_constant__ CUtensorMap tm_f1,
-    const __grid_constant__ CUtensorMap tm_x0, const __grid_constant__ CUtensorMap tm_x1,
-    const __grid_constant__ BwdArgs a) {
-  constexpr int kTileBytes = kTile * D * 2;
-  constexpr int kChunks = D / 64;                 // 64-element (128-byte) column chunks per tile
-  constexpr int kChunkBytes = kTile * 128;
-  constexpr uint32_t kIdescS = ptx::idesc_f16(128, 128, kBF16, false);
-  constexpr uint32_t kIdescG = ptx::idesc_f16(128, D, kBF16, true);
-
-  extern __shared__ unsigned char smem_raw[];
-  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  Control* ctl = reinterpret_cast<Control*>(smem + (2 + 2 * kStages) * kTileBytes);
-  const uint32_t sF = ptx::smem_u32(smem);
-  const uint32_t sX = sF + 2 * kTileBytes;        // stage s: X0 at sX + 2 s tiles, X1 behind it
-  const uint32_t bar0 = ptx::smem_u32(&ctl->bars[0]);
-  auto bar = [&](int i) { return bar0 + 8u * static_cast<uint32_t>(i); };
-  volatile int* abort_flag = &ctl->abort_flag;
-
-  const int warp = ptx::warp_index();
-  const int lane = threadIdx.x % 32;
-  // work item: key items are listed by tile, query items by pair of tiles
-  const int nlist = kKeys ? a.ntiles : (a.ntiles + 1) / 2;
-  const int index = kKeys ? blockIdx.x : blockIdx.x >> 1;
-  const int item = a.order ? a.order[index] : index;
-  const int mh = item / nlist;
-  const int tile = kKeys ? item - mh * nlist : 2 * (item - mh * nlist) + (blockIdx.x & 1);
-  const int fshift = kKeys ? 0 : 4 * (blockIdx.x & 1);
-  if (tile >= a.ntiles) return;
-  const int bh = blockIdx.y * a.Hm + mh;
-  const int row0 = tile * kTile;
-  int cnt = a.counts[item];
-  if (kKeys && row0 >= max(a.kvl_lo, a.kvl_hi)) cnt = 0;
-  const int32_t* ent = a.entries + static_cast<int64_t>(item) * a.ntiles;
-
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < kNumBarriers; ++i) ptx::mbar_init(bar(i), (i == kPDone || i == kDSDone) ? 256u : 1u);
-    ctl->abort_flag = 0;
-    ptx::fence_barrier_init();
-    ptx::prefetch_tensormap(&tm_f0);
-    ptx::prefetch_tensormap(&tm_f1);
-    ptx::prefetch_tensormap(&tm_x0);
-    ptx::prefetch_tensormap(&tm_x1);
-  }
-  if (warp == 2) {
-    ptx::tmem_alloc(ptx::smem_u32(&ctl->tmem_base), 512);
-    ptx::tmem_relinquish();
-    ptx::tc_fence_before();
-  }
-  __syncthreads();
-  ptx::tc_fence_after();
-  const uint32_t tmem = ctl->tmem_base;
-  auto flags_of = [&](int en) { return (en >> fshift) & 0xf; };
-
-  if (warp == 0) {
-    // ------------------------------------------------------------------ TMA producer
-    if (ptx::elect_one() && cnt > 0) {
-      ptx::mbar_expect_tx(bar(kFixed), 2 * kTileBytes);
-      for (int c = 0; c < kChunks; ++c) {
-        ptx::tma_load_3d(sF + c * kChunkBytes, &tm_f0, bar(kFixed), c * 64, row0, bh);
-        ptx::tma_load_3d(sF + kTileBytes + c * kChunkBytes, &tm_f1, bar(kFixed), c * 64, row0, bh);
-      }
-      bool ok = true;
-      int n = 0;
-      for (int e = 0; e < cnt && ok; ++e) {
-        if (!flags_of(ent[e])) continue;
-        const int s = n % kStages;
-        ok = ptx::mbar_wait(bar(kEmpty + s), ((n / kStages) & 1) ^ 1, abort_flag);
-        if (!ok) { report(a.status, 1, 0, e); break; }
-        const int x0 = (ent[e] >> 8) * kTile;
-        const uint32_t to = sX + 2 * s * kTileBytes;
-        ptx::mbar_expect_tx(bar(kFull + s), 2 * kTileBytes + (kKeys ? 2 * kTile * 4 : 0));
-        for (int c = 0; c < kChunks; ++c) {
-          ptx::tma_load_3d(to + c * kChunkBytes, &tm_x0, bar(kFull + s), c * 64, x0, bh);
-          ptx::tma_load_3d(to + kTileBytes + c * kChunkBytes, &tm_x1, bar(kFull + s), c * 64, x0, bh);
-        }
-        if (kKeys) {
-          const int64_t at = static_cast<int64_t>(bh) * a.npad + x0;
-          ptx::bulk_load(ptx::smem_u32(ctl->stats[s][0]), a.nlse + at, kTile * 4, bar(kFull + s));
-          ptx::bulk_load(ptx::smem_u32(ctl->stats[s][1]), a.ndelta + at, kTile * 4, bar(kFull + s));
-        }
-        ++n;
-      }
-      if (!ok) {
-        // give copies in flight a bounded time to land (their barriers may never be consumed)
-        for (int i = 0; i < 4096 && !ptx::mbar_try_wait(bar(kFixed), 0); ++i) {}
-        for (int m = max(0, n - kStages); m < n; ++m)
-          for (int i = 0; i < 4096 && !ptx::mbar_try_wait(bar(kFull + m % kStages), (m / kStages) & 1); ++i) {}
-      }
-    }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------------ MMA issuer
-    if (ptx::elect_one()) {
-      auto advance = [](uint64_t desc, uint32_t bytes) -> uint64_t {
-        return (desc & 0xffffffff00000000ull) | static_cast<uint32_t>(static_cast<uint32_t>(desc) + (bytes >> 4));
-      };
-      const uint64_t df = ptx::smem_desc_sw128(sF, 16, 1024);              // K-major: F0, F1 and the X tiles
-      const uint64_t dx = advance(df, sX - sF);
-      const uint64_t dg = ptx::smem_desc_sw128(sX, kChunkBytes, 1024);     // MN-major: the X tiles
-      // which = 0: S = F0 X0^T, 1: dP = F1 X1^T
-      auto first = [&](int which, int s) {
-        const uint64_t a0 = advance(df, which * kTileBytes), b0 = advance(dx, (2 * s + which) * kTileBytes);
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (kk / 4) * kChunkBytes + (kk % 4) * 32;
-          ptx::mma_ss(tmem + which * 128, advance(a0, off), advance(b0, off), kIdescS, kk > 0 ? 1u : 0u);
-        }
-        ptx::tc_commit(bar(kSFull + which));
-      };
-      // which = 0: acc1 += P X1, 1: acc0 += dS X0
-      auto second = [&](int which, int s, uint32_t acc) {
-        const uint64_t b0 = advance(dg, (2 * s + 1 - which) * kTileBytes);
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-          ptx::mma_ts(tmem + (which ? 256 : 384), tmem + which * 128 + (kk / 4) * 64 + (kk % 4) * 8, advance(b0, kk * 2048),
-                      kIdescG, (acc || kk > 0) ? 1u : 0u);
-      };
-      bool ok = true;
-      int e = 0, n = 0;
-      auto next_kept = [&](int from) {
-        while (from < cnt && !flags_of(ent[from])) ++from;
-        return from;
-      };
-      e = next_kept(0);
-      if (e < cnt) {
-        ok = ptx::mbar_wait(bar(kFixed), 0, abort_flag) && ptx::mbar_wait(bar(kFull), 0, abort_flag);
-        if (!ok) report(a.status, 2, 1, -1);
-        ptx::tc_fence_after();
-        if (ok) { first(0, 0); first(1, 0); }
-      }
-      while (e < cnt && ok) {
-        const int s = n % kStages, s1 = (n + 1) % kStages;
-        const int e1 = next_kept(e + 1);
-        const bool next = e1 < cnt;
-        ok = ptx::mbar_wait(bar(kPDone), n & 1, abort_flag);
-        if (!ok) { report(a.status, 3, 1, e); break; }
-        ptx::tc_fence_after();
-        if (kKeys) second(0, s, n > 0);
-        if (next) {
-          ok = ptx::mbar_wait(bar(kFull + s1), ((n + 1) / kStages) & 1, abort_flag);
-          if (!ok) { report(a.status, 2, 1, e); break; }
-          ptx::tc_fence_after();
-          first(0, s1);
-        }
-        ok = ptx::mbar_wait(bar(kDSDone), n & 1, abort_flag);
-        if (!ok) { report(a.status, 3, 1, e); break; }
-        ptx::tc_fence_after();
-        second(1, s, n > 0);
-        ptx::tc_commit(bar(kEmpty + s));
-        if (next) first(1, s1);
-        e = e1;
-        ++n;
-      }
-      ptx::tc_commit(bar(kFinal));
-    }
-  } else if (warp >= 4) {
-    // ------------------------------------------------------------------ elementwise
-    const int h = (warp - 4) / 4;                 // column half
-    const int r = (warp % 4) * 32 + lane;         // row inside the tile
-    const int grow = row0 + r;
-    const uint32_t lane_base = static_cast<uint32_t>((warp % 4) * 32) << 16;
-    const uint32_t tS = tmem + lane_base + h * 64;
-    const uint32_t tP = tS + 128;
-    const int kv_min = min(a.kvl_lo, a.kvl_hi);
-    // bit of the sub-block that this thread's row and columns lie in
-    const int keep_bit = kKeys ? 2 * h + (r >> 6) : 2 * (r >> 6) + h;
-    float nl_row = 0.f, nd_row = 0.f;
-    if (!kKeys) {
-      nl_row = a.nlse[static_cast<int64_t>(bh) * a.npad + grow];
-      nd_row = a.ndelta[static_cast<int64_t>(bh) * a.npad + grow];
-    }
-    const uint64_t scale2 = ptx::pack_f32x2(a.scale_log2, a.scale_log2);
-    const uint64_t nl2 = ptx::pack_f32x2(nl_row, nl_row), nd2 = ptx::pack_f32x2(nd_row, nd_row);
-    const float kDown = kBF16 ? 1.f : 1.f / 256.f;
-    const uint64_t down2 = ptx::pack_f32x2(kDown, kDown);
-    bool ok = true;
-    int n = 0;
-    for (int e = 0; e < cnt; ++e) {
-      const int fl = flags_of(ent[e]);
-      if (!fl) continue;
-      const int s = n % kStages;
-      const int x0 = (ent[e] >> 8) * kTile;
-      // columns [0, keep_below) and [keep_from, 64) of this thread are kept
-      int keep_below = 64, keep_from = 64;
-      if (fl != 0xf || (kKeys ? row0 : x0) + kTile > kv_min) {
-        if (!((fl >> keep_bit) & 1)) {
-          keep_below = 0;
-        } else if (kKeys) {
-          const int split = min(max(a.q_split - x0 - 64 * h, 0), 64);
-          keep_below = grow < a.kvl_lo ? split : 0;
-          keep_from = grow < a.kvl_hi ? split : 64;
-        } else {
-          keep_below = (grow < a.q_split ? a.kvl_lo : a.kvl_hi) - x0 - 64 * h;
-        }
-      }
-      const bool whole = keep_below >= keep_from || keep_below >= 64;
-      const bool any_masked = __any_sync(0xffffffffu, !whole);
-      if (kKeys) ok = ptx::mbar_wait(bar(kFull + s), (n / kStages) & 1, abort_flag);      // the statistics
-      ok = ok && ptx::mbar_wait(bar(kSFull), n & 1, abort_flag);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) { if (lane == 0) report(a.status, 4, 2 + h, e); break; }
-      ptx::tc_fence_after();
-      float p[64];
-#pragma unroll
-      for (int c = 0; c < 2; ++c) ptx::tmem_ld32(tS + c * 32, reinterpret_cast<uint32_t*>(p) + c * 32);
-      ptx::tmem_ld_wait();
-      const ulonglong2* nlv = reinterpret_cast<const ulonglong2*>(ctl->stats[s][0] + 64 * h);
-      const ulonglong2* ndv = reinterpret_cast<const ulonglong2*>(ctl->stats[s][1] + 64 * h);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const ulonglong2 nl = kKeys ? nlv[i] : make_ulonglong2(nl2, nl2);
-        float x0f, x1f, x2f, x3f;
-        ptx::unpack_f32x2(ptx::fma_f32x2(ptx::pack_f32x2(p[4 * i], p[4 * i + 1]), scale2, nl.x), x0f, x1f);
-        ptx::unpack_f32x2(ptx::fma_f32x2(ptx::pack_f32x2(p[4 * i + 2], p[4 * i + 3]), scale2, nl.y), x2f, x3f);
-        p[4 * i] = ptx::ex2(x0f);
-        p[4 * i + 1] = ptx::ex2(x1f);
-        p[4 * i + 2] = ptx::ex2(x2f);
-        p[4 * i + 3] = ptx::ex2(x3f);
-      }
-      if (any_masked) {
-#pragma unroll
-        for (int c = 0; c < 64; ++c) p[c] = (c < keep_below || c >= keep_from) ? p[c] : 0.f;
-      }
-      if (kKeys) {
-        uint32_t pk[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) pk[i] = pack2<kBF16>(p[2 * i], p[2 * i + 1]);
-        ptx::tmem_st32(tS, pk);
-        ptx::tmem_st_wait();
-      }
-      ptx::tc_fence_before();
-      ptx::mbar_arrive(bar(kPDone));
-
-      ok = ptx::mbar_wait(bar(kDPFull), n & 1, abort_flag);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) { if (lane == 0) report(a.status, 5, 2 + h, e); break; }
-      ptx::tc_fence_after();
-      float d[64];
-#pragma unroll
-      for (int c = 0; c < 2; ++c) ptx::tmem_ld32(tP + c * 32, reinterpret_cast<uint32_t*>(d) + c * 32);
-      ptx::tmem_ld_wait();
-      if (any_masked) {                           // what lies in a masked place may be anything
-#pragma unroll
-        for (int c = 0; c < 64; ++c) d[c] = (c < keep_below || c >= keep_from) ? d[c] : 0.f;
-      }
-      uint32_t dk[32];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const ulonglong2 nd = kKeys ? ndv[i] : make_ulonglong2(nd2, nd2);
-        uint64_t t0 = ptx::pack_f32x2(d[4 * i], d[4 * i + 1]), t1 = ptx::pack_f32x2(d[4 * i + 2], d[4 * i + 3]);
-        t0 = kBF16 ? ptx::add_f32x2(t0, nd.x) : ptx::fma_f32x2(t0, down2, nd.x);
-        t1 = kBF16 ? ptx::add_f32x2(t1, nd.y) : ptx::fma_f32x2(t1, down2, nd.y);
-        t0 = ptx::mul_f32x2(t0, ptx::pack_f32x2(p[4 * i], p[4 * i + 1]));
-        t1 = ptx::mul_f32x2(t1, ptx::pack_f32x2(p[4 * i + 2], p[4 * i + 3]));
-        float y0, y1, y2, y3;
-        ptx::unpack_f32x2(t0, y0, y1);
-        ptx::unpack_f32x2(t1, y2, y3);
-        dk[2 * i] = pack2<kBF16>(y0, y1);
-        dk[2 * i + 1] = pack2<kBF16>(y2, y3);
-      }
-      ptx::tmem_st32(tP, dk);
-      ptx::tmem_st_wait();
-      ptx::tc_fence_before();
-      ptx::mbar_arrive(bar(kDSDone));
-      ++n;
-    }
-    if (ok) {
-      ok = ptx::mbar_wait(bar(kFinal), 0, abort_flag);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok && lane == 0) report(a.status, 6, 2 + h, -1);
-    }
-    if (ok) {
-      ptx::tc_fence_after();
-      const float g1_scale = kBF16 ? 1.f : exp2f(-kHalfShift);
-      // accumulator `which` of D columns: half h of the warps stores half of them
-#pragma unroll
-      for (int which = 0; which < (kKeys ? 2 : 1); ++which) {
-        const float f = which ? g1_scale : a.scale;
-        uint4* dst = reinterpret_cast<uint4*>(static_cast<unsigned char*>(which ? a.g1 : a.g0) +
-                                              (static_cast<int64_t>(bh) * a.N + grow) * D * 2) + h * (D / 16);
-#pragma unroll
-        for (int c = 0; c < D / 64; ++c) {
-          float o[32];
-          if (n > 0) {
-            ptx::tmem_ld32(tmem + lane_base + (which ? 384 : 256) + h * (D / 2) + c * 32, reinterpret_cast<uint32_t*>(o));
-            ptx::tmem_ld_wait();
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = 0.f;
-          }
-          if (grow < a.N) {
-#pragma unroll
-            for (int q4 = 0; q4 < 4; ++q4) {
-              uint4 w;
-              w.x = pack2<kBF16>(o[q4 * 8 + 0] * f, o[q4 * 8 + 1] * f);
-              w.y = pack2<kBF16>(o[q4 * 8 + 2] * f, o[q4 * 8 + 3] * f);
-              w.z = pack2<kBF16>(o[q4 * 8 + 4] * f, o[q4 * 8 + 5] * f);
-              w.w = pack2<kBF16>(o[q4 * 8 + 6] * f, o[q4 * 8 + 7] * f);
-              dst[c * 4 + q4] = w;
-            }
-          }
-        }
-      }
-    }
-  }
-
-  ptx::tc_fence_before();
-  __syncthreads();
-  if (warp == 2) {
-    ptx::tc_fence_after();
-    ptx::tmem_dealloc(tmem, 512);
-  }
-}
-
-struct Lists {
-  const int32_t *counts, *entries, *order;
-};
-
 template <int D, bool kBF16>
-int launch(const void* q, const void* k, const void* v, const void* out, const void* dout, const float* lse, int dtype, int BH,
-           int N, const Lists& ql, const Lists& kl, int Hm, float softmax_scale, int q_split, int kvl_lo, int kvl_hi, void* dq,
-           void* dk, void* dv, float* ws, int32_t* status, cudaStream_t st) {
-  const int nt = ceil_div(N, kTile), npad = nt * kTile;
-  const int kv_rows = max(1, max(kvl_lo, kvl_hi));
+int launch(BwdArgs a, const void* out, const float* lse, int dtype, int BH, float* ws, cudaStream_t st) {
+  const int kv_rows = max(1, max(a.kvl_lo, a.kvl_hi));
   CUtensorMap tq, tk, tv, tdo;
-  if (int rc = make_tmap_rows(&tq, q, dtype, BH, N, D, kTile)) return rc;
-  if (int rc = make_tmap_rows(&tdo, dout, dtype, BH, N, D, kTile)) return rc;
-  if (int rc = make_tmap_first_rows(&tk, k, dtype, BH, N, kv_rows, D, kTile)) return rc;
-  if (int rc = make_tmap_first_rows(&tv, v, dtype, BH, N, kv_rows, D, kTile)) return rc;
-  float* nlse = ws;
-  float* ndelta = ws + static_cast<int64_t>(BH) * npad;
-  bwd_stats_kernel<D, kBF16><<<dim3(npad / (2048 / D), BH), 256, 0, st>>>(out, dout, lse, N, npad, nlse, ndelta);
+  if (int rc = make_tmap_rows(&tq, a.q, dtype, BH, a.N, D, kBlock)) return rc;
+  if (int rc = make_tmap_rows(&tdo, a.dout, dtype, BH, a.N, D, kBlock)) return rc;
+  if (int rc = make_tmap_first_rows(&tk, a.k, dtype, BH, a.N, kv_rows, D, kBlock)) return rc;
+  if (int rc = make_tmap_first_rows(&tv, a.v, dtype, BH, a.N, kv_rows, D, kBlock)) return rc;
+  auto kernel = sparse_attn_bwd_kernel<D, kBF16>;
+  const size_t smem = kTilesBytes<D> + 1024 + sizeof(Control);
+  if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem)) return rc;
+  a.nlse = ws;
+  a.ndelta = ws + static_cast<int64_t>(BH) * a.npad;
+  bwd_stats_kernel<D, kBF16><<<dim3(a.npad / (2048 / D), BH), 256, 0, st>>>(out, a.dout, lse, a.N, a.npad, ws, ws + static_cast<int64_t>(BH) * a.npad);
   MODDIT_CHECK_LAUNCH("bwd_stats_kernel");
-  BwdArgs a{};
-  a.nlse = nlse; a.ndelta = ndelta; a.status = status;
-  a.Hm = Hm; a.N = N; a.ntiles = nt; a.npad = npad; a.q_split = q_split; a.kvl_lo = kvl_lo; a.kvl_hi = kvl_hi;
-  a.scale = softmax_scale; a.scale_log2 = softmax_scale * kLog2e;
-  const size_t smem = smem_bytes<D>();
-  auto keys = sparse_attn_bwd_kernel<D, kBF16, true>;
-  auto queries = sparse_attn_bwd_kernel<D, kBF16, false>;
-  if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(keys), smem)) return rc;
-  if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(queries), smem)) return rc;
-  a.counts = kl.counts; a.entries = kl.entries; a.order = kl.order; a.g0 = dk; a.g1 = dv;
-  keys<<<dim3(nt * Hm, BH / Hm), kThreads, smem, st>>>(tk, tv, tq, tdo, a);
-  MODDIT_CHECK_LAUNCH("sparse_attn_bwd_kernel (keys)");
-  a.counts = ql.counts; a.entries = ql.entries; a.order = ql.order; a.g0 = dq; a.g1 = nullptr;
-  queries<<<dim3(2 * ((nt + 1) / 2) * Hm, BH / Hm), kThreads, smem, st>>>(tq, tdo, tk, tv, a);
-  MODDIT_CHECK_LAUNCH("sparse_attn_bwd_kernel (queries)");
+  const int64_t blocks = static_cast<int64_t>(2 * a.ntiles + (a.ntiles & 1)) * BH;
+  kernel<<<static_cast<unsigned>(blocks), kThreads, smem, st>>>(tq, tk, tv, tdo, a);
+  MODDIT_CHECK_LAUNCH("sparse_attn_bwd_kernel");
   return MODDIT_OK;
 }
 
@@ -524,13 +925,20 @@ extern "C" int moddit_sparse_attn_bwd(const void* q, const void* k, const void* 
     return fail(MODDIT_E_WORKSPACE, "sparse_attn_bwd: a 16-byte aligned workspace of %zu bytes is needed",
                 moddit_sparse_attn_bwd_workspace_bytes(BH, N));
   if (int rc = require_sm100()) return rc;
-  const Lists ql{q_counts, q_entries, q_order}, kl{k_counts, k_entries, k_order};
+  if (static_cast<int64_t>(2 * ceil_div(N, kTile) + 1) * BH > (1ll << 31) - 1)
+    return fail(MODDIT_E_UNSUPPORTED, "sparse_attn_bwd: %d heads of %d rows are too many work items", BH, N);
+  BwdArgs a{};
+  a.key_lists = Lists{k_counts, k_entries, k_order};
+  a.query_lists = Lists{q_counts, q_entries, q_order};
+  a.q = q; a.k = k; a.v = v; a.dout = dout;
+  a.dq = dq; a.dk = dk; a.dv = dv; a.status = status;
+  a.Hm = Hm; a.batches = BH / Hm; a.N = N;
+  a.ntiles = ceil_div(N, kTile); a.npad = a.ntiles * kTile;
+  a.q_split = q_split; a.kvl_lo = kv_len_lo; a.kvl_hi = kv_len_hi;
+  a.scale = softmax_scale; a.scale_log2 = softmax_scale * kLog2e;
   float* ws = static_cast<float*>(workspace);
   cudaStream_t st = as_stream(stream);
-#define MODDIT_BWD(DIM, BF16)                                                                                             \
-  launch<DIM, BF16>(q, k, v, out, dout, lse, dtype, BH, N, ql, kl, Hm, softmax_scale, q_split, kv_len_lo, kv_len_hi, dq, dk, \
-                    dv, ws, status, st)
-  if (D == 128) return dtype == MODDIT_BF16 ? MODDIT_BWD(128, true) : MODDIT_BWD(128, false);
-  return dtype == MODDIT_BF16 ? MODDIT_BWD(64, true) : MODDIT_BWD(64, false);
-#undef MODDIT_BWD
+  if (D == 128)
+    return dtype == MODDIT_BF16 ? launch<128, true>(a, out, lse, dtype, BH, ws, st) : launch<128, false>(a, out, lse, dtype, BH, ws, st);
+  return dtype == MODDIT_BF16 ? launch<64, true>(a, out, lse, dtype, BH, ws, st) : launch<64, false>(a, out, lse, dtype, BH, ws, st);
 }
