@@ -87,36 +87,30 @@ __device__ __forceinline__ Item item_of(const BwdArgs& a) {
   return it;
 }
 
-// The streamed 64-row blocks of a work item in list order, with the halves of the item's rows that keep each.
-// An entry of a list names a streamed tile of 128 rows and its kept quarters; blocks past `limit` are left out.
+// The streamed 64-row blocks of a work item, in list order, as (first row << 2) | halves: bit i of `halves` says that rows
+// [64 i, 64 i + 64) of the item keep the block.  A list entry names a streamed tile of 128 rows and its kept quarters; blocks
+// that start at or past `limit` are left out.  One warp writes them to shared memory and returns how many there are.
 template <bool kKeys>
-struct Walk {
-  const int32_t* ent;
-  int left, shift, limit;
-  int en, next_en, half;
-  int x0, bits;                       // first row of the block, bit i: rows [64 i, 64 i + 64) of the item keep it
-  __device__ __forceinline__ Walk(const int32_t* entries, int count, int flag_shift, int row_limit)
-      : ent(entries), left(count), shift(flag_shift), limit(row_limit), en(0), half(2), x0(0), bits(0) {
-    next_en = left > 0 ? __ldg(ent) : 0;
-  }
-  __device__ __forceinline__ bool next() {
-    while (true) {
-      if (half == 2) {
-        if (left == 0) return false;
-        en = next_en;
-        --left;
-        ++ent;
-        if (left > 0) next_en = __ldg(ent);
-        half = 0;
-      }
-      const int fl = en >> shift;
-      bits = kKeys ? (fl >> (2 * half)) & 3 : ((fl >> half) & 1) | ((fl >> (1 + half)) & 2);
-      x0 = (en >> 8) * kTile + kBlock * half;
-      ++half;
-      if (bits != 0 && x0 < limit) return true;
+__device__ __forceinline__ int expand(const int32_t* ent, int count, int shift, int limit, int32_t* blocks) {
+  const int lane = threadIdx.x % 32;
+  int n = 0;
+  for (int e0 = 0; e0 < count; e0 += 32) {
+    const int en = e0 + lane < count ? __ldg(ent + e0 + lane) : 0;
+    const int fl = en >> shift, x0 = (en >> 8) * kTile;
+    int bits[2];
+    for (int half = 0; half < 2; ++half) {
+      bits[half] = kKeys ? (fl >> (2 * half)) & 3 : ((fl >> half) & 1) | ((fl >> (1 + half)) & 2);
+      if (e0 + lane >= count || x0 + kBlock * half >= limit) bits[half] = 0;
     }
+    const unsigned lo = __ballot_sync(0xffffffffu, bits[0] != 0), hi = __ballot_sync(0xffffffffu, bits[1] != 0);
+    const unsigned below = (1u << lane) - 1;
+    const int at = n + __popc(lo & below) + __popc(hi & below);
+    if (bits[0]) blocks[at] = (x0 << 2) | bits[0];
+    if (bits[1]) blocks[at + (bits[0] != 0)] = ((x0 + kBlock) << 2) | bits[1];
+    n += __popc(lo) + __popc(hi);
   }
-};
+  return n;
+}
 
 __device__ __forceinline__ void report(int32_t* status, int code, int role, int where) {
   if (atomicCAS(status, 0, code) == 0) {
@@ -208,9 +202,20 @@ struct KeyRows {
     bool on;
     int split, lo, hi;
   };
-  __device__ __forceinline__ bool kept(const Mask& m, int lh, int g, int i) const {
-    const int c = 8 * g + 2 * (threadIdx.x % 4) + (i & 1), row = 2 * lh + (i >> 1);
-    return (((c < m.split) ? m.lo : m.hi) >> row) & 1;
+  // zeros in the masked places of column groups [g0, g1)
+  __device__ __forceinline__ void clear(float (&v)[2][32], const Mask& m, int g0, int g1) {
+#pragma unroll
+    for (int g = 0; g < 8; ++g)
+      if (g >= g0 && g < g1)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int rows = 8 * g + 2 * static_cast<int>(threadIdx.x % 4) + i < m.split ? m.lo : m.hi;
+#pragma unroll
+          for (int row = 0; row < 4; ++row) {
+            float& x = v[row >> 1][4 * g + 2 * (row & 1) + i];
+            x = ((rows >> row) & 1) ? x : 0.f;
+          }
+        }
   }
   __device__ __forceinline__ void load(uint32_t tS) {
     ptx::tmem_ld_16x64(tS, reinterpret_cast<uint32_t*>(p[0]));
@@ -233,13 +238,18 @@ struct KeyRows {
           ptx::unpack_f32x2(ptx::fma_f32x2(ptx::pack_f32x2(v[0], v[1]), scale2, nl2), x0, x1);
           v[0] = ptx::ex2(x0);
           v[1] = ptx::ex2(x1);
-          if (m.on) {
-            v[0] = kept(m, lh, g, 2 * j) ? v[0] : 0.f;
-            v[1] = kept(m, lh, g, 2 * j + 1) ? v[1] : 0.f;
-          }
-          pk[lh][2 * gg + j] = pack2<kBF16>(v[0], v[1]);
         }
     }
+    if (m.on) clear(p, m, 4 * part, 4 * part + 4);
+#pragma unroll
+    for (int gg = 0; gg < 4; ++gg)
+#pragma unroll
+      for (int lh = 0; lh < 2; ++lh)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float* v = p[lh] + 4 * (4 * part + gg) + 2 * j;
+          pk[lh][2 * gg + j] = pack2<kBF16>(v[0], v[1]);
+        }
     ptx::tmem_st_16x4g(tS + 16 * part, pk[0]);
     ptx::tmem_st_16x4g(tS + (16u << 16) + 16 * part, pk[1]);
   }
@@ -248,6 +258,7 @@ struct KeyRows {
     ptx::tmem_ld_16x64(tP, reinterpret_cast<uint32_t*>(d[0]));
     ptx::tmem_ld_16x64(tP + (16u << 16), reinterpret_cast<uint32_t*>(d[1]));
     ptx::tmem_ld_wait();
+    if (m.on) clear(d, m, 0, 8);      // what lies in a masked place may be anything
     uint32_t pk[2][16];
 #pragma unroll
     for (int g = 0; g < 8; ++g) {
@@ -256,11 +267,7 @@ struct KeyRows {
       for (int lh = 0; lh < 2; ++lh)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          float* v = d[lh] + 4 * g + 2 * j;
-          if (m.on) {                 // what lies in a masked place may be anything
-            v[0] = kept(m, lh, g, 2 * j) ? v[0] : 0.f;
-            v[1] = kept(m, lh, g, 2 * j + 1) ? v[1] : 0.f;
-          }
+          const float* v = d[lh] + 4 * g + 2 * j;
           const uint64_t t = ptx::mul_f32x2(minus_delta<kBF16>(ptx::pack_f32x2(v[0], v[1]), nd2),
                                             ptx::pack_f32x2(p[lh][4 * g + 2 * j], p[lh][4 * g + 2 * j + 1]));
           float y0, y1;
@@ -319,11 +326,9 @@ struct Block {                        // what all roles of a block know
   uint32_t tmem;
   volatile int* abort_flag;
   uint32_t bar0;
-  int row0, bh, count, shift, limit;
-  const int32_t* ent;
+  int row0, bh, count;                // count: streamed blocks
+  const int32_t* blocks;              // of `expand`
   __device__ __forceinline__ uint32_t bar(int i) const { return bar0 + 8u * static_cast<uint32_t>(i); }
-  template <bool kKeys>
-  __device__ __forceinline__ Walk<kKeys> walk() const { return Walk<kKeys>(ent, count, shift, limit); }
 };
 
 __device__ __forceinline__ uint64_t advance(uint64_t desc, uint32_t bytes) {
@@ -333,11 +338,14 @@ __device__ __forceinline__ uint64_t advance(uint64_t desc, uint32_t bytes) {
 
 constexpr int kMaxStages = 8;
 constexpr int kNumBarriers = 2 * kMaxStages + 10;
+constexpr int kMaxBlocks = 7168;       // streamed blocks of a work item: 458,752 rows
 struct __align__(16) Control {
   float stats[kMaxStages][2][kBlock]; // key items: -lse * log2 e and -delta of the streamed query rows
   unsigned long long bars[kNumBarriers];
   uint32_t tmem_base;
   int abort_flag;
+  int count;
+  int32_t blocks[kMaxBlocks + 4];       // read ahead past the end
 };
 
 // bytes of tiles in shared memory; behind them the control block, before them up to 1024 bytes of alignment
@@ -365,22 +373,21 @@ struct Chains {
 
   static __device__ __forceinline__ void produce(const Block& b, const BwdArgs& a, const Control* ctl, const CUtensorMap* tx0,
                                                  const CUtensorMap* tx1) {
-    auto w = b.walk<kKeys>();
     const uint32_t sX = ptx::smem_u32(b.smem);
     bool ok = true;
     int k = 0;
-    for (; w.next(); ++k) {
-      const int s = k % kStages;
+    for (; k < b.count; ++k) {
+      const int s = k % kStages, x0 = b.blocks[k] >> 2;
       ok = ptx::mbar_wait(b.bar(kEmpty + s), ((k / kStages) & 1) ^ 1, b.abort_flag);
       if (!ok) { report(a.status, 1, 0, k); break; }
       const uint32_t to = sX + 2 * s * kBlockBytes;
       ptx::mbar_expect_tx(b.bar(kFull + s), 2 * kBlockBytes + (kKeys ? 2 * kBlock * 4 : 0));
       for (int c = 0; c < kChunks; ++c) {
-        ptx::tma_load_3d(to + c * kChunkBytes, tx0, b.bar(kFull + s), c * 64, w.x0, b.bh);
-        ptx::tma_load_3d(to + kBlockBytes + c * kChunkBytes, tx1, b.bar(kFull + s), c * 64, w.x0, b.bh);
+        ptx::tma_load_3d(to + c * kChunkBytes, tx0, b.bar(kFull + s), c * 64, x0, b.bh);
+        ptx::tma_load_3d(to + kBlockBytes + c * kChunkBytes, tx1, b.bar(kFull + s), c * 64, x0, b.bh);
       }
       if (kKeys) {
-        const int64_t at = static_cast<int64_t>(b.bh) * a.npad + w.x0;
+        const int64_t at = static_cast<int64_t>(b.bh) * a.npad + x0;
         ptx::bulk_load(ptx::smem_u32(ctl->stats[s][0]), a.nlse + at, kBlock * 4, b.bar(kFull + s));
         ptx::bulk_load(ptx::smem_u32(ctl->stats[s][1]), a.ndelta + at, kBlock * 4, b.bar(kFull + s));
       }
@@ -420,31 +427,21 @@ struct Chains {
       ptx::tc_fence_after();
       return ok;
     };
-    auto w = b.walk<kKeys>();
-    int known = 0;                    // blocks found so far
-    bool more = true;
-    auto have = [&](int k) {          // whether there is a block k (asked in order)
-      if (more && known <= k) {
-        more = w.next();
-        known += more;
-      }
-      return k < known;
-    };
-    if (have(0)) {
+    if (b.count > 0) {
       bool ok = ptx::mbar_wait(b.bar(kFixed), 0, b.abort_flag);
       if (!ok) report(a.status, 2, 1, -1);
       ptx::tc_fence_after();
-      for (int k = 0; k < 2 && ok && have(k); ++k) {
+      for (int k = 0; k < 2 && ok && k < b.count; ++k) {
         ok = landed(k);
         if (ok) { first(0, k); first(1, k); }
       }
-      for (int k = 0; ok && k <= known; ++k) {
-        if (k < known) {
+      for (int k = 0; ok && k <= b.count; ++k) {
+        if (k < b.count) {
           ok = ptx::mbar_wait(b.bar(kPDone + (k & 1)), (k >> 1) & 1, b.abort_flag);
           if (!ok) { report(a.status, 3, 1, k); break; }
           ptx::tc_fence_after();
           if (kKeys) second(0, k);
-          if (have(k + 2)) {
+          if (k + 2 < b.count) {
             ok = landed(k + 2);
             if (!ok) break;
             first(0, k + 2);
@@ -456,7 +453,7 @@ struct Chains {
           ptx::tc_fence_after();
           second(1, k - 1);
           ptx::tc_commit(b.bar(kEmpty + (k - 1) % kStages));
-          if (k + 1 < known && k + 1 >= 2) first(1, k + 1);
+          if (k + 1 < b.count) first(1, k + 1);
         }
       }
     }
@@ -503,11 +500,11 @@ struct Chains {
         rows_hi |= (key < a.kvl_hi) << j;
       }
     const uint64_t scale2 = ptx::pack_f32x2(a.scale_log2, a.scale_log2);
-    auto w = b.walk<kKeys>();
     bool ok = true;
-    int k = 0;
-    for (; w.next(); ++k) {
-      if ((k & 1) != c) continue;
+    int next = b.blocks[c];           // read ahead; past the end it is not used
+    for (int k = c; k < b.count; k += 2) {
+      const int x0 = next >> 2, bits = next & 3;
+      next = b.blocks[k + 2];
       const uint32_t par = (k >> 1) & 1;
       const int s = k % kStages;
       if (kKeys) ok = ptx::mbar_wait(b.bar(kFull + s), (k / kStages) & 1, b.abort_flag);      // the statistics
@@ -515,7 +512,7 @@ struct Chains {
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) { if (lane == 0) report(a.status, 5, 2 + c, k); break; }
       ptx::tc_fence_after();
-      const bool mine = (w.bits >> (wq >> 1)) & 1;
+      const bool mine = (bits >> (wq >> 1)) & 1;
       if (!mine) {                                // these rows keep nothing of the block
         if (kKeys) store_zeros(tS);
         hand_over(b.bar(kPDone + c));
@@ -528,7 +525,7 @@ struct Chains {
       }
       if constexpr (kKeys) {
         KeyRows<kBF16> x;
-        const typename KeyRows<kBF16>::Mask m{b.row0 + kTile > kv_min, a.q_split - w.x0, rows_lo, rows_hi};
+        const typename KeyRows<kBF16>::Mask m{b.row0 + kTile > kv_min, a.q_split - x0, rows_lo, rows_hi};
         x.load(tS);
         x.probabilities(0, tS, scale2, ctl->stats[s][0], m);
         x.probabilities(1, tS, scale2, ctl->stats[s][0], m);
@@ -539,7 +536,7 @@ struct Chains {
         x.scores_gradient(tP, ctl->stats[s][1], m);
       } else {
         QueryRows<kBF16> x;
-        const int below = lim - w.x0;
+        const int below = lim - x0;
         x.load(tS);
         ptx::tc_fence_before();
         ptx::mbar_arrive(b.bar(kPDone + c));      // P stays in registers: the next scores may overwrite these
@@ -561,8 +558,8 @@ struct Chains {
     auto to = [&](void* g) { return reinterpret_cast<uint4*>(static_cast<unsigned char*>(g) + at) + c * (D / 16); };
     const bool in = grow < a.N;
     const uint32_t t = b.tmem + lane_base + c * (D / 2);
-    store_rows<kBF16, D / 2>(t + kAcc0, k > 0, in, a.scale, to(kKeys ? a.dk : a.dq));
-    if (kKeys) store_rows<kBF16, D / 2>(t + kAcc1, k > 0, in, kBF16 ? 1.f : exp2f(-kHalfShift), to(a.dv));
+    store_rows<kBF16, D / 2>(t + kAcc0, b.count > 0, in, a.scale, to(kKeys ? a.dk : a.dq));
+    if (kKeys) store_rows<kBF16, D / 2>(t + kAcc1, b.count > 0, in, kBF16 ? 1.f : exp2f(-kHalfShift), to(a.dv));
   }
 };
 
@@ -584,10 +581,8 @@ struct Pairs {
 
   static __device__ __forceinline__ void produce(const Block& b, const BwdArgs& a, const Control* ctl, const CUtensorMap* tf0,
                                                  const CUtensorMap* tf1, const CUtensorMap* tx0, const CUtensorMap* tx1) {
-    auto w = b.walk<true>();
     const uint32_t sF = ptx::smem_u32(b.smem), sX = sF + 2 * kTileBytes;
-    bool more = w.next();
-    if (!more) return;
+    if (b.count == 0) return;
     ptx::mbar_expect_tx(b.bar(kFixed), 2 * kTileBytes);
     for (int c = 0; c < 2; ++c)
       for (int h = 0; h < 2; ++h) {
@@ -597,17 +592,13 @@ struct Pairs {
       }
     bool ok = true;
     int n = 0;
-    for (; more; ++n) {
+    for (; 2 * n < b.count; ++n) {
       const int s = n % kStages;
       ok = ptx::mbar_wait(b.bar(kEmpty + s), ((n / kStages) & 1) ^ 1, b.abort_flag);
       if (!ok) { report(a.status, 1, 0, n); break; }
       ptx::mbar_expect_tx(b.bar(kFull + s), 2 * kTileBytes + 4 * kBlock * 4);
-      int x0 = w.x0;
       for (int h = 0; h < 2; ++h) {
-        if (h == 1) {                 // an odd last block is there twice: its second copy is masked
-          more = w.next();
-          if (more) x0 = w.x0;
-        }
+        const int x0 = b.blocks[min(2 * n + h, b.count - 1)] >> 2;      // an odd last block is there twice, once masked
         const uint32_t to = sX + 2 * s * kTileBytes + h * kHalfBytes;
         for (int c = 0; c < 2; ++c) {
           ptx::tma_load_3d(to + c * kChunkBytes, tx0, b.bar(kFull + s), c * 64, x0, b.bh);
@@ -617,7 +608,6 @@ struct Pairs {
         ptx::bulk_load(ptx::smem_u32(ctl->stats[2 * s + h][0]), a.nlse + at, kBlock * 4, b.bar(kFull + s));
         ptx::bulk_load(ptx::smem_u32(ctl->stats[2 * s + h][1]), a.ndelta + at, kBlock * 4, b.bar(kFull + s));
       }
-      if (more) more = w.next();
     }
     if (!ok) {
       for (int i = 0; i < 4096 && !ptx::mbar_try_wait(b.bar(kFixed), 0); ++i) {}
@@ -648,18 +638,17 @@ struct Pairs {
       ptx::mma_ts(b.tmem + (which ? 256 : 384), b.tmem + which * 128 + (kk / 4) * 64 + (kk % 4) * 8, advance(b0, kk * 2048),
                   kIdescG, acc);
     };
-    auto w = b.walk<true>();
-    bool next = w.next();
+    const int steps = (b.count + 1) / 2;
     bool ok = true;
-    if (next) {
+    if (steps > 0) {
       ok = ptx::mbar_wait(b.bar(kFixed), 0, b.abort_flag) && ptx::mbar_wait(b.bar(kFull), 0, b.abort_flag);
       if (!ok) report(a.status, 2, 1, -1);
       ptx::tc_fence_after();
       if (ok) { first(0, 0); first(1, 0); }
     }
-    for (int n = 0; next && ok; ++n) {
+    for (int n = 0; n < steps && ok; ++n) {
       const int s = n % kStages, s1 = (n + 1) % kStages;
-      next = w.next() && w.next();              // whether there is a step n + 1
+      const bool next = n + 1 < steps;
       for (int part = 0; part < 2; ++part) {
         ok = ptx::mbar_wait(b.bar(kPLo + part), n & 1, b.abort_flag);
         if (!ok) { report(a.status, 3, 1, n); break; }
@@ -700,17 +689,11 @@ struct Pairs {
       rows_hi |= (key < a.kvl_hi) << j;
     }
     const uint64_t scale2 = ptx::pack_f32x2(a.scale_log2, a.scale_log2);
-    auto w = b.walk<true>();
     bool ok = true;
-    int n = 0;
-    for (bool more = w.next(); more; ++n) {
-      int x0 = w.x0, bits = w.bits;
-      more = w.next();
-      if (h == 1) {
-        x0 = w.x0;
-        bits = more ? w.bits : 0;
-      }
-      if (more) more = w.next();
+    int next = b.blocks[h];           // read ahead; past the end it counts for nothing
+    for (int n = 0; 2 * n < b.count; ++n) {
+      const int x0 = next >> 2, bits = 2 * n + h < b.count ? next & 3 : 0;
+      next = b.blocks[2 * n + 2 + h];
       const int s = n % kStages;
       ok = ptx::mbar_wait(b.bar(kFull + s), (n / kStages) & 1, b.abort_flag) &&        // the statistics
            ptx::mbar_wait(b.bar(kSFull), n & 1, b.abort_flag);
@@ -748,8 +731,8 @@ struct Pairs {
     const int64_t at = (static_cast<int64_t>(b.bh) * a.N + grow) * D * 2;
     auto to = [&](void* g) { return reinterpret_cast<uint4*>(static_cast<unsigned char*>(g) + at) + h * 8; };
     const uint32_t t = b.tmem + lane_base + h * 64;
-    store_rows<kBF16, 64>(t + 256, n > 0, grow < a.N, a.scale, to(a.dk));
-    store_rows<kBF16, 64>(t + 384, n > 0, grow < a.N, kBF16 ? 1.f : exp2f(-kHalfShift), to(a.dv));
+    store_rows<kBF16, 64>(t + 256, b.count > 0, grow < a.N, a.scale, to(a.dk));
+    store_rows<kBF16, 64>(t + 384, b.count > 0, grow < a.N, kBF16 ? 1.f : exp2f(-kHalfShift), to(a.dv));
   }
 };
 
@@ -778,10 +761,7 @@ __global__ void __launch_bounds__(kThreads, 1) sparse_attn_bwd_kernel(
   const int kv_max = max(a.kvl_lo, a.kvl_hi);
   b.bh = it.batch * a.Hm + mh;
   b.row0 = tile * kTile;
-  b.shift = it.keys ? 0 : 4 * (it.pos & 1);
-  b.limit = it.keys ? a.N : kv_max;
-  b.count = (it.keys && b.row0 >= kv_max) ? 0 : __ldg(l.counts + item);
-  b.ent = l.entries + static_cast<int64_t>(item) * a.ntiles;
+  b.blocks = ctl->blocks;
 
   auto with_kind = [&](auto&& f) {
     if (it.keys) {
@@ -807,9 +787,17 @@ __global__ void __launch_bounds__(kThreads, 1) sparse_attn_bwd_kernel(
     ptx::tmem_relinquish();
     ptx::tc_fence_before();
   }
+  if (warp == 3) {
+    const int count = (it.keys && b.row0 >= kv_max) ? 0 : __ldg(l.counts + item);
+    const int32_t* ent = l.entries + static_cast<int64_t>(item) * a.ntiles;
+    const int n = it.keys ? expand<true>(ent, count, 0, a.N, ctl->blocks)
+                          : expand<false>(ent, count, 4 * (it.pos & 1), kv_max, ctl->blocks);
+    if (lane == 0) ctl->count = n;
+  }
   __syncthreads();
   ptx::tc_fence_after();
   b.tmem = ctl->tmem_base;
+  b.count = ctl->count;
 
   if (warp == 0) {
     if (ptx::elect_one()) {
@@ -925,6 +913,7 @@ extern "C" int moddit_sparse_attn_bwd(const void* q, const void* k, const void* 
     return fail(MODDIT_E_WORKSPACE, "sparse_attn_bwd: a 16-byte aligned workspace of %zu bytes is needed",
                 moddit_sparse_attn_bwd_workspace_bytes(BH, N));
   if (int rc = require_sm100()) return rc;
+  if (N > kMaxBlocks * kBlock) return fail(MODDIT_E_UNSUPPORTED, "sparse_attn_bwd: N=%d exceeds %d", N, kMaxBlocks * kBlock);
   if (static_cast<int64_t>(2 * ceil_div(N, kTile) + 1) * BH > (1ll << 31) - 1)
     return fail(MODDIT_E_UNSUPPORTED, "sparse_attn_bwd: %d heads of %d rows are too many work items", BH, N);
   BwdArgs a{};
