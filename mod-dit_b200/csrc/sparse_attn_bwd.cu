@@ -16,8 +16,7 @@
 // P and dS stay in tensor memory, 16 bits wide, over the scores they came from, as the A operand of the second products;
 // X0 and X1 serve as K-major operands of the first products and as MN-major operands of the second from one copy in shared
 // memory.
-// Roles (12 warps): 0 TMA producer, 1 MMA issuer, 2 tensor-memory allocation, 4-11 elementwise: thread = row (lane) and 64 of
-// the tile's 128 columns.
+// Roles (20 warps): 0 TMA producer, 1 MMA issuer, 2 tensor-memory allocation, 3 the item's block list, 4-19 elementwise.
 // Tensor memory (512 columns): S [0,128) dP [128,256) acc0 [256,256+D) acc1 [384,384+D); P and dS overwrite columns
 // [64 h, 64 h + 32) of S and dP for column half h.
 // The issue order  acc1 += P(e) X1, S(e+1), acc0 += dS(e) X0, dP(e+1)  keeps the tensor pipe busy with the first two while
@@ -37,7 +36,8 @@
 namespace moddit {
 namespace {
 
-constexpr int kThreads = 384;
+constexpr int kThreads = 640;          // 4 control warps, 4 warpgroups
+constexpr int kCols = 32;              // streamed columns of a thread
 constexpr int kTile = 128;             // rows of a work item
 constexpr int kBlock = 64;             // streamed rows that are kept or left out together
 constexpr float kLog2e = 1.4426950408889634f;
@@ -140,152 +140,141 @@ __device__ __forceinline__ uint64_t minus_delta(uint64_t dp, uint64_t nd) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// Elementwise work on one 64-column block: P = 2^(S scale + nlse) and dS = P (dP - delta).
+// Elementwise work on kCols columns: P = 2^(S scale + nlse) and dS = P (dP - delta).  P and dS are packed over the first half
+// of the columns that they come from.
 //
-// Query items: a thread has one row and all 64 columns, so the row's statistics are two registers.
+// Query items: a thread has one row, so the row's statistics are two registers.
 template <bool kBF16>
 struct QueryRows {
-  float p[64];
+  float p[kCols];
   __device__ __forceinline__ void load(uint32_t tS) {
     ptx::tmem_ld32(tS, reinterpret_cast<uint32_t*>(p));
-    ptx::tmem_ld32(tS + 32, reinterpret_cast<uint32_t*>(p) + 32);
     ptx::tmem_ld_wait();
   }
   __device__ __forceinline__ void probabilities(uint64_t scale2, float nl, int below) {      // columns >= below are masked
     const uint64_t nl2 = ptx::pack_f32x2(nl, nl);
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
+    for (int i = 0; i < kCols / 2; ++i) {
       float x0, x1;
       ptx::unpack_f32x2(ptx::fma_f32x2(ptx::pack_f32x2(p[2 * i], p[2 * i + 1]), scale2, nl2), x0, x1);
       p[2 * i] = ptx::ex2(x0);
       p[2 * i + 1] = ptx::ex2(x1);
     }
-    if (__any_sync(0xffffffffu, below < kBlock)) {
+    if (__any_sync(0xffffffffu, below < kCols)) {
 #pragma unroll
-      for (int c = 0; c < 64; ++c) p[c] = c < below ? p[c] : 0.f;
+      for (int c = 0; c < kCols; ++c) p[c] = c < below ? p[c] : 0.f;
     }
   }
   // reads dP, stores dS over it
   __device__ __forceinline__ void scores_gradient(uint32_t tP, float nd, int below) {
     const uint64_t nd2 = ptx::pack_f32x2(nd, nd);
-    const bool masked = __any_sync(0xffffffffu, below < kBlock);
-    float d[64];
+    const bool masked = __any_sync(0xffffffffu, below < kCols);
+    float d[kCols];
     ptx::tmem_ld32(tP, reinterpret_cast<uint32_t*>(d));
-    ptx::tmem_ld32(tP + 32, reinterpret_cast<uint32_t*>(d) + 32);
     ptx::tmem_ld_wait();
     if (masked) {                     // what lies in a masked place may be anything
 #pragma unroll
-      for (int c = 0; c < 64; ++c) d[c] = c < below ? d[c] : 0.f;
+      for (int c = 0; c < kCols; ++c) d[c] = c < below ? d[c] : 0.f;
     }
-    uint32_t pk[32];
+    uint32_t pk[kCols / 2];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
+    for (int i = 0; i < kCols / 2; ++i) {
       const uint64_t t = ptx::mul_f32x2(minus_delta<kBF16>(ptx::pack_f32x2(d[2 * i], d[2 * i + 1]), nd2),
                                         ptx::pack_f32x2(p[2 * i], p[2 * i + 1]));
       float y0, y1;
       ptx::unpack_f32x2(t, y0, y1);
       pk[i] = pack2<kBF16>(y0, y1);
     }
-    ptx::tmem_st32(tP, pk);
+    ptx::tmem_st16(tP, pk);
   }
 };
 
-// Key items: columns are queries, so every column has statistics of its own.  A thread has four rows and sixteen columns
-// (fragments of tcgen05.ld.16x256b): it reads 16 column statistics from shared memory for 64 values.  With one row and 64
-// columns a thread it would read all 64, a warp-wide shared-memory access each - as many cycles of the shared memory as the
+// Key items: columns are queries, so every column has statistics of its own.  A thread has four rows and eight columns
+// (fragments of tcgen05.ld.16x256b): it reads 8 column statistics from shared memory for 32 values.  With one row and 32
+// columns a thread it would read all 32, a warp-wide shared-memory access each - as many cycles of the shared memory as the
 // products of a tile take from it.
 template <bool kBF16>
 struct KeyRows {
-  float p[2][32];
-  // which places are masked: rows by `lo`, `hi` (bit j: row i / 4 + 8 j may see queries before / from `split` on)
+  float p[2][16];
+  // which places are masked: rows by `lo`, `hi` (bit j: row i / 4 + 8 j may see queries before / from column `split` on)
   struct Mask {
     bool on;
     int split, lo, hi;
   };
-  // zeros in the masked places of column groups [g0, g1)
-  __device__ __forceinline__ void clear(float (&v)[2][32], const Mask& m, int g0, int g1) {
+  // zeros in the masked places
+  __device__ __forceinline__ void clear(float (&v)[2][16], const Mask& m) {
 #pragma unroll
-    for (int g = 0; g < 8; ++g)
-      if (g >= g0 && g < g1)
+    for (int g = 0; g < 4; ++g)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int rows = 8 * g + 2 * static_cast<int>(threadIdx.x % 4) + i < m.split ? m.lo : m.hi;
+      for (int i = 0; i < 2; ++i) {
+        const int rows = 8 * g + 2 * static_cast<int>(threadIdx.x % 4) + i < m.split ? m.lo : m.hi;
 #pragma unroll
-          for (int row = 0; row < 4; ++row) {
-            float& x = v[row >> 1][4 * g + 2 * (row & 1) + i];
-            x = ((rows >> row) & 1) ? x : 0.f;
-          }
+        for (int row = 0; row < 4; ++row) {
+          float& x = v[row >> 1][4 * g + 2 * (row & 1) + i];
+          x = ((rows >> row) & 1) ? x : 0.f;
         }
+      }
   }
   __device__ __forceinline__ void load(uint32_t tS) {
-    ptx::tmem_ld_16x64(tS, reinterpret_cast<uint32_t*>(p[0]));
-    ptx::tmem_ld_16x64(tS + (16u << 16), reinterpret_cast<uint32_t*>(p[1]));
+    ptx::tmem_ld_16x32(tS, reinterpret_cast<uint32_t*>(p[0]));
+    ptx::tmem_ld_16x32(tS + (16u << 16), reinterpret_cast<uint32_t*>(p[1]));
     ptx::tmem_ld_wait();
   }
-  // column groups [4 part, 4 part + 4): computes P and stores it over the first columns of S
-  __device__ __forceinline__ void probabilities(int part, uint32_t tS, uint64_t scale2, const float* nl, const Mask& m) {
+  // f(half of the lanes, pair of values, column group) over all pairs of a thread
+  template <class F>
+  __device__ __forceinline__ void pairs(F&& f) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+#pragma unroll
+      for (int lh = 0; lh < 2; ++lh)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) f(lh, 2 * g + j, g);
+  }
+  // P, stored over the first half of the columns of S
+  __device__ __forceinline__ void probabilities(uint32_t tS, uint64_t scale2, const float* nl, const Mask& m) {
+    uint64_t nl2[4];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) nl2[g] = *reinterpret_cast<const uint64_t*>(nl + 8 * g + 2 * (threadIdx.x % 4));
+    pairs([&](int lh, int i, int g) {
+      float x0, x1;
+      ptx::unpack_f32x2(ptx::fma_f32x2(ptx::pack_f32x2(p[lh][2 * i], p[lh][2 * i + 1]), scale2, nl2[g]), x0, x1);
+      p[lh][2 * i] = ptx::ex2(x0);
+      p[lh][2 * i + 1] = ptx::ex2(x1);
+    });
+    if (m.on) clear(p, m);
     uint32_t pk[2][8];
-#pragma unroll
-    for (int gg = 0; gg < 4; ++gg) {
-      const int g = 4 * part + gg;
-      const uint64_t nl2 = *reinterpret_cast<const uint64_t*>(nl + 8 * g + 2 * (threadIdx.x % 4));
-#pragma unroll
-      for (int lh = 0; lh < 2; ++lh)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float* v = p[lh] + 4 * g + 2 * j;
-          float x0, x1;
-          ptx::unpack_f32x2(ptx::fma_f32x2(ptx::pack_f32x2(v[0], v[1]), scale2, nl2), x0, x1);
-          v[0] = ptx::ex2(x0);
-          v[1] = ptx::ex2(x1);
-        }
-    }
-    if (m.on) clear(p, m, 4 * part, 4 * part + 4);
-#pragma unroll
-    for (int gg = 0; gg < 4; ++gg)
-#pragma unroll
-      for (int lh = 0; lh < 2; ++lh)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float* v = p[lh] + 4 * (4 * part + gg) + 2 * j;
-          pk[lh][2 * gg + j] = pack2<kBF16>(v[0], v[1]);
-        }
-    ptx::tmem_st_16x4g(tS + 16 * part, pk[0]);
-    ptx::tmem_st_16x4g(tS + (16u << 16) + 16 * part, pk[1]);
+    pairs([&](int lh, int i, int) { pk[lh][i] = pack2<kBF16>(p[lh][2 * i], p[lh][2 * i + 1]); });
+    ptx::tmem_st_16x4g(tS, pk[0]);
+    ptx::tmem_st_16x4g(tS + (16u << 16), pk[1]);
   }
   __device__ __forceinline__ void scores_gradient(uint32_t tP, const float* nd, const Mask& m) {
-    float d[2][32];
-    ptx::tmem_ld_16x64(tP, reinterpret_cast<uint32_t*>(d[0]));
-    ptx::tmem_ld_16x64(tP + (16u << 16), reinterpret_cast<uint32_t*>(d[1]));
+    uint64_t nd2[4];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) nd2[g] = *reinterpret_cast<const uint64_t*>(nd + 8 * g + 2 * (threadIdx.x % 4));
+    float d[2][16];
+    ptx::tmem_ld_16x32(tP, reinterpret_cast<uint32_t*>(d[0]));
+    ptx::tmem_ld_16x32(tP + (16u << 16), reinterpret_cast<uint32_t*>(d[1]));
     ptx::tmem_ld_wait();
-    if (m.on) clear(d, m, 0, 8);      // what lies in a masked place may be anything
-    uint32_t pk[2][16];
-#pragma unroll
-    for (int g = 0; g < 8; ++g) {
-      const uint64_t nd2 = *reinterpret_cast<const uint64_t*>(nd + 8 * g + 2 * (threadIdx.x % 4));
-#pragma unroll
-      for (int lh = 0; lh < 2; ++lh)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float* v = d[lh] + 4 * g + 2 * j;
-          const uint64_t t = ptx::mul_f32x2(minus_delta<kBF16>(ptx::pack_f32x2(v[0], v[1]), nd2),
-                                            ptx::pack_f32x2(p[lh][4 * g + 2 * j], p[lh][4 * g + 2 * j + 1]));
-          float y0, y1;
-          ptx::unpack_f32x2(t, y0, y1);
-          pk[lh][2 * g + j] = pack2<kBF16>(y0, y1);
-        }
-    }
-    ptx::tmem_st_16x8g(tP, pk[0]);
-    ptx::tmem_st_16x8g(tP + (16u << 16), pk[1]);
+    if (m.on) clear(d, m);            // what lies in a masked place may be anything
+    uint32_t pk[2][8];
+    pairs([&](int lh, int i, int g) {
+      const uint64_t t = ptx::mul_f32x2(minus_delta<kBF16>(ptx::pack_f32x2(d[lh][2 * i], d[lh][2 * i + 1]), nd2[g]),
+                                        ptx::pack_f32x2(p[lh][2 * i], p[lh][2 * i + 1]));
+      float y0, y1;
+      ptx::unpack_f32x2(t, y0, y1);
+      pk[lh][i] = pack2<kBF16>(y0, y1);
+    });
+    ptx::tmem_st_16x4g(tP, pk[0]);
+    ptx::tmem_st_16x4g(tP + (16u << 16), pk[1]);
   }
 };
 
-// 32 packed columns of zeros (P or dS of rows that keep nothing of a block)
+// Packed zeros (P or dS of rows that keep nothing of a block)
 __device__ __forceinline__ void store_zeros(uint32_t t) {
-  uint32_t z[32];
+  uint32_t z[kCols / 2];
 #pragma unroll
-  for (int i = 0; i < 32; ++i) z[i] = 0u;
-  ptx::tmem_st32(t, z);
+  for (int i = 0; i < kCols / 2; ++i) z[i] = 0u;
+  ptx::tmem_st16(t, z);
 }
 
 __device__ __forceinline__ void hand_over(uint32_t bar) {
@@ -294,30 +283,27 @@ __device__ __forceinline__ void hand_over(uint32_t bar) {
   ptx::mbar_arrive(bar);
 }
 
-// kCols accumulator columns of this thread's row, times f, as 16-bit values to dst; zeros where nothing was accumulated
-template <bool kBF16, int kCols>
+// kWidth accumulator columns of this thread's row, times f, as 16-bit values to dst; zeros where nothing was accumulated
+template <bool kBF16, int kWidth>
 __device__ __forceinline__ void store_rows(uint32_t t, bool any, bool in, float f, uint4* dst) {
+  float o[kWidth];
+  if (any) {
+    if constexpr (kWidth == 32) ptx::tmem_ld32(t, reinterpret_cast<uint32_t*>(o));
+    else ptx::tmem_ld16(t, reinterpret_cast<uint32_t*>(o));
+    ptx::tmem_ld_wait();
+  } else {
 #pragma unroll
-  for (int c = 0; c < kCols / 32; ++c) {
-    float o[32];
-    if (any) {
-      ptx::tmem_ld32(t + c * 32, reinterpret_cast<uint32_t*>(o));
-      ptx::tmem_ld_wait();
-    } else {
+    for (int i = 0; i < kWidth; ++i) o[i] = 0.f;
+  }
+  if (!in) return;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) o[i] = 0.f;
-    }
-    if (in) {
-#pragma unroll
-      for (int q4 = 0; q4 < 4; ++q4) {
-        uint4 w;
-        w.x = pack2<kBF16>(o[q4 * 8 + 0] * f, o[q4 * 8 + 1] * f);
-        w.y = pack2<kBF16>(o[q4 * 8 + 2] * f, o[q4 * 8 + 3] * f);
-        w.z = pack2<kBF16>(o[q4 * 8 + 4] * f, o[q4 * 8 + 5] * f);
-        w.w = pack2<kBF16>(o[q4 * 8 + 6] * f, o[q4 * 8 + 7] * f);
-        dst[c * 4 + q4] = w;
-      }
-    }
+  for (int i = 0; i < kWidth / 8; ++i) {
+    uint4 w;
+    w.x = pack2<kBF16>(o[i * 8 + 0] * f, o[i * 8 + 1] * f);
+    w.y = pack2<kBF16>(o[i * 8 + 2] * f, o[i * 8 + 3] * f);
+    w.z = pack2<kBF16>(o[i * 8 + 4] * f, o[i * 8 + 5] * f);
+    w.w = pack2<kBF16>(o[i * 8 + 6] * f, o[i * 8 + 7] * f);
+    dst[i] = w;
   }
 }
 
@@ -353,7 +339,7 @@ template <int D>
 constexpr size_t kTilesBytes = static_cast<size_t>(D == 128 ? 192 : 128) * 1024;
 
 // ---------------------------------------------------------------------------------------------------------------
-// Two chains: warpgroup c takes the streamed blocks c, c + 2, c + 4, ... through scores, dP and dS of its own, half a step
+// Two chains: warpgroups 2 c and 2 c + 1 take the streamed blocks c, c + 2, c + 4, ... through scores, dP and dS of its own, half a step
 // behind the other one, so that one has exponentials to do while the other one waits or packs.  The fixed tiles live in
 // tensor memory as A operands, which halves what the products read from shared memory.
 // Tensor memory: S_c [64 c, 64 c + 64), dP_c 128 + the same, acc0 [256, 256 + D), acc1 behind it (D = 64), F0, F1 from 384 on.
@@ -368,7 +354,7 @@ struct Chains {
   enum { kFixed = 0, kSFull = 1, kDPFull = 3, kPDone = 5, kDSDone = 7, kFinal = 9, kFull = 10, kEmpty = kFull + kStages };
 
   static __device__ __forceinline__ int arrivals(int i) {
-    return i == kFixed ? 256 : (i >= kPDone && i < kFinal) ? 128 : 1;
+    return i == kFixed ? 512 : (i >= kPDone && i < kFinal) ? 256 : 1;
   }
 
   static __device__ __forceinline__ void produce(const Block& b, const BwdArgs& a, const Control* ctl, const CUtensorMap* tx0,
@@ -418,7 +404,7 @@ struct Chains {
       const uint64_t b0 = advance(dg, (2 * (k % kStages) + 1 - which) * kBlockBytes);
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk)
-        ptx::mma_ts(b.tmem + (which ? kAcc0 : kAcc1), b.tmem + which * 128 + (k & 1) * 64 + kk * 8, advance(b0, kk * 2048),
+        ptx::mma_ts(b.tmem + (which ? kAcc0 : kAcc1), b.tmem + which * 128 + (k & 1) * 64 + (kk >> 1) * 32 + (kk & 1) * 8, advance(b0, kk * 2048),
                     kIdescG, (k > 0 || kk > 0) ? 1u : 0u);
     };
     auto landed = [&](int k) {
@@ -460,32 +446,32 @@ struct Chains {
     ptx::tc_commit(b.bar(kFinal));
   }
 
-  // This thread's row of F0 (chain 0) or F1 (chain 1) into tensor memory; rows at and past `rows` are zero.
-  static __device__ __forceinline__ void load_fixed(const Block& b, const BwdArgs& a, const void* f, int c, uint32_t lane_base,
+  // Half of this thread's row of F0 or F1 into tensor memory; rows at and past `rows` are zero.
+  static __device__ __forceinline__ void load_fixed(const Block& b, const BwdArgs& a, const void* f, uint32_t to, int half,
                                                     int grow, int rows) {
     const uint4* src = reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(f) +
-                                                      (static_cast<int64_t>(b.bh) * a.N + grow) * D * 2);
+                                                      (static_cast<int64_t>(b.bh) * a.N + grow) * D * 2) + half * (D / 16);
+    uint32_t v[D / 4];
 #pragma unroll
-    for (int j = 0; j < D / 64; ++j) {
-      uint32_t v[32];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint4 x = grow < rows ? __ldg(src + 8 * j + i) : make_uint4(0, 0, 0, 0);
-        v[4 * i] = x.x; v[4 * i + 1] = x.y; v[4 * i + 2] = x.z; v[4 * i + 3] = x.w;
-      }
-      ptx::tmem_st32(b.tmem + lane_base + kF + c * (D / 2) + 32 * j, v);
+    for (int i = 0; i < D / 16; ++i) {
+      const uint4 x = grow < rows ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
+      v[4 * i] = x.x; v[4 * i + 1] = x.y; v[4 * i + 2] = x.z; v[4 * i + 3] = x.w;
     }
+    if constexpr (D == 128) ptx::tmem_st32(to + half * 32, v);
+    else ptx::tmem_st16(to + half * 16, v);
     hand_over(b.bar(kFixed));
   }
 
   static __device__ __forceinline__ void compute(const Block& b, const BwdArgs& a, const Control* ctl, int warp, int lane) {
-    const int c = (warp - 4) / 4;                 // chain
+    const int c = (warp - 4) / 8;                 // chain
+    const int u = ((warp - 4) / 4) & 1;           // half of its columns
     const int wq = warp % 4;                      // tensor-memory lane quarter
     const int grow = b.row0 + wq * 32 + lane;
     const uint32_t lane_base = static_cast<uint32_t>(wq * 32) << 16;
-    const uint32_t tS = b.tmem + lane_base + c * 64, tP = tS + 128;
+    const uint32_t tS = b.tmem + lane_base + c * 64 + u * kCols, tP = tS + 128;
     const int kv_min = min(a.kvl_lo, a.kvl_hi), kv_max = max(a.kvl_lo, a.kvl_hi);
-    load_fixed(b, a, kKeys ? (c ? a.v : a.k) : (c ? a.dout : a.q), c, lane_base, grow, kKeys ? kv_max : a.N);
+    load_fixed(b, a, kKeys ? (c ? a.v : a.k) : (c ? a.dout : a.q), b.tmem + lane_base + kF + c * (D / 2), u, grow,
+               kKeys ? kv_max : a.N);
     float nl = 0.f, nd = 0.f;
     if (!kKeys) {
       nl = a.nlse[static_cast<int64_t>(b.bh) * a.npad + grow];
@@ -525,18 +511,17 @@ struct Chains {
       }
       if constexpr (kKeys) {
         KeyRows<kBF16> x;
-        const typename KeyRows<kBF16>::Mask m{b.row0 + kTile > kv_min, a.q_split - x0, rows_lo, rows_hi};
+        const typename KeyRows<kBF16>::Mask m{b.row0 + kTile > kv_min, a.q_split - x0 - u * kCols, rows_lo, rows_hi};
         x.load(tS);
-        x.probabilities(0, tS, scale2, ctl->stats[s][0], m);
-        x.probabilities(1, tS, scale2, ctl->stats[s][0], m);
+        x.probabilities(tS, scale2, ctl->stats[s][0] + u * kCols, m);
         hand_over(b.bar(kPDone + c));
         ok = __all_sync(0xffffffffu, ptx::mbar_wait(b.bar(kDPFull + c), par, b.abort_flag));
         if (!ok) { if (lane == 0) report(a.status, 6, 2 + c, k); break; }
         ptx::tc_fence_after();
-        x.scores_gradient(tP, ctl->stats[s][1], m);
+        x.scores_gradient(tP, ctl->stats[s][1] + u * kCols, m);
       } else {
         QueryRows<kBF16> x;
-        const int below = lim - x0;
+        const int below = lim - x0 - u * kCols;
         x.load(tS);
         ptx::tc_fence_before();
         ptx::mbar_arrive(b.bar(kPDone + c));      // P stays in registers: the next scores may overwrite these
@@ -555,11 +540,12 @@ struct Chains {
     if (!ok) return;
     ptx::tc_fence_after();
     const int64_t at = (static_cast<int64_t>(b.bh) * a.N + grow) * D * 2;
-    auto to = [&](void* g) { return reinterpret_cast<uint4*>(static_cast<unsigned char*>(g) + at) + c * (D / 16); };
+    const int col = (2 * c + u) * (D / 4);
+    auto to = [&](void* g) { return reinterpret_cast<uint4*>(static_cast<unsigned char*>(g) + at + 2 * col); };
     const bool in = grow < a.N;
-    const uint32_t t = b.tmem + lane_base + c * (D / 2);
-    store_rows<kBF16, D / 2>(t + kAcc0, b.count > 0, in, a.scale, to(kKeys ? a.dk : a.dq));
-    if (kKeys) store_rows<kBF16, D / 2>(t + kAcc1, b.count > 0, in, kBF16 ? 1.f : exp2f(-kHalfShift), to(a.dv));
+    const uint32_t t = b.tmem + lane_base + col;
+    store_rows<kBF16, D / 4>(t + kAcc0, b.count > 0, in, a.scale, to(kKeys ? a.dk : a.dq));
+    if (kKeys) store_rows<kBF16, D / 4>(t + kAcc1, b.count > 0, in, kBF16 ? 1.f : exp2f(-kHalfShift), to(a.dv));
   }
 };
 
@@ -575,9 +561,9 @@ struct Pairs {
   static constexpr int kTileBytes = kTile * D * 2;
   static constexpr int kChunkBytes = kTile * 128;
   static constexpr int kHalfBytes = kBlock * 128;       // a block's rows of one 64-element chunk
-  enum { kFixed = 0, kSFull, kDPFull, kPLo, kPHi, kDSDone, kFinal, kFull, kEmpty = kFull + kStages, kUsed = kEmpty + kStages };
+  enum { kFixed = 0, kSFull, kDPFull, kPDone, kDSDone, kFinal, kFull, kEmpty = kFull + kStages, kUsed = kEmpty + kStages };
 
-  static __device__ __forceinline__ int arrivals(int i) { return (i >= kPLo && i <= kDSDone) ? 256 : 1; }
+  static __device__ __forceinline__ int arrivals(int i) { return (i == kPDone || i == kDSDone) ? 512 : 1; }
 
   static __device__ __forceinline__ void produce(const Block& b, const BwdArgs& a, const Control* ctl, const CUtensorMap* tf0,
                                                  const CUtensorMap* tf1, const CUtensorMap* tx0, const CUtensorMap* tx1) {
@@ -632,11 +618,13 @@ struct Pairs {
       }
       ptx::tc_commit(b.bar(kSFull + which));
     };
-    // acc += A X over 16-query steps: kk = 4 h + j has its A operand at 64 h + 8 j
-    auto second = [&](int which, int s, int kk, uint32_t acc) {
+    // which = 0: acc1 += P X1, 1: acc0 += dS X0; a warpgroup's 32 columns are two steps of 16
+    auto second = [&](int which, int s, uint32_t acc) {
       const uint64_t b0 = advance(dg, (2 * s + 1 - which) * kTileBytes);
-      ptx::mma_ts(b.tmem + (which ? 256 : 384), b.tmem + which * 128 + (kk / 4) * 64 + (kk % 4) * 8, advance(b0, kk * 2048),
-                  kIdescG, acc);
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk)
+        ptx::mma_ts(b.tmem + (which ? 256 : 384), b.tmem + which * 128 + (kk >> 1) * 32 + (kk & 1) * 8, advance(b0, kk * 2048),
+                    kIdescG, (acc || kk > 0) ? 1u : 0u);
     };
     const int steps = (b.count + 1) / 2;
     bool ok = true;
@@ -649,16 +637,10 @@ struct Pairs {
     for (int n = 0; n < steps && ok; ++n) {
       const int s = n % kStages, s1 = (n + 1) % kStages;
       const bool next = n + 1 < steps;
-      for (int part = 0; part < 2; ++part) {
-        ok = ptx::mbar_wait(b.bar(kPLo + part), n & 1, b.abort_flag);
-        if (!ok) { report(a.status, 3, 1, n); break; }
-        ptx::tc_fence_after();
-        second(0, s, 2 * part, (n > 0 || part > 0) ? 1u : 0u);
-        second(0, s, 2 * part + 1, 1u);
-        second(0, s, 2 * part + 4, 1u);
-        second(0, s, 2 * part + 5, 1u);
-      }
-      if (!ok) break;
+      ok = ptx::mbar_wait(b.bar(kPDone), n & 1, b.abort_flag);
+      if (!ok) { report(a.status, 3, 1, n); break; }
+      ptx::tc_fence_after();
+      second(0, s, n > 0);
       if (next) {
         ok = ptx::mbar_wait(b.bar(kFull + s1), ((n + 1) / kStages) & 1, b.abort_flag);
         if (!ok) { report(a.status, 2, 1, n); break; }
@@ -668,8 +650,7 @@ struct Pairs {
       ok = ptx::mbar_wait(b.bar(kDSDone), n & 1, b.abort_flag);
       if (!ok) { report(a.status, 4, 1, n); break; }
       ptx::tc_fence_after();
-#pragma unroll
-      for (int kk = 0; kk < 8; ++kk) second(1, s, kk, (n > 0 || kk > 0) ? 1u : 0u);
+      second(1, s, n > 0);
       ptx::tc_commit(b.bar(kEmpty + s));
       if (next) first(1, s1);
     }
@@ -677,10 +658,11 @@ struct Pairs {
   }
 
   static __device__ __forceinline__ void compute(const Block& b, const BwdArgs& a, const Control* ctl, int warp, int lane) {
-    const int h = (warp - 4) / 4;                 // which of the two streamed blocks
+    const int h = (warp - 4) / 8;                 // which of the two streamed blocks
+    const int u = ((warp - 4) / 4) & 1;           // half of its columns
     const int wq = warp % 4;
     const uint32_t lane_base = static_cast<uint32_t>(wq * 32) << 16;
-    const uint32_t tS = b.tmem + lane_base + h * 64, tP = tS + 128;
+    const uint32_t tS = b.tmem + lane_base + h * 64 + u * kCols, tP = tS + 128;
     const int kv_min = min(a.kvl_lo, a.kvl_hi);
     int rows_lo = 0, rows_hi = 0;
     for (int j = 0; j < 4; ++j) {
@@ -702,22 +684,18 @@ struct Pairs {
       ptx::tc_fence_after();
       const bool mine = (bits >> (wq >> 1)) & 1;
       KeyRows<kBF16> x;
-      const typename KeyRows<kBF16>::Mask m{b.row0 + kTile > kv_min, a.q_split - x0, rows_lo, rows_hi};
+      const typename KeyRows<kBF16>::Mask m{b.row0 + kTile > kv_min, a.q_split - x0 - u * kCols, rows_lo, rows_hi};
       if (mine) {
         x.load(tS);
-        x.probabilities(0, tS, scale2, ctl->stats[2 * s + h][0], m);
-        hand_over(b.bar(kPLo));
-        x.probabilities(1, tS, scale2, ctl->stats[2 * s + h][0], m);
-        hand_over(b.bar(kPHi));
+        x.probabilities(tS, scale2, ctl->stats[2 * s + h][0] + u * kCols, m);
       } else {
         store_zeros(tS);
-        hand_over(b.bar(kPLo));
-        ptx::mbar_arrive(b.bar(kPHi));
       }
+      hand_over(b.bar(kPDone));
       ok = __all_sync(0xffffffffu, ptx::mbar_wait(b.bar(kDPFull), n & 1, b.abort_flag));
       if (!ok) { if (lane == 0) report(a.status, 6, 2 + h, n); break; }
       ptx::tc_fence_after();
-      if (mine) x.scores_gradient(tP, ctl->stats[2 * s + h][1], m);
+      if (mine) x.scores_gradient(tP, ctl->stats[2 * s + h][1] + u * kCols, m);
       else store_zeros(tP);
       hand_over(b.bar(kDSDone));
     }
@@ -729,10 +707,11 @@ struct Pairs {
     ptx::tc_fence_after();
     const int grow = b.row0 + wq * 32 + lane;
     const int64_t at = (static_cast<int64_t>(b.bh) * a.N + grow) * D * 2;
-    auto to = [&](void* g) { return reinterpret_cast<uint4*>(static_cast<unsigned char*>(g) + at) + h * 8; };
-    const uint32_t t = b.tmem + lane_base + h * 64;
-    store_rows<kBF16, 64>(t + 256, b.count > 0, grow < a.N, a.scale, to(a.dk));
-    store_rows<kBF16, 64>(t + 384, b.count > 0, grow < a.N, kBF16 ? 1.f : exp2f(-kHalfShift), to(a.dv));
+    const int col = (2 * h + u) * 32;
+    auto to = [&](void* g) { return reinterpret_cast<uint4*>(static_cast<unsigned char*>(g) + at + 2 * col); };
+    const uint32_t t = b.tmem + lane_base + col;
+    store_rows<kBF16, 32>(t + 256, b.count > 0, grow < a.N, a.scale, to(a.dk));
+    store_rows<kBF16, 32>(t + 384, b.count > 0, grow < a.N, kBF16 ? 1.f : exp2f(-kHalfShift), to(a.dv));
   }
 };
 
