@@ -280,7 +280,8 @@ __device__ __forceinline__ void store_zeros(uint32_t t) {
 __device__ __forceinline__ void hand_over(uint32_t bar) {
   ptx::tmem_st_wait();
   ptx::tc_fence_before();
-  ptx::mbar_arrive(bar);
+  __syncwarp();
+  if (threadIdx.x % 32 == 0) ptx::mbar_arrive(bar);
 }
 
 // kWidth accumulator columns of this thread's row, times f, as 16-bit values to dst; zeros where nothing was accumulated
@@ -354,7 +355,7 @@ struct Chains {
   enum { kFixed = 0, kSFull = 1, kDPFull = 3, kPDone = 5, kDSDone = 7, kFinal = 9, kFull = 10, kEmpty = kFull + kStages };
 
   static __device__ __forceinline__ int arrivals(int i) {
-    return i == kFixed ? 512 : (i >= kPDone && i < kFinal) ? 256 : 1;
+    return i == kFixed ? 16 : (i >= kPDone && i < kFinal) ? 8 : 1;
   }
 
   static __device__ __forceinline__ void produce(const Block& b, const BwdArgs& a, const Control* ctl, const CUtensorMap* tx0,
@@ -493,8 +494,7 @@ struct Chains {
       next = b.blocks[k + 2];
       const uint32_t par = (k >> 1) & 1;
       const int s = k % kStages;
-      if (kKeys) ok = ptx::mbar_wait(b.bar(kFull + s), (k / kStages) & 1, b.abort_flag);      // the statistics
-      ok = ok && ptx::mbar_wait(b.bar(kSFull + c), par, b.abort_flag);
+      ok = ptx::mbar_wait(b.bar(kSFull + c), par, b.abort_flag);      // the statistics came with the operands
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) { if (lane == 0) report(a.status, 5, 2 + c, k); break; }
       ptx::tc_fence_after();
@@ -524,7 +524,8 @@ struct Chains {
         const int below = lim - x0 - u * kCols;
         x.load(tS);
         ptx::tc_fence_before();
-        ptx::mbar_arrive(b.bar(kPDone + c));      // P stays in registers: the next scores may overwrite these
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(b.bar(kPDone + c));      // P stays in registers: the next scores may overwrite these
         x.probabilities(scale2, nl, below);
         ok = __all_sync(0xffffffffu, ptx::mbar_wait(b.bar(kDPFull + c), par, b.abort_flag));
         if (!ok) { if (lane == 0) report(a.status, 6, 2 + c, k); break; }
@@ -563,7 +564,7 @@ struct Pairs {
   static constexpr int kHalfBytes = kBlock * 128;       // a block's rows of one 64-element chunk
   enum { kFixed = 0, kSFull, kDPFull, kPDone, kDSDone, kFinal, kFull, kEmpty = kFull + kStages, kUsed = kEmpty + kStages };
 
-  static __device__ __forceinline__ int arrivals(int i) { return (i == kPDone || i == kDSDone) ? 512 : 1; }
+  static __device__ __forceinline__ int arrivals(int i) { return (i == kPDone || i == kDSDone) ? 16 : 1; }
 
   static __device__ __forceinline__ void produce(const Block& b, const BwdArgs& a, const Control* ctl, const CUtensorMap* tf0,
                                                  const CUtensorMap* tf1, const CUtensorMap* tx0, const CUtensorMap* tx1) {
@@ -677,8 +678,7 @@ struct Pairs {
       const int x0 = next >> 2, bits = 2 * n + h < b.count ? next & 3 : 0;
       next = b.blocks[2 * n + 2 + h];
       const int s = n % kStages;
-      ok = ptx::mbar_wait(b.bar(kFull + s), (n / kStages) & 1, b.abort_flag) &&        // the statistics
-           ptx::mbar_wait(b.bar(kSFull), n & 1, b.abort_flag);
+      ok = ptx::mbar_wait(b.bar(kSFull), n & 1, b.abort_flag);      // the statistics came with the operands
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) { if (lane == 0) report(a.status, 5, 2 + h, n); break; }
       ptx::tc_fence_after();

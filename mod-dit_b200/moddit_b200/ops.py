@@ -123,6 +123,28 @@ class _timed:
         return False
 
 
+class _entry(_timed):
+    """`_timed` on `dev` as the current device; switches devices only where another one is current."""
+    __slots__ = ("prev",)
+
+    def __enter__(self):
+        current = torch.cuda.current_device()
+        self.prev = -1 if self.dev.index in (None, current) else current
+        if self.prev >= 0:
+            torch.cuda.set_device(self.dev)
+        return super().__enter__()
+
+    def __exit__(self, *exc):
+        super().__exit__(*exc)
+        if self.prev >= 0:
+            torch.cuda.set_device(self.prev)
+        return False
+
+
+def _addr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
 def _ptr(t: Optional[torch.Tensor]):
     return ctypes.c_void_p(0 if t is None else t.data_ptr())
 
@@ -338,13 +360,13 @@ def qkv_prologue_bwd(dq: Optional[torch.Tensor], dk: Optional[torch.Tensor], dv:
     if any(r is not None for r in res.values()):
         wsb = lib.moddit_qkv_prologue_bwd_workspace_bytes(B, S, H, D, kind)
         ws = torch.empty(wsb, device=dev, dtype=torch.uint8)
-    with torch.cuda.device(dev), _timed("moddit_qkv_prologue_bwd", dev):
+    with _entry("moddit_qkv_prologue_bwd", dev):
         check(lib.moddit_qkv_prologue_bwd(
-            _ptr(dq), _ptr(dk), _ptr(dv), _ptr(inputs[0]), _ptr(inputs[1]), dt, B, S, H, D, stride, kind, _ptr(q_weight),
-            _ptr(k_weight), float(eps), _ptr(rope_cos), _ptr(rope_sin), _lib.ROPE_FORM[rope_form], lo, hi, N, int(src_row0),
-            _ptr(out[0] if dq is not None else None), _ptr(out[1] if dk is not None else None),
-            _ptr(out[2] if dv is not None else None), out_stride, _ptr(res["q_weight"]), _ptr(res["q_bias"]),
-            _ptr(res["k_weight"]), _ptr(res["k_bias"]), _ptr(ws), wsb, _stream(dev)), "moddit_qkv_prologue_bwd")
+            _addr(dq), _addr(dk), _addr(dv), _addr(inputs[0]), _addr(inputs[1]), dt, B, S, H, D, stride, kind, _addr(q_weight),
+            _addr(k_weight), eps, _addr(rope_cos), _addr(rope_sin), _lib.ROPE_FORM[rope_form], lo, hi, N, src_row0,
+            _addr(out[0]) if dq is not None else None, _addr(out[1]) if dk is not None else None,
+            _addr(out[2]) if dv is not None else None, out_stride, _addr(res["q_weight"]), _addr(res["q_bias"]),
+            _addr(res["k_weight"]), _addr(res["k_bias"]), _addr(ws), wsb, _stream(dev)), "moddit_qkv_prologue_bwd")
     return tuple(out), res
 
 
@@ -907,7 +929,7 @@ def post_status(device) -> None:
     if slot is None:
         slot = [torch.zeros(4, dtype=torch.int32).pin_memory(), None]
         _POSTED[idx] = slot
-    if slot[1] is not None and not slot[1].query():
+    elif slot[1] is not None and not slot[1].query():
         return                                   # the previous copy has not landed yet: it reports the same words
     slot[0].copy_(_status_words(device), non_blocking=True)
     ev = torch.cuda.Event()
@@ -1026,11 +1048,12 @@ def sparse_attn_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
     if q.dim() != 4:
         raise ValueError("query, key, value, output and its gradient must be (B, H, N, D) tensors")
     dt = _qkv_dtype(q)
+    shape, dtype = q.shape, q.dtype
     for t in (k, v, out, dout):
-        if t.shape != q.shape or t.dtype != q.dtype:
+        if t.shape != shape or t.dtype != dtype:
             raise ValueError("query, key, value, output and its gradient must have identical shapes and dtypes")
-    B, H, N, D = q.shape
-    if tuple(lse.shape) != (B, H, N) or lse.dtype != torch.float32:
+    B, H, N, D = shape
+    if lse.shape != shape[:3] or lse.dtype != torch.float32:
         raise ValueError("lse must be the float32 (B, H, N) tensor that the forward returned")
     _need_contig(dout=dout, q=q, k=k, v=v, out=out, lse=lse)
     nt = (N + 127) // 128
@@ -1041,14 +1064,14 @@ def sparse_attn_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
         raise ValueError("tile_lists and key_lists must come from one mask")
     dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
     wsb = lib.moddit_sparse_attn_bwd_workspace_bytes(B * H, N)
-    ws = torch.empty(max(wsb, 16), device=dev, dtype=torch.uint8)
-    st = _status_words(dev)
-    with torch.cuda.device(dev), _timed("moddit_sparse_attn_bwd", dev):
+    ws = torch.empty(wsb, device=dev, dtype=torch.uint8)
+    with _entry("moddit_sparse_attn_bwd", dev):
         check(lib.moddit_sparse_attn_bwd(
-            _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(dout), _ptr(lse), dt, B * H, N, D, _ptr(lists.counts),
-            _ptr(lists.entries), _ptr(lists.order), _ptr(key_lists.counts), _ptr(key_lists.entries), _ptr(key_lists.order),
-            Hm, float(D ** -0.5 if softmax_scale is None else softmax_scale), N if q_split is None else int(q_split),
-            N if kv_len_lo is None else int(kv_len_lo), N if kv_len_hi is None else int(kv_len_hi), _ptr(dq), _ptr(dk),
-            _ptr(dv), _ptr(ws), wsb, _ptr(st), _stream(dev)), "moddit_sparse_attn_bwd")
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(), lse.data_ptr(), dt, B * H, N, D,
+            lists.counts.data_ptr(), lists.entries.data_ptr(), lists.order.data_ptr(), key_lists.counts.data_ptr(),
+            key_lists.entries.data_ptr(), key_lists.order.data_ptr(), Hm,
+            D ** -0.5 if softmax_scale is None else softmax_scale, N if q_split is None else q_split,
+            N if kv_len_lo is None else kv_len_lo, N if kv_len_hi is None else kv_len_hi, dq.data_ptr(), dk.data_ptr(),
+            dv.data_ptr(), ws.data_ptr(), wsb, _status_words(dev).data_ptr(), _stream(dev)), "moddit_sparse_attn_bwd")
     _after_launch(dev, check_status)
     return dq, dk, dv
