@@ -24,7 +24,8 @@ namespace moddit {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kRows = 4;                // rows per thread of an item of the per-head kernel
+constexpr int kRows = 2;                // rows per thread of an item of the per-head kernel
+constexpr int kHeads = 2;               // heads of them in flight
 
 template <typename T>
 struct Pair;
@@ -83,51 +84,68 @@ struct BwdArgs {
   const float* sin;
   int64_t token_stride, out_stride;
   int B, S, H, N_out, src_row0, rope_form, rope_lo, rope_hi;
+  int heads_per_item;      // of the per-head kernel
   float eps;
 };
 
-// Turns eight gradients of token s (columns 8 c to 8 c + 7 of a head) back through the rotation.
-template <int D>
-__device__ __forceinline__ void unrotate(const BwdArgs& a, int s, int c, float (&g)[8]) {
-  if (a.cos == nullptr || s < a.rope_lo || s >= a.rope_hi) return;
+// The factors that turn a pair's gradients back, for columns 8 c to 8 c + 7 of token s: the forward has
+//   out0 = y0 cs0 - y1 sn0,  out1 = y0 sn1 + y1 cs1,  so  dy0 = g0 cs0 + g1 sn1,  dy1 = g1 cs1 - g0 sn0.
+struct Turn {
   float cs[8], sn[8];
+};
+template <int D>
+__device__ __forceinline__ Turn turn_of(const BwdArgs& a, int s, int c) {
+  Turn t;
+  if (a.cos == nullptr || s < a.rope_lo || s >= a.rope_hi) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t.cs[i] = 1.f, t.sn[i] = 0.f;
+    return t;
+  }
   if (a.rope_form == MODDIT_ROPE_PAIR) {
     const int64_t at = static_cast<int64_t>(s - a.rope_lo) * (D / 2) + c * 4;
     const float4 c4 = __ldg(reinterpret_cast<const float4*>(a.cos + at)), s4 = __ldg(reinterpret_cast<const float4*>(a.sin + at));
     const float cv[4] = {c4.x, c4.y, c4.z, c4.w}, sv[4] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      cs[2 * i] = cs[2 * i + 1] = cv[i];
-      sn[2 * i] = sn[2 * i + 1] = sv[i];
+      t.cs[2 * i] = t.cs[2 * i + 1] = cv[i];
+      t.sn[2 * i] = t.sn[2 * i + 1] = sv[i];
     }
-  } else {
-    const int64_t at = static_cast<int64_t>(s - a.rope_lo) * D + c * 8;
+    return t;
+  }
+  const int64_t at = static_cast<int64_t>(s - a.rope_lo) * D + c * 8;
 #pragma unroll
-    for (int i = 0; i < 8; i += 4) {
-      *reinterpret_cast<float4*>(cs + i) = __ldg(reinterpret_cast<const float4*>(a.cos + at + i));
-      *reinterpret_cast<float4*>(sn + i) = __ldg(reinterpret_cast<const float4*>(a.sin + at + i));
-    }
-    if (a.rope_form == MODDIT_ROPE_EVEN_COS_ODD_SIN) {
+  for (int i = 0; i < 8; i += 4) {
+    *reinterpret_cast<float4*>(t.cs + i) = __ldg(reinterpret_cast<const float4*>(a.cos + at + i));
+    *reinterpret_cast<float4*>(t.sn + i) = __ldg(reinterpret_cast<const float4*>(a.sin + at + i));
+  }
+  if (a.rope_form == MODDIT_ROPE_EVEN_COS_ODD_SIN) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        cs[2 * i + 1] = cs[2 * i];
-        sn[2 * i] = sn[2 * i + 1];
-      }
+    for (int i = 0; i < 4; ++i) {
+      t.cs[2 * i + 1] = t.cs[2 * i];
+      t.sn[2 * i] = t.sn[2 * i + 1];
     }
   }
-  // out0 = y0 cs0 - y1 sn0, out1 = y0 sn1 + y1 cs1
+  return t;
+}
+__device__ __forceinline__ void turn_back(const Turn& t, float (&g)[8]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float g0 = g[2 * i], g1 = g[2 * i + 1];
-    g[2 * i] = g0 * cs[2 * i] + g1 * sn[2 * i + 1];
-    g[2 * i + 1] = g1 * cs[2 * i + 1] - g0 * sn[2 * i];
+    g[2 * i] = g0 * t.cs[2 * i] + g1 * t.sn[2 * i + 1];
+    g[2 * i + 1] = g1 * t.cs[2 * i + 1] - g0 * t.sn[2 * i];
   }
 }
 
-// Grid: x = persistent blocks, y = tensor.  An item is kRows rows per thread of one head; neighbouring items are the heads of
-// the same tokens, so the table rows are shared.
+__device__ __forceinline__ uint4 load16(const void* p, bool in) {
+  return in ? __ldg(static_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
+}
+
+// Grid: x = persistent blocks, y = tensor.  An item is kRows rows per thread of `heads_per_item` heads: a thread has the same
+// columns of the same tokens in every head, so the rotary factors are read once and stay in registers (float32 tables of D
+// values weigh more per row and head than the rows themselves: through the L2 for every head they were the bound).  kHeads
+// heads are loaded before the first is worked on.
 template <typename T, int D, int kNorm>
-__global__ void __launch_bounds__(kThreads) prologue_bwd_kernel(const __grid_constant__ BwdArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) prologue_bwd_kernel(const __grid_constant__ BwdArgs a) {
   constexpr int kTpr = D / 8;                     // threads per row
   constexpr int kRpp = kThreads / kTpr;           // rows per pass
   constexpr float kInvD = 1.0f / D;
@@ -138,85 +156,107 @@ __global__ void __launch_bounds__(kThreads) prologue_bwd_kernel(const __grid_con
   T* __restrict__ dx = static_cast<T*>(a.dx[which]);
   const int c = threadIdx.x % kTpr, rg = threadIdx.x / kTpr;
   const bool normed = kNorm != MODDIT_NORM_NONE && which < 2;
+  const bool turned = which < 2 && a.cos != nullptr;
+  const T* __restrict__ x_in = normed ? static_cast<const T*>(a.x[which]) : nullptr;
   float w[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) w[i] = 1.f;
   if (normed && a.weight[which] != nullptr) unpack<T>(__ldg(static_cast<const uint4*>(a.weight[which]) + c), w);
   float dw[8] = {}, db[8] = {};
-  const int blocks = (a.S + kRows * kRpp - 1) / (kRows * kRpp);
-  const int64_t items = static_cast<int64_t>(a.B) * blocks * a.H;
-  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const int h = static_cast<int>(item % a.H);
-    const int64_t bt = item / a.H;
-    const int b = static_cast<int>(bt / blocks);
-    const int s0 = static_cast<int>(bt - static_cast<int64_t>(b) * blocks) * kRows * kRpp + rg;
-    const T* gp = g_in + ((static_cast<int64_t>(b) * a.H + h) * a.N_out + a.src_row0) * D + c * 8;
-    const int64_t tok0 = static_cast<int64_t>(b) * a.S;
-    uint4 gv[kRows], xv[kRows];
+
+  auto work = [&](uint4 gv, uint4 xv, const Turn& turn, bool in) -> uint4 {
+    float g[8];
+    unpack<T>(gv, g);
+    if (turned) turn_back(turn, g);
+    if (normed) {
+      float x[8];
+      unpack<T>(xv, x);
+      if constexpr (kNorm == MODDIT_NORM_RMS_HEAD) {
+        float ss = 0.f, sg = 0.f;
 #pragma unroll
-    for (int u = 0; u < kRows; ++u) {
-      const int s = s0 + u * kRpp;
-      const bool in = s < a.S;
-      gv[u] = in ? __ldg(reinterpret_cast<const uint4*>(gp + static_cast<int64_t>(s) * D)) : make_uint4(0, 0, 0, 0);
-      if (normed)
-        xv[u] = in ? __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.x[which]) + (tok0 + s) * a.token_stride + h * D + c * 8))
-                   : make_uint4(0, 0, 0, 0);
-    }
-#pragma unroll
-    for (int u = 0; u < kRows; ++u) {
-      const int s = s0 + u * kRpp;
-      uint4 res = gv[u];
-      if (which < 2 && (normed || a.cos != nullptr)) {
-        float g[8];
-        unpack<T>(gv[u], g);
-        if (s < a.S) unrotate<D>(a, s, c, g);
-        if (normed) {
-          float x[8];
-          unpack<T>(xv[u], x);
-          if constexpr (kNorm == MODDIT_NORM_RMS_HEAD) {
-            float ss = 0.f, sg = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              ss = fmaf(x[i], x[i], ss);
-              sg = fmaf(g[i] * w[i], x[i], sg);
-            }
-            const float ms = lane_sum<kTpr>(ss) * kInvD;
-            const float r = s < a.S ? rsqrtf(ms + a.eps) : 0.f;     // rows past the end add nothing, eps = 0 included
-            const float f = -r * r * (lane_sum<kTpr>(sg) * kInvD);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              dw[i] = fmaf(g[i], x[i] * r, dw[i]);
-              g[i] = r * fmaf(x[i], f, g[i] * w[i]);
-            }
-          } else if constexpr (kNorm == MODDIT_NORM_LAYER) {
-            float sx = 0.f, sg = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              sx += x[i];
-              sg = fmaf(g[i], w[i], sg);
-            }
-            const float mean = lane_sum<kTpr>(sx) * kInvD, mg = lane_sum<kTpr>(sg) * kInvD;
-            float ss = 0.f, sgx = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              x[i] -= mean;
-              ss = fmaf(x[i], x[i], ss);
-              sgx = fmaf(g[i] * w[i], x[i], sgx);
-            }
-            const float ms = lane_sum<kTpr>(ss) * kInvD;
-            const float r = s < a.S ? rsqrtf(ms + a.eps) : 0.f;     // rows past the end add nothing, eps = 0 included
-            const float f = -r * r * (lane_sum<kTpr>(sgx) * kInvD);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              dw[i] = fmaf(g[i], x[i] * r, dw[i]);
-              db[i] += g[i];
-              g[i] = r * (fmaf(x[i], f, g[i] * w[i]) - mg);
-            }
-          }
+        for (int i = 0; i < 8; ++i) {
+          ss = fmaf(x[i], x[i], ss);
+          sg = fmaf(g[i] * w[i], x[i], sg);
         }
-        res = pack8<T>(g);
+        const float ms = lane_sum<kTpr>(ss) * kInvD;
+        const float r = in ? rsqrtf(ms + a.eps) : 0.f;     // rows past the end add nothing, eps = 0 included
+        const float f = -r * r * (lane_sum<kTpr>(sg) * kInvD);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          dw[i] = fmaf(g[i], x[i] * r, dw[i]);
+          g[i] = r * fmaf(x[i], f, g[i] * w[i]);
+        }
+      } else if constexpr (kNorm == MODDIT_NORM_LAYER) {
+        float sx = 0.f, sg = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          sx += x[i];
+          sg = fmaf(g[i], w[i], sg);
+        }
+        const float mean = lane_sum<kTpr>(sx) * kInvD, mg = lane_sum<kTpr>(sg) * kInvD;
+        float ss = 0.f, sgx = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          x[i] -= mean;
+          ss = fmaf(x[i], x[i], ss);
+          sgx = fmaf(g[i] * w[i], x[i], sgx);
+        }
+        const float ms = lane_sum<kTpr>(ss) * kInvD;
+        const float r = in ? rsqrtf(ms + a.eps) : 0.f;
+        const float f = -r * r * (lane_sum<kTpr>(sgx) * kInvD);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          dw[i] = fmaf(g[i], x[i] * r, dw[i]);
+          db[i] += g[i];
+          g[i] = r * (fmaf(x[i], f, g[i] * w[i]) - mg);
+        }
       }
-      if (s < a.S) *reinterpret_cast<uint4*>(dx + (tok0 + s) * a.out_stride + h * D + c * 8) = res;
+    }
+    return pack8<T>(g);
+  };
+
+  const int tiles = (a.S + kRows * kRpp - 1) / (kRows * kRpp);
+  const int chunks = (a.H + a.heads_per_item - 1) / a.heads_per_item;
+  const int64_t items = static_cast<int64_t>(a.B) * tiles * chunks;
+  const int64_t head_rows = static_cast<int64_t>(a.N_out) * D;
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int chunk = static_cast<int>(item % chunks);
+    const int64_t bt = item / chunks;
+    const int b = static_cast<int>(bt / tiles);
+    const int s0 = static_cast<int>(bt - static_cast<int64_t>(b) * tiles) * kRows * kRpp + rg;
+    const int h0 = chunk * a.heads_per_item, h1 = min(a.H, h0 + a.heads_per_item);
+    const T *gp[kRows], *xp[kRows];
+    T* dp[kRows];
+    bool in[kRows];
+    Turn turn[kRows];
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) {
+      const int s = s0 + u * kRpp;
+      const int64_t tok = static_cast<int64_t>(b) * a.S + s;
+      in[u] = s < a.S;
+      gp[u] = g_in + (static_cast<int64_t>(b) * a.H * a.N_out + a.src_row0 + s) * D + c * 8;
+      xp[u] = x_in + tok * a.token_stride + c * 8;
+      dp[u] = dx + tok * a.out_stride + c * 8;
+      if (turned) turn[u] = turn_of<D>(a, s, c);
+    }
+    for (int h = h0; h < h1; h += kHeads) {
+      uint4 gv[kHeads][kRows], xv[kHeads][kRows];
+#pragma unroll
+      for (int j = 0; j < kHeads; ++j)
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) {
+          const bool there = in[u] && h + j < h1;
+          gv[j][u] = load16(gp[u] + (h + j) * head_rows, there);
+          if (normed) xv[j][u] = load16(xp[u] + (h + j) * D, there);
+        }
+#pragma unroll
+      for (int j = 0; j < kHeads; ++j)
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) {
+          const bool there = in[u] && h + j < h1;
+          const uint4 res = (normed || turned) ? work(gv[j][u], xv[j][u], turn[u], there) : gv[j][u];
+          if (there) *reinterpret_cast<uint4*>(dp[u] + (h + j) * D) = res;
+        }
     }
   }
   if (normed && a.part[which] != nullptr) {
@@ -236,13 +276,17 @@ __global__ void __launch_bounds__(kThreads) prologue_bwd_kernel(const __grid_con
 
 // Normalisation over all heads of a token.  A block has one token per warp at a time.  First every warp sums x^2 and g w x
 // over its token; then a thread takes fixed pieces of eight columns through the block's tokens, whose rows it reads again
-// (they are in the L2), writes dx and adds to its columns' weight gradient, which lives in shared memory.
+// (from the L2), writes dx and adds to its columns' weight gradient, which lives in shared memory.  A piece lies at the same
+// columns of its head for all pieces of a lane or thread, so the rotary factors are read once a token: in the second part from
+// shared memory, where the first part's lanes have put them.
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) prologue_bwd_all_heads_kernel(const __grid_constant__ BwdArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) prologue_bwd_all_heads_kernel(const __grid_constant__ BwdArgs a) {
   constexpr int kTpr = D / 8;
   constexpr int kTokens = kThreads / 32;
+  constexpr int kBatch = 4;                       // pieces in flight per lane in the first part
   extern __shared__ float dw_s[];                 // H * D
   __shared__ float r_s[kTokens], f_s[kTokens];
+  __shared__ __align__(16) float cs_s[kTokens][D], sn_s[kTokens][D];
   const int which = blockIdx.y;
   const T* __restrict__ g_in = static_cast<const T*>(a.g[which]);
   if (g_in == nullptr) return;
@@ -252,32 +296,42 @@ __global__ void __launch_bounds__(kThreads) prologue_bwd_all_heads_kernel(const 
   const int W = a.H * D, pieces = W / 8;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const bool sums = which < 2 && a.part[which] != nullptr;
+  const bool turned = which < 2 && a.cos != nullptr;
   if (sums)
     for (int i = threadIdx.x; i < W; i += kThreads) dw_s[i] = 0.f;
   const float inv_w = 1.f / static_cast<float>(W);
   const int groups = (a.S + kTokens - 1) / kTokens;
-  auto g_at = [&](int b, int s, int p) {
-    return reinterpret_cast<const uint4*>(g_in + ((static_cast<int64_t>(b) * a.H + p / kTpr) * a.N_out + a.src_row0 + s) * D) + p % kTpr;
-  };
-  auto x_at = [&](int b, int s, int p) {
-    return reinterpret_cast<const uint4*>(x_in + (static_cast<int64_t>(b) * a.S + s) * a.token_stride) + p;
+  const int64_t head_rows = static_cast<int64_t>(a.N_out) * D;
+  auto weights = [&](int p, float (&w)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = 1.f;
+    if (wp != nullptr) unpack<T>(__ldg(wp + p), w);
   };
   for (int64_t grp = blockIdx.x; grp < static_cast<int64_t>(a.B) * groups; grp += gridDim.x) {
     const int b = static_cast<int>(grp / groups);
     const int s0 = static_cast<int>(grp - static_cast<int64_t>(b) * groups) * kTokens;
+    const T* g0 = g_in + (static_cast<int64_t>(b) * a.H * a.N_out + a.src_row0 + s0) * D;        // token s0 of head 0
+    const T* x0 = x_in + (static_cast<int64_t>(b) * a.S + s0) * a.token_stride;
+    T* d0 = dx + (static_cast<int64_t>(b) * a.S + s0) * a.out_stride;
     if (which < 2) {
-      const int s = s0 + warp;
+      const bool in = s0 + warp < a.S;
+      const Turn turn = turn_of<D>(a, in ? s0 + warp : -1, lane % kTpr);
       float ss = 0.f, sg = 0.f;
-      if (s < a.S) {
-#pragma unroll 4
-        for (int p = lane; p < pieces; p += 32) {
-          float g[8], x[8], w[8];
-          unpack<T>(__ldg(g_at(b, s, p)), g);
-          unpack<T>(__ldg(x_at(b, s, p)), x);
+      for (int p0 = lane; p0 < pieces && in; p0 += 32 * kBatch) {
+        uint4 gv[kBatch], xv[kBatch];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) w[i] = 1.f;
-          if (wp != nullptr) unpack<T>(__ldg(wp + p), w);
-          unrotate<D>(a, s, p % kTpr, g);
+        for (int j = 0; j < kBatch; ++j) {
+          const int p = p0 + 32 * j;
+          gv[j] = load16(g0 + (p / kTpr) * head_rows + warp * D + (p % kTpr) * 8, p < pieces);
+          xv[j] = load16(x0 + warp * a.token_stride + p * 8, p < pieces);
+        }
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          float g[8], x[8], w[8];
+          unpack<T>(gv[j], g);
+          unpack<T>(xv[j], x);
+          weights(min(p0 + 32 * j, pieces - 1), w);
+          if (turned) turn_back(turn, g);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             ss = fmaf(x[i], x[i], ss);
@@ -288,28 +342,48 @@ __global__ void __launch_bounds__(kThreads) prologue_bwd_all_heads_kernel(const 
       ss = lane_sum<32>(ss);
       sg = lane_sum<32>(sg);
       __syncthreads();                            // the previous group's factors have been read
+      if (turned && lane < kTpr) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          cs_s[warp][lane * 8 + i] = turn.cs[i];
+          sn_s[warp][lane * 8 + i] = turn.sn[i];
+        }
+      }
       if (lane == 0) {
-        const float r = rsqrtf(ss * inv_w + a.eps);
+        const float r = in ? rsqrtf(ss * inv_w + a.eps) : 0.f;
         r_s[warp] = r;
         f_s[warp] = -r * r * (sg * inv_w);
       }
       __syncthreads();
     }
     for (int p = threadIdx.x; p < pieces; p += kThreads) {
-      float w[8], dw[8] = {};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = 1.f;
-      if (wp != nullptr) unpack<T>(__ldg(wp + p), w);
+      const int c = p % kTpr;
+      const T* gp = g0 + (p / kTpr) * head_rows + c * 8;
+      uint4 gv[kTokens], xv[kTokens];
 #pragma unroll
       for (int t = 0; t < kTokens; ++t) {
-        const int s = s0 + t;
-        if (s >= a.S) break;
-        uint4 res = __ldg(g_at(b, s, p));
+        const bool in = s0 + t < a.S;
+        gv[t] = load16(gp + t * D, in);
+        if (which < 2) xv[t] = load16(x0 + t * a.token_stride + p * 8, in);
+      }
+      float w[8], dw[8] = {};
+      if (which < 2) weights(p, w);
+#pragma unroll
+      for (int t = 0; t < kTokens; ++t) {
+        uint4 res = gv[t];
         if (which < 2) {
           float g[8], x[8];
-          unpack<T>(res, g);
-          unpack<T>(__ldg(x_at(b, s, p)), x);
-          unrotate<D>(a, s, p % kTpr, g);
+          unpack<T>(gv[t], g);
+          unpack<T>(xv[t], x);
+          if (turned) {
+            Turn turn;
+#pragma unroll
+            for (int i = 0; i < 8; i += 4) {
+              *reinterpret_cast<float4*>(turn.cs + i) = *reinterpret_cast<const float4*>(&cs_s[t][c * 8 + i]);
+              *reinterpret_cast<float4*>(turn.sn + i) = *reinterpret_cast<const float4*>(&sn_s[t][c * 8 + i]);
+            }
+            turn_back(turn, g);
+          }
           const float r = r_s[t], f = f_s[t];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
@@ -318,7 +392,7 @@ __global__ void __launch_bounds__(kThreads) prologue_bwd_all_heads_kernel(const 
           }
           res = pack8<T>(g);
         }
-        *(reinterpret_cast<uint4*>(dx + (static_cast<int64_t>(b) * a.S + s) * a.out_stride) + p) = res;
+        if (s0 + t < a.S) *reinterpret_cast<uint4*>(d0 + t * a.out_stride + p * 8) = res;
       }
       if (sums)
 #pragma unroll
@@ -356,13 +430,20 @@ __global__ void __launch_bounds__(kThreads) prologue_bwd_sums_kernel(const __gri
 }
 
 // Persistent blocks per tensor: a fixed number, whatever the GPU, so that the order of the sums does not depend on it; more
-// than the items of a tensor would only add rows of zeros.
-constexpr int kBlocksPerHead = 592;      // per-head kernel
+// than the items of a tensor would only add rows of zeros.  Short inputs are cut into fewer heads per item, so that there are
+// that many.
+constexpr int kBlocksPerHead = 296;
 constexpr int kBlocksAllHeads = 296;
+int heads_per_item(int B, int S, int H, int D) {
+  const int64_t tiles = static_cast<int64_t>(B) * ceil_div(S, kRows * kThreads / (D / 8));
+  const int chunks = static_cast<int>(std::min<int64_t>(H, (kBlocksPerHead + tiles - 1) / tiles));
+  return ceil_div(H, chunks);
+}
 int blocks_for(int B, int S, int H, int D, int norm_kind) {
   if (norm_kind == MODDIT_NORM_RMS_ALL_HEADS)
     return static_cast<int>(std::min<int64_t>(kBlocksAllHeads, static_cast<int64_t>(B) * ceil_div(S, kThreads / 32)));
-  return static_cast<int>(std::min<int64_t>(kBlocksPerHead, static_cast<int64_t>(B) * ceil_div(S, kRows * kThreads / (D / 8)) * H));
+  return static_cast<int>(std::min<int64_t>(kBlocksPerHead, static_cast<int64_t>(B) * ceil_div(S, kRows * kThreads / (D / 8)) *
+                                                                ceil_div(H, heads_per_item(B, S, H, D))));
 }
 
 template <typename T, int D>
@@ -478,6 +559,7 @@ extern "C" int moddit_qkv_prologue_bwd(const void* dq, const void* dk, const voi
   a.B = B; a.S = S; a.H = H; a.N_out = N_out; a.src_row0 = src_row0;
   a.rope_form = rope_form; a.rope_lo = rope_lo; a.rope_hi = rope_hi;
   a.eps = eps;
+  a.heads_per_item = heads_per_item(B, S, H, D);
   cudaStream_t st = as_stream(stream);
   if (dtype == MODDIT_BF16)
     return D == 128 ? launch_bwd<__nv_bfloat16, 128>(a, norm_kind, blocks, sums, st) : launch_bwd<__nv_bfloat16, 64>(a, norm_kind, blocks, sums, st);
