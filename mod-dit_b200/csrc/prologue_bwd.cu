@@ -25,7 +25,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kRows = 2;                // rows per thread of an item of the per-head kernel
-constexpr int kHeads = 2;               // heads of them in flight
+constexpr int kStages = 5;              // heads of them in flight
 
 template <typename T>
 struct Pair;
@@ -93,7 +93,8 @@ struct BwdArgs {
 struct Turn {
   float cs[8], sn[8];
 };
-template <int D>
+// kPair: tables of one value per pair (MODDIT_ROPE_PAIR)
+template <int D, bool kPair>
 __device__ __forceinline__ Turn turn_of(const BwdArgs& a, int s, int c) {
   Turn t;
   if (a.cos == nullptr || s < a.rope_lo || s >= a.rope_hi) {
@@ -101,7 +102,7 @@ __device__ __forceinline__ Turn turn_of(const BwdArgs& a, int s, int c) {
     for (int i = 0; i < 8; ++i) t.cs[i] = 1.f, t.sn[i] = 0.f;
     return t;
   }
-  if (a.rope_form == MODDIT_ROPE_PAIR) {
+  if constexpr (kPair) {
     const int64_t at = static_cast<int64_t>(s - a.rope_lo) * (D / 2) + c * 4;
     const float4 c4 = __ldg(reinterpret_cast<const float4*>(a.cos + at)), s4 = __ldg(reinterpret_cast<const float4*>(a.sin + at));
     const float cv[4] = {c4.x, c4.y, c4.z, c4.w}, sv[4] = {s4.x, s4.y, s4.z, s4.w};
@@ -110,22 +111,25 @@ __device__ __forceinline__ Turn turn_of(const BwdArgs& a, int s, int c) {
       t.cs[2 * i] = t.cs[2 * i + 1] = cv[i];
       t.sn[2 * i] = t.sn[2 * i + 1] = sv[i];
     }
-    return t;
-  }
-  const int64_t at = static_cast<int64_t>(s - a.rope_lo) * D + c * 8;
+  } else {
+    const int64_t at = static_cast<int64_t>(s - a.rope_lo) * D + c * 8;
 #pragma unroll
-  for (int i = 0; i < 8; i += 4) {
-    *reinterpret_cast<float4*>(t.cs + i) = __ldg(reinterpret_cast<const float4*>(a.cos + at + i));
-    *reinterpret_cast<float4*>(t.sn + i) = __ldg(reinterpret_cast<const float4*>(a.sin + at + i));
-  }
-  if (a.rope_form == MODDIT_ROPE_EVEN_COS_ODD_SIN) {
+    for (int i = 0; i < 8; i += 4) {
+      *reinterpret_cast<float4*>(t.cs + i) = __ldg(reinterpret_cast<const float4*>(a.cos + at + i));
+      *reinterpret_cast<float4*>(t.sn + i) = __ldg(reinterpret_cast<const float4*>(a.sin + at + i));
+    }
+    if (a.rope_form == MODDIT_ROPE_EVEN_COS_ODD_SIN) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      t.cs[2 * i + 1] = t.cs[2 * i];
-      t.sn[2 * i] = t.sn[2 * i + 1];
+      for (int i = 0; i < 4; ++i) {
+        t.cs[2 * i + 1] = t.cs[2 * i];
+        t.sn[2 * i] = t.sn[2 * i + 1];
+      }
     }
   }
   return t;
+}
+__device__ __forceinline__ uint4 load16(const void* p, bool in) {
+  return in ? __ldg(static_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
 }
 __device__ __forceinline__ void turn_back(const Turn& t, float (&g)[8]) {
 #pragma unroll
@@ -136,20 +140,25 @@ __device__ __forceinline__ void turn_back(const Turn& t, float (&g)[8]) {
   }
 }
 
-__device__ __forceinline__ uint4 load16(const void* p, bool in) {
-  return in ? __ldg(static_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
+// 16 bytes into shared memory, zeros where `in` is false (src is not read then)
+__device__ __forceinline__ void copy_async16(void* dst, const void* src, bool in) {
+  const uint32_t d = static_cast<uint32_t>(__cvta_generic_to_shared(dst));
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(__cvta_generic_to_global(src)), "r"(in ? 16 : 0)
+               : "memory");
 }
 
 // Grid: x = persistent blocks, y = tensor.  An item is kRows rows per thread of `heads_per_item` heads: a thread has the same
 // columns of the same tokens in every head, so the rotary factors are read once and stay in registers (float32 tables of D
-// values weigh more per row and head than the rows themselves: through the L2 for every head they were the bound).  kHeads
-// heads are loaded before the first is worked on.
-template <typename T, int D, int kNorm>
+// values weigh more per row and head than the rows themselves: through the L2 for every head they were the bound).  A thread
+// copies its pieces of the next kStages - 1 heads asynchronously into places of its own in shared memory, so that bytes are in
+// flight while it computes, without registers for them and without a barrier.  57,728 tokens x 16 heads of 128: loads into
+// registers, two heads at a time, 400 us; like this 320.
+template <typename T, int D, int kNorm, bool kPair>
 __global__ void __launch_bounds__(kThreads, 2) prologue_bwd_kernel(const __grid_constant__ BwdArgs a) {
   constexpr int kTpr = D / 8;                     // threads per row
   constexpr int kRpp = kThreads / kTpr;           // rows per pass
   constexpr float kInvD = 1.0f / D;
-  __shared__ float red[kRpp][D];
+  extern __shared__ uint4 ring[];                 // [kStages][kRows][g, x][kThreads]; at the end the sums of kRpp rows
   const int which = blockIdx.y;
   const T* __restrict__ g_in = static_cast<const T*>(a.g[which]);
   if (g_in == nullptr) return;
@@ -237,37 +246,47 @@ __global__ void __launch_bounds__(kThreads, 2) prologue_bwd_kernel(const __grid_
       gp[u] = g_in + (static_cast<int64_t>(b) * a.H * a.N_out + a.src_row0 + s) * D + c * 8;
       xp[u] = x_in + tok * a.token_stride + c * 8;
       dp[u] = dx + tok * a.out_stride + c * 8;
-      if (turned) turn[u] = turn_of<D>(a, s, c);
+      if (turned) turn[u] = turn_of<D, kPair>(a, s, c);
     }
-    for (int h = h0; h < h1; h += kHeads) {
-      uint4 gv[kHeads][kRows], xv[kHeads][kRows];
-#pragma unroll
-      for (int j = 0; j < kHeads; ++j)
-#pragma unroll
-        for (int u = 0; u < kRows; ++u) {
-          const bool there = in[u] && h + j < h1;
-          gv[j][u] = load16(gp[u] + (h + j) * head_rows, there);
-          if (normed) xv[j][u] = load16(xp[u] + (h + j) * D, there);
-        }
-#pragma unroll
-      for (int j = 0; j < kHeads; ++j)
+    auto fetch = [&](int h) {
+      if (h < h1) {
+        uint4* to = ring + ((h - h0) % kStages) * (2 * kRows * kThreads) + threadIdx.x;
 #pragma unroll
         for (int u = 0; u < kRows; ++u) {
-          const bool there = in[u] && h + j < h1;
-          const uint4 res = (normed || turned) ? work(gv[j][u], xv[j][u], turn[u], there) : gv[j][u];
-          if (there) *reinterpret_cast<uint4*>(dp[u] + (h + j) * D) = res;
+          copy_async16(to + 2 * u * kThreads, in[u] ? gp[u] + h * head_rows : g_in, in[u]);
+          if (normed) copy_async16(to + (2 * u + 1) * kThreads, in[u] ? xp[u] + h * D : x_in, in[u]);
         }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    for (int j = 0; j < kStages - 1; ++j) fetch(h0 + j);
+    for (int h = h0; h < h1; ++h) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+      const uint4* from = ring + ((h - h0) % kStages) * (2 * kRows * kThreads) + threadIdx.x;
+      uint4 gv[kRows], xv[kRows];
+#pragma unroll
+      for (int u = 0; u < kRows; ++u) {
+        gv[u] = from[2 * u * kThreads];
+        if (normed) xv[u] = from[(2 * u + 1) * kThreads];
+      }
+      fetch(h + kStages - 1);
+#pragma unroll
+      for (int u = 0; u < kRows; ++u) {
+        const uint4 res = (normed || turned) ? work(gv[u], xv[u], turn[u], in[u]) : gv[u];
+        if (in[u]) *reinterpret_cast<uint4*>(dp[u] + h * D) = res;
+      }
     }
   }
   if (normed && a.part[which] != nullptr) {
+    float* red = reinterpret_cast<float*>(ring);
     for (int k = 0; k < (kNorm == MODDIT_NORM_LAYER ? 2 : 1); ++k) {
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < 8; ++i) red[rg][c * 8 + i] = k ? db[i] : dw[i];
+      for (int i = 0; i < 8; ++i) red[rg * D + c * 8 + i] = k ? db[i] : dw[i];
       __syncthreads();
       if (threadIdx.x < D) {
         float t = 0.f;
-        for (int j = 0; j < kRpp; ++j) t += red[j][threadIdx.x];
+        for (int j = 0; j < kRpp; ++j) t += red[j * D + threadIdx.x];
         a.part[which][(static_cast<int64_t>(k) * gridDim.x + blockIdx.x) * D + threadIdx.x] = t;
       }
     }
@@ -279,7 +298,10 @@ __global__ void __launch_bounds__(kThreads, 2) prologue_bwd_kernel(const __grid_
 // (from the L2), writes dx and adds to its columns' weight gradient, which lives in shared memory.  A piece lies at the same
 // columns of its head for all pieces of a lane or thread, so the rotary factors are read once a token: in the second part from
 // shared memory, where the first part's lanes have put them.
-template <typename T, int D>
+// 8,640 tokens of 40 x 128: 179 us, 61 % of the measured copy bandwidth; bound by instructions and the two parts' latencies.
+// Slower: a group's rows kept in shared memory between the parts, copied a group ahead (204 us with two blocks an SM, 257 with
+// one: block-wide sums and fewer warps), half as many tokens in flight with three or four blocks an SM (190 - 230).
+template <typename T, int D, bool kPair>
 __global__ void __launch_bounds__(kThreads, 2) prologue_bwd_all_heads_kernel(const __grid_constant__ BwdArgs a) {
   constexpr int kTpr = D / 8;
   constexpr int kTokens = kThreads / 32;
@@ -315,16 +337,21 @@ __global__ void __launch_bounds__(kThreads, 2) prologue_bwd_all_heads_kernel(con
     T* d0 = dx + (static_cast<int64_t>(b) * a.S + s0) * a.out_stride;
     if (which < 2) {
       const bool in = s0 + warp < a.S;
-      const Turn turn = turn_of<D>(a, in ? s0 + warp : -1, lane % kTpr);
+      const Turn turn = turn_of<D, kPair>(a, in ? s0 + warp : -1, lane % kTpr);
       float ss = 0.f, sg = 0.f;
+      const T* gp = g0 + (lane / kTpr) * head_rows + warp * D + (lane % kTpr) * 8;
+      const T* xp = x0 + warp * a.token_stride + lane * 8;
+      const int64_t step = (32 / kTpr) * head_rows;
       for (int p0 = lane; p0 < pieces && in; p0 += 32 * kBatch) {
         uint4 gv[kBatch], xv[kBatch];
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
-          const int p = p0 + 32 * j;
-          gv[j] = load16(g0 + (p / kTpr) * head_rows + warp * D + (p % kTpr) * 8, p < pieces);
-          xv[j] = load16(x0 + warp * a.token_stride + p * 8, p < pieces);
+          const bool there = p0 + 32 * j < pieces;
+          gv[j] = load16(gp, there);
+          xv[j] = load16(xp + j * 256, there);
+          gp += step;
         }
+        xp += kBatch * 256;
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
           float g[8], x[8], w[8];
@@ -387,8 +414,9 @@ __global__ void __launch_bounds__(kThreads, 2) prologue_bwd_all_heads_kernel(con
           const float r = r_s[t], f = f_s[t];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            dw[i] = fmaf(g[i], x[i] * r, dw[i]);
-            g[i] = r * fmaf(x[i], f, g[i] * w[i]);
+            const float xr = x[i] * r;
+            dw[i] = fmaf(g[i], xr, dw[i]);
+            g[i] = fmaf(xr, f, r * (g[i] * w[i]));
           }
           res = pack8<T>(g);
         }
@@ -434,6 +462,7 @@ __global__ void __launch_bounds__(kThreads) prologue_bwd_sums_kernel(const __gri
 // that many.
 constexpr int kBlocksPerHead = 296;
 constexpr int kBlocksAllHeads = 296;
+constexpr int kMaxWidth = 48 * 1024;                 // values of a token: their sums lie in shared memory
 int heads_per_item(int B, int S, int H, int D) {
   const int64_t tiles = static_cast<int64_t>(B) * ceil_div(S, kRows * kThreads / (D / 8));
   const int chunks = static_cast<int>(std::min<int64_t>(H, (kBlocksPerHead + tiles - 1) / tiles));
@@ -446,26 +475,28 @@ int blocks_for(int B, int S, int H, int D, int norm_kind) {
                                                                 ceil_div(H, heads_per_item(B, S, H, D))));
 }
 
+template <typename T, int D, bool kPair>
+int launch_rows(const BwdArgs& a, int norm_kind, int blocks, cudaStream_t st) {
+  if (norm_kind == MODDIT_NORM_RMS_ALL_HEADS) {
+    auto kernel = prologue_bwd_all_heads_kernel<T, D, kPair>;
+    const size_t smem = sizeof(float) * a.H * D;
+    if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem)) return rc;
+    kernel<<<dim3(blocks, 3), kThreads, smem, st>>>(a);
+  } else {
+    auto kernel = norm_kind == MODDIT_NORM_NONE       ? prologue_bwd_kernel<T, D, MODDIT_NORM_NONE, kPair>
+                  : norm_kind == MODDIT_NORM_RMS_HEAD ? prologue_bwd_kernel<T, D, MODDIT_NORM_RMS_HEAD, kPair>
+                                                      : prologue_bwd_kernel<T, D, MODDIT_NORM_LAYER, kPair>;
+    const size_t smem = sizeof(uint4) * kStages * kRows * 2 * kThreads;
+    if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem)) return rc;
+    kernel<<<dim3(blocks, 3), kThreads, smem, st>>>(a);
+  }
+  return MODDIT_OK;
+}
+
 template <typename T, int D>
 int launch_bwd(const BwdArgs& a, int norm_kind, int blocks, const SumArgs& sums, cudaStream_t st) {
-  const dim3 grid(blocks, 3);
-  switch (norm_kind) {
-    case MODDIT_NORM_NONE:
-      prologue_bwd_kernel<T, D, MODDIT_NORM_NONE><<<grid, kThreads, 0, st>>>(a);
-      break;
-    case MODDIT_NORM_RMS_HEAD:
-      prologue_bwd_kernel<T, D, MODDIT_NORM_RMS_HEAD><<<grid, kThreads, 0, st>>>(a);
-      break;
-    case MODDIT_NORM_LAYER:
-      prologue_bwd_kernel<T, D, MODDIT_NORM_LAYER><<<grid, kThreads, 0, st>>>(a);
-      break;
-    default: {
-      auto kernel = prologue_bwd_all_heads_kernel<T, D>;
-      const size_t smem = sizeof(float) * a.H * D;
-      if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem)) return rc;
-      kernel<<<grid, kThreads, smem, st>>>(a);
-    }
-  }
+  const bool pair = a.rope_form == MODDIT_ROPE_PAIR;
+  if (int rc = pair ? launch_rows<T, D, true>(a, norm_kind, blocks, st) : launch_rows<T, D, false>(a, norm_kind, blocks, st)) return rc;
   MODDIT_CHECK_LAUNCH("prologue_bwd_kernel");
   if (sums.out[0][0] || sums.out[0][1] || sums.out[1][0] || sums.out[1][1]) {
     const int width = norm_kind == MODDIT_NORM_RMS_ALL_HEADS ? a.H * D : D;
@@ -529,13 +560,17 @@ extern "C" int moddit_qkv_prologue_bwd(const void* dq, const void* dk, const voi
                        "norm_kind %d has no such parameter", norm_kind);
     }
   MODDIT_CHECK_ARG((rope_cos == nullptr) == (rope_sin == nullptr), "rope_cos and rope_sin go together");
+  if (rope_cos == nullptr) rope_form = MODDIT_ROPE_PAIR;
+  if (norm_kind == MODDIT_NORM_RMS_ALL_HEADS)
+    MODDIT_CHECK_ARG(static_cast<int64_t>(B) * S <= (1ll << 30), "B * S = %lld tokens are too many", static_cast<long long>(B) * S);
   if (rope_cos != nullptr) {
     MODDIT_CHECK_ARG(aligned16(rope_cos) && aligned16(rope_sin), "rotary tables must be 16-byte aligned");
     MODDIT_CHECK_ARG(0 <= rope_lo && rope_lo <= rope_hi && rope_hi <= S, "rotary range [%d, %d) outside 0..%d", rope_lo, rope_hi, S);
     MODDIT_CHECK_ARG(rope_form >= MODDIT_ROPE_ELEMENTWISE && rope_form <= MODDIT_ROPE_PAIR, "unknown rope_form %d", rope_form);
   }
-  if (norm_kind == MODDIT_NORM_RMS_ALL_HEADS && width > 48 * 1024)
-    return fail(MODDIT_E_UNSUPPORTED, "a normalisation over all heads covers at most 49,152 values, got %lld", static_cast<long long>(width));
+  if (norm_kind == MODDIT_NORM_RMS_ALL_HEADS && width > kMaxWidth)
+    return fail(MODDIT_E_UNSUPPORTED, "a normalisation over all heads covers at most %d values, got %lld", kMaxWidth,
+                static_cast<long long>(width));
   if (any && (workspace == nullptr || !aligned16(workspace) || ws_bytes < moddit_qkv_prologue_bwd_workspace_bytes(B, S, H, D, norm_kind)))
     return fail(MODDIT_E_WORKSPACE, "parameter gradients need a 16-byte aligned workspace of %zu bytes",
                 moddit_qkv_prologue_bwd_workspace_bytes(B, S, H, D, norm_kind));
