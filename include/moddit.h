@@ -329,11 +329,21 @@ int moddit_sparse_attn_fwd(const void* q, const void* k, const void* v, int dtyp
                            float softmax_scale, int q_split, int kv_len_lo, int kv_len_hi, void* out,
                            float* lse, int32_t* status, void* stream);
 
+/* moddit_sparse_attn_fwd that also stores what rounding took from the output: out + out_lo is the row to about 16 (bfloat16) or
+ * 22 bits (float16).  For the backward pass: where a row attends to few keys, dout v^T - delta is a small difference of large
+ * numbers, and a delta from 16-bit rows is wrong by more than it is worth (a row with nearly all of its weight on one key).
+ * out, out_lo and lse must not be NULL. */
+int moddit_sparse_attn_fwd_residual(const void* q, const void* k, const void* v, int dtype, int BH, int N, int D,
+                                    const int32_t* counts, const int32_t* entries, const int32_t* order, int Hm,
+                                    float softmax_scale, int q_split, int kv_len_lo, int kv_len_hi, void* out,
+                                    void* out_lo, float* lse, int32_t* status, void* stream);
+
 /* Gradients of the block-sparse attention: with s = softmax_scale * q.k over the pairs that the forward kept and
  * P = exp(s - lse), computed again tile by tile, and delta = sum(dout * out) per row,
  *   dv = P^T dout,  ds = P * (dout v^T - delta),  dq = softmax_scale * ds k,  dk = softmax_scale * ds^T q.
  * No reference counterpart (the reference runs inference only).  Results do not depend on the order in which blocks run.
  *   q,k,v, Hm, softmax_scale, q_split, kv_len_lo, kv_len_hi : as in the forward;  out, lse : what it gave
+ *   out_lo    : NULL or what moddit_sparse_attn_fwd_residual gave besides: delta is then taken from out + out_lo
  *   dout, dq, dk, dv : (BH, N, D) like q;  none of the outputs may overlap an input
  *   q_counts, q_entries, q_order : lists of moddit_tile_lists;  k_counts, k_entries, k_order : lists of moddit_key_lists for
  *               the same mask (the orders may be NULL)
@@ -343,8 +353,8 @@ int moddit_sparse_attn_fwd(const void* q, const void* k, const void* v, int dtyp
  * never read; all other rows have to be finite, because a tile is multiplied whole where its mask keeps any of it.
  */
 size_t moddit_sparse_attn_bwd_workspace_bytes(int BH, int N);
-int moddit_sparse_attn_bwd(const void* q, const void* k, const void* v, const void* out, const void* dout, const float* lse,
-                           int dtype, int BH, int N, int D, const int32_t* q_counts, const int32_t* q_entries,
+int moddit_sparse_attn_bwd(const void* q, const void* k, const void* v, const void* out, const void* out_lo,
+                           const void* dout, const float* lse, int dtype, int BH, int N, int D, const int32_t* q_counts, const int32_t* q_entries,
                            const int32_t* q_order, const int32_t* k_counts, const int32_t* k_entries,
                            const int32_t* k_order, int Hm, float softmax_scale, int q_split, int kv_len_lo,
                            int kv_len_hi, void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,

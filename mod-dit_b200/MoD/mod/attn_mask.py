@@ -29,6 +29,7 @@ from MoD.mod.get_radial_mask import get_radial_mask
 from MoD.mod.state import is_warmup_complete
 from MoD.mod.triton_flash_sparsity import dense_attention_with_lse, flash_attn_with_sparsity_map
 from moddit_b200 import _lib
+from moddit_b200 import autograd as _autograd
 from moddit_b200 import ops as _ops
 
 
@@ -185,6 +186,30 @@ def _engine_lists(mask: torch.Tensor, block_size: int, seq_len: int):
     return _ops.tile_lists(mask, block_size, seq_len), False
 
 
+def _needs_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+
+
+def _key_lists(mask: torch.Tensor, mask_heads: int, block_size: int, seq_len: int):
+    """Key-side work lists for the backward pass of `_engine_lists`' (or the state's) lists of `mask_heads` heads."""
+    if mask.dim() == 2:
+        mask = mask.unsqueeze(0)
+    nb = (seq_len + block_size - 1) // block_size
+    if mask.shape[-1] != nb or mask.shape[-2] != nb:
+        mask = torch.ones(1, nb, nb, device=mask.device, dtype=torch.bool)
+    return _ops.key_lists(mask[:mask_heads], block_size, seq_len)       # lists of one head serve a mask that all heads share
+
+
+def _dense(query, key, value, kv_len: int):
+    """Dense attention over the first kv_len keys; differentiable where the inputs ask for gradients."""
+    if not _needs_grad(query, key, value):
+        return dense_attention_with_lse(query, key, value, kv_len=kv_len)[0]
+    nb = (query.shape[2] + 127) // 128
+    mask = torch.ones(1, nb, nb, device=query.device, dtype=torch.bool)
+    return _autograd.sparse_attention(query, key, value, _ops.tile_lists(mask, 128, query.shape[2]),
+                                      _ops.key_lists(mask, 128, query.shape[2]), kv_len_lo=kv_len, kv_len_hi=kv_len)
+
+
 def _events(ready):
     if ready is None:
         return ()
@@ -255,7 +280,8 @@ def AttentionSparseEngine(query, key, value, mask, pre_defined_mask=None, video_
 
     Video query rows (index < video_token_num) see the keys below the valid length rounded up to 64, text
     rows see exactly the valid keys - the split the reference gets from its two third-party kernels.
-    One kernel launch covers both; the result is (B,H,S,D).  When the mask is a stand-in that keeps every
+    One kernel launch covers both; the result is (B,H,S,D).  Where query, key or value require gradients the result is
+    differentiable with respect to them, the mask being a constant (not with `_scatter` or `_group_ready`).  When the mask is a stand-in that keeps every
     block (a caller passing a mask of another shape, as the dense steps do), every row sees exactly the valid
     keys, like the reference's dense branch (:268-276).  Whether a full-shape mask happens to be all true is
     not looked up (the reference pays a host synchronisation per call for that): it goes down the sparse
@@ -281,6 +307,9 @@ def AttentionSparseEngine(query, key, value, mask, pre_defined_mask=None, video_
         if query.shape[0] != 1 or lists.counts.shape[0] != query.shape[1]:
             raise ValueError("head groups need a batch of one and one mask per head")
         return _engine_by_head_groups(query, key, value, lists, _group_ready, _scatter, **fwd_kw)
+    if _scatter is None and _needs_grad(query, key, value):
+        return _autograd.sparse_attention(query, key, value, lists, _key_lists(mask, counts.shape[0], block_size, seq_len),
+                                          **fwd_kw)
     return _ops.sparse_attn_fwd(query, key, value, counts, entries, order=order, check_status="deferred",
                                 scatter=_scatter, **fwd_kw)
 
@@ -443,8 +472,7 @@ def SparseAttentionWithMap(
         for ev in _events((kwargs.get('value_ready'), kwargs.get('qk_ready'))) + _events(kwargs.get('head_group_ready')):
             torch.cuda.current_stream(query.device).wait_event(ev)     # inputs still arriving on other streams
         query, key, value = query.contiguous(), key.contiguous(), value.contiguous()
-        valid = _valid_kv(pre_defined_mask, seq_len)
-        output, _ = dense_attention_with_lse(query, key, value, kv_len=valid)
+        output = _dense(query, key, value, _valid_kv(pre_defined_mask, seq_len))
         return output, {'mode': 'warmup', 'mask': None}
     sparse_type = warmup_state['sparse_type']
     if sparse_type == 'svg':
@@ -475,7 +503,7 @@ def SparseAttentionWithMap(
             output, block_sparse_map = compute_block_sparse_map_triton(query, key, value, warmup_state)
             update_warmup(warmup_state, current_step, block_sparse_map.squeeze(0))
         else:
-            output, _ = dense_attention_with_lse(query, key, value, kv_len=_valid_kv(pre_defined_mask, seq_len))
+            output = _dense(query, key, value, _valid_kv(pre_defined_mask, seq_len))
         if current_step == warmup_steps - 1:
             mask_info = predict_mask_from_warmup(warmup_state, seq_len, top_k=warmup_state['top_k'],
                                                  layer_idx=layer_idx)
@@ -536,7 +564,7 @@ def _radial_step(query, key, value, warmup_state, logger, pre_defined_mask, curr
         warmup_state['_radial_sparsity'] = 1.0 - float(mask[0].float().mean())
     if current_step < warmup_state['warmup_steps']:
         logger.info(f"Layer {layer_idx}, Mask Sparsity: {warmup_state['_radial_sparsity']:.3%}")
-        output, _ = dense_attention_with_lse(query, key, value, kv_len=seq_len)
+        output = _dense(query, key, value, seq_len)
         return output, {'mode': 'warmup', 'mask': None}
     output = AttentionSparseEngine(query, key, value, warmup_state['mask'], pre_defined_mask=pre_defined_mask,
                                    video_token_num=warmup_state.get('video_token_num', 0), block_size=bs,
@@ -607,7 +635,7 @@ def _pooled_step(query, key, value, warmup_state, logger, pre_defined_mask, curr
 
     if current_step < warmup_steps - 2:
         wait_value()
-        output, _ = dense_attention_with_lse(query, key, value, kv_len=_valid_kv(pre_defined_mask, seq_len))
+        output = _dense(query, key, value, _valid_kv(pre_defined_mask, seq_len))
         return output, {'mode': 'warmup', 'mask': None}
     if pooled_qk is None:                               # query and key are read by the pooling itself
         for ev in _events(qk_ready) + _events(head_group_ready):
@@ -643,7 +671,7 @@ def _pooled_step(query, key, value, warmup_state, logger, pre_defined_mask, curr
         warmup_state['current_steps'] = current_step + 1
         warmup_state['prev_full_maps'] = dark
         wait_value()
-        output, _ = dense_attention_with_lse(query, key, value, kv_len=_valid_kv(pre_defined_mask, seq_len))
+        output = _dense(query, key, value, _valid_kv(pre_defined_mask, seq_len))
         return output, {'mode': 'warmup', 'mask': None}
     history.append(feats)
     if len(history) > 2:

@@ -93,6 +93,27 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   }
 }
 
+// Eight float32 values as 16-bit ones; with `lo` also what the rounding took from them (gradients subtract sums that nearly
+// cancel and want the output closer than its 16 bits).
+template <bool kBF16, bool kResidual>
+__device__ __forceinline__ void store8(const float (&o)[8], uint4* dst, uint4* lo) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = pack2<kBF16>(o[2 * i], o[2 * i + 1]);
+  *dst = make_uint4(w[0], w[1], w[2], w[3]);
+  if constexpr (kResidual) {
+    uint32_t r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float2 v;
+      if constexpr (kBF16) v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
+      else v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      r[i] = pack2<kBF16>(o[2 * i] - v.x, o[2 * i + 1] - v.y);
+    }
+    *lo = make_uint4(r[0], r[1], r[2], r[3]);
+  }
+}
+
 // Which work item a block has.  The first 2 * n_single blocks have one query tile each, the two of a pair next to each other;
 // the others have a pair.
 struct BlockItem {
@@ -122,12 +143,12 @@ int single_pairs(int sms, int items, int batches, int pairs_beside) {
   return min(items, static_cast<int>(idle * mine / (mine + pairs_beside)));
 }
 
-template <int D, bool kBF16>
+template <int D, bool kBF16, bool kResidual>
 __global__ void __launch_bounds__(kThreads, 1) sparse_attn_fwd_kernel(
     const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
     const __grid_constant__ CUtensorMap tm_v, const int32_t* __restrict__ counts,
     const int32_t* __restrict__ entries, const int32_t* __restrict__ order, int Hm, int ntk, int N, float scale_log2, int q_split, int kvl_lo,
-    int kvl_hi, int n_single, void* __restrict__ out_raw, float* __restrict__ lse, int32_t* __restrict__ status,
+    int kvl_hi, int n_single, void* __restrict__ out_raw, void* __restrict__ lo_raw, float* __restrict__ lse, int32_t* __restrict__ status,
     const __grid_constant__ OutScatter scatter) {
   constexpr int kTileBytes = kTile * D * 2;       // one Q, K or V tile
   constexpr int kChunks = D / 64;                 // 64-element (128-byte) column chunks per tile
@@ -439,6 +460,7 @@ __global__ void __launch_bounds__(kThreads, 1) sparse_attn_fwd_kernel(
       ptx::tc_fence_after();
       const float inv = (done > 0 && l > 0.f) ? 1.f / l : 0.f;
       uint4* dst;
+      uint4* lo = reinterpret_cast<uint4*>(static_cast<unsigned char*>(lo_raw) + (static_cast<int64_t>(bh) * N + grow) * D * 2);
       if (scatter.n_peers > 0) {
         const int r = min(grow / scatter.rows_per_peer, scatter.n_peers - 1);
         dst = reinterpret_cast<uint4*>(
@@ -461,12 +483,10 @@ __global__ void __launch_bounds__(kThreads, 1) sparse_attn_fwd_kernel(
         if (grow < N) {
 #pragma unroll
           for (int q4 = 0; q4 < 4; ++q4) {
-            uint4 w;
-            w.x = pack2<kBF16>(o[q4 * 8 + 0] * inv, o[q4 * 8 + 1] * inv);
-            w.y = pack2<kBF16>(o[q4 * 8 + 2] * inv, o[q4 * 8 + 3] * inv);
-            w.z = pack2<kBF16>(o[q4 * 8 + 4] * inv, o[q4 * 8 + 5] * inv);
-            w.w = pack2<kBF16>(o[q4 * 8 + 6] * inv, o[q4 * 8 + 7] * inv);
-            dst[c * 4 + q4] = w;
+            float f[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = o[q4 * 8 + i] * inv;
+            store8<kBF16, kResidual>(f, dst + c * 4 + q4, lo + c * 4 + q4);
           }
         }
       }
@@ -564,12 +584,12 @@ __device__ __forceinline__ void exp_pairs(const float* v, float scale_log2, floa
   }
 }
 
-template <bool kBF16>
+template <bool kBF16, bool kResidual>
 __global__ void __launch_bounds__(kThreads64, 1) sparse_attn_fwd_d64_kernel(
     const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
     const __grid_constant__ CUtensorMap tm_v, const int32_t* __restrict__ counts,
     const int32_t* __restrict__ entries, const int32_t* __restrict__ order, int Hm, int ntk, int N, float scale_log2,
-    int q_split, int kvl_lo, int kvl_hi, int n_single, void* __restrict__ out_raw, float* __restrict__ lse,
+    int q_split, int kvl_lo, int kvl_hi, int n_single, void* __restrict__ out_raw, void* __restrict__ lo_raw, float* __restrict__ lse,
     int32_t* __restrict__ status, const __grid_constant__ OutScatter scatter) {
   constexpr int D = 64;
   constexpr int kTileBytes = kTile * D * 2;       // one Q, K or V tile: 128 rows x 128 bytes
@@ -856,6 +876,7 @@ __global__ void __launch_bounds__(kThreads64, 1) sparse_attn_fwd_d64_kernel(
       const float inv = lt > 0.f ? 1.f / lt : 0.f;
       const float f0 = w0 * inv, f1 = w1 * inv;
       uint4* dst;
+      uint4* lo = reinterpret_cast<uint4*>(static_cast<unsigned char*>(lo_raw) + (static_cast<int64_t>(bh) * N + grow) * D * 2);
       if (scatter.n_peers > 0) {
         const int pr = min(grow / scatter.rows_per_peer, scatter.n_peers - 1);
         dst = reinterpret_cast<uint4*>(
@@ -879,12 +900,10 @@ __global__ void __launch_bounds__(kThreads64, 1) sparse_attn_fwd_d64_kernel(
         if (grow < N) {
 #pragma unroll
           for (int q4 = 0; q4 < 2; ++q4) {
-            uint4 w;
-            w.x = pack2<kBF16>(o[q4 * 8 + 0], o[q4 * 8 + 1]);
-            w.y = pack2<kBF16>(o[q4 * 8 + 2], o[q4 * 8 + 3]);
-            w.z = pack2<kBF16>(o[q4 * 8 + 4], o[q4 * 8 + 5]);
-            w.w = pack2<kBF16>(o[q4 * 8 + 6], o[q4 * 8 + 7]);
-            dst[c * 2 + q4] = w;
+            float f[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = o[q4 * 8 + i];
+            store8<kBF16, kResidual>(f, dst + c * 2 + q4, lo + c * 2 + q4);
           }
         }
       }
@@ -905,14 +924,14 @@ __global__ void __launch_bounds__(kThreads64, 1) sparse_attn_fwd_d64_kernel(
 template <bool kBF16>
 int launch_d64(const void* q, const void* k, const void* v, int dtype, int BH, int N, const int32_t* counts,
                const int32_t* entries, const int32_t* order, int Hm, float softmax_scale, int q_split, int kvl_lo,
-               int kvl_hi, int pairs_beside, void* out, float* lse, int32_t* status, const OutScatter& scatter, cudaStream_t st) {
+               int kvl_hi, int pairs_beside, void* out, void* lo, float* lse, int32_t* status, const OutScatter& scatter, cudaStream_t st) {
   CUtensorMap tq, tk, tv;
   if (int rc = make_tmap_rows(&tq, q, dtype, BH, N, 64, kTile)) return rc;
   if (int rc = make_tmap_rows(&tk, k, dtype, BH, N, 64, kTile)) return rc;
   if (int rc = make_tmap_rows(&tv, v, dtype, BH, N, 64, kTile)) return rc;
   const int ntq = ceil_div(N, kTile);
   const int npairs = (ntq + 1) / 2;
-  auto kernel = sparse_attn_fwd_d64_kernel<kBF16>;
+  auto kernel = lo ? sparse_attn_fwd_d64_kernel<kBF16, true> : sparse_attn_fwd_d64_kernel<kBF16, false>;
   const size_t smem = smem_bytes_d64();
   if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem)) return rc;
   const float scale_log2 = softmax_scale * 1.4426950408889634f;
@@ -920,7 +939,7 @@ int launch_d64(const void* q, const void* k, const void* v, int dtype, int BH, i
   if (int rc = sm_count(&sms)) return rc;
   const int n_single = single_pairs(sms, npairs * Hm, BH / Hm, pairs_beside);
   kernel<<<dim3(npairs * Hm + n_single, BH / Hm), kThreads64, smem, st>>>(tq, tk, tv, counts, entries, order, Hm, ntq, N,
-                                                                         scale_log2, q_split, kvl_lo, kvl_hi, n_single, out,
+                                                                         scale_log2, q_split, kvl_lo, kvl_hi, n_single, out, lo,
                                                                          lse, status, scatter);
   MODDIT_CHECK_LAUNCH("sparse_attn_fwd_d64_kernel");
   return MODDIT_OK;
@@ -929,14 +948,14 @@ int launch_d64(const void* q, const void* k, const void* v, int dtype, int BH, i
 template <int D, bool kBF16>
 int launch(const void* q, const void* k, const void* v, int dtype, int BH, int N, const int32_t* counts,
            const int32_t* entries, const int32_t* order, int Hm, float softmax_scale, int q_split, int kvl_lo, int kvl_hi,
-           int pairs_beside, void* out, float* lse, int32_t* status, const OutScatter& scatter, cudaStream_t st) {
+           int pairs_beside, void* out, void* lo, float* lse, int32_t* status, const OutScatter& scatter, cudaStream_t st) {
   CUtensorMap tq, tk, tv;
   if (int rc = make_tmap_rows(&tq, q, dtype, BH, N, D, kTile)) return rc;
   if (int rc = make_tmap_rows(&tk, k, dtype, BH, N, D, kTile)) return rc;
   if (int rc = make_tmap_rows(&tv, v, dtype, BH, N, D, kTile)) return rc;
   const int ntq = ceil_div(N, kTile);
   const int npairs = (ntq + 1) / 2;
-  auto kernel = sparse_attn_fwd_kernel<D, kBF16>;
+  auto kernel = lo ? sparse_attn_fwd_kernel<D, kBF16, true> : sparse_attn_fwd_kernel<D, kBF16, false>;
   const size_t smem = smem_bytes<D>();
   if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem)) return rc;
   const float scale_log2 = softmax_scale * 1.4426950408889634f;
@@ -944,7 +963,7 @@ int launch(const void* q, const void* k, const void* v, int dtype, int BH, int N
   if (int rc = sm_count(&sms)) return rc;
   const int n_single = single_pairs(sms, npairs * Hm, BH / Hm, pairs_beside);
   kernel<<<dim3(npairs * Hm + n_single, BH / Hm), kThreads, smem, st>>>(tq, tk, tv, counts, entries, order, Hm, ntq, N,
-                                                                       scale_log2, q_split, kvl_lo, kvl_hi, n_single, out,
+                                                                       scale_log2, q_split, kvl_lo, kvl_hi, n_single, out, lo,
                                                                        lse, status, scatter);
   MODDIT_CHECK_LAUNCH("sparse_attn_fwd_kernel");
   return MODDIT_OK;
@@ -962,7 +981,7 @@ extern "C" int moddit_sparse_attn_single_pairs(int sms, int pairs, int batches, 
 static int sparse_attn_dispatch(const void* q, const void* k, const void* v, int dtype, int BH, int N, int D,
                                 const int32_t* counts, const int32_t* entries, const int32_t* order, int Hm,
                                 float softmax_scale, int q_split, int kv_len_lo, int kv_len_hi, int pairs_beside, void* out,
-                                float* lse, int32_t* status, const OutScatter& scatter, void* stream) {
+                                void* lo, float* lse, int32_t* status, const OutScatter& scatter, void* stream) {
   MODDIT_CHECK_ARG(q && k && v && counts && entries && status, "sparse_attn_fwd: null pointer");
   MODDIT_CHECK_ARG(out || scatter.n_peers > 0, "sparse_attn_fwd: no output destination");
   MODDIT_CHECK_ARG(BH > 0 && BH <= 65535 && N > 0 && Hm > 0, "sparse_attn_fwd: BH=%d N=%d Hm=%d out of range", BH, N, Hm);
@@ -973,22 +992,22 @@ static int sparse_attn_dispatch(const void* q, const void* k, const void* v, int
   MODDIT_CHECK_ARG(pairs_beside >= 0, "sparse_attn_fwd: pairs_beside=%d must not be negative", pairs_beside);
   if (D != 64 && D != 128) return fail(MODDIT_E_UNSUPPORTED, "sparse_attn_fwd: head_dim must be 64 or 128, got %d", D);
   if (dtype != MODDIT_BF16 && dtype != MODDIT_FP16) return fail(MODDIT_E_ARG, "sparse_attn_fwd: unknown dtype %d", dtype);
-  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out))
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(lo))
     return fail(MODDIT_E_ALIGN, "sparse_attn_fwd: q, k, v and out must be 16-byte aligned");
   if (int rc = require_sm100()) return rc;
   cudaStream_t st = as_stream(stream);
   if (D == 128) {
     return dtype == MODDIT_BF16
                ? launch<128, true>(q, k, v, dtype, BH, N, counts, entries, order, Hm, softmax_scale, q_split, kv_len_lo,
-                                   kv_len_hi, pairs_beside, out, lse, status, scatter, st)
+                                   kv_len_hi, pairs_beside, out, lo, lse, status, scatter, st)
                : launch<128, false>(q, k, v, dtype, BH, N, counts, entries, order, Hm, softmax_scale, q_split, kv_len_lo,
-                                    kv_len_hi, pairs_beside, out, lse, status, scatter, st);
+                                    kv_len_hi, pairs_beside, out, lo, lse, status, scatter, st);
   }
   return dtype == MODDIT_BF16
              ? launch_d64<true>(q, k, v, dtype, BH, N, counts, entries, order, Hm, softmax_scale, q_split, kv_len_lo, kv_len_hi,
-                                pairs_beside, out, lse, status, scatter, st)
+                                pairs_beside, out, lo, lse, status, scatter, st)
              : launch_d64<false>(q, k, v, dtype, BH, N, counts, entries, order, Hm, softmax_scale, q_split, kv_len_lo, kv_len_hi,
-                                 pairs_beside, out, lse, status, scatter, st);
+                                 pairs_beside, out, lo, lse, status, scatter, st);
 }
 
 static int scatter_to(OutScatter* sc, void* const* peer_out, int n_peers, int N, int head_base) {
@@ -1014,7 +1033,17 @@ extern "C" int moddit_sparse_attn_fwd(const void* q, const void* k, const void* 
   clear_error();
   MODDIT_CHECK_ARG(out, "sparse_attn_fwd: null output pointer");
   return sparse_attn_dispatch(q, k, v, dtype, BH, N, D, counts, entries, order, Hm, softmax_scale, q_split, kv_len_lo,
-                              kv_len_hi, 0, out, lse, status, OutScatter{}, stream);
+                              kv_len_hi, 0, out, nullptr, lse, status, OutScatter{}, stream);
+}
+
+extern "C" int moddit_sparse_attn_fwd_residual(const void* q, const void* k, const void* v, int dtype, int BH, int N, int D,
+                                               const int32_t* counts, const int32_t* entries, const int32_t* order, int Hm,
+                                               float softmax_scale, int q_split, int kv_len_lo, int kv_len_hi, void* out,
+                                               void* out_lo, float* lse, int32_t* status, void* stream) {
+  clear_error();
+  MODDIT_CHECK_ARG(out && out_lo && lse, "sparse_attn_fwd_residual: null output pointer");
+  return sparse_attn_dispatch(q, k, v, dtype, BH, N, D, counts, entries, order, Hm, softmax_scale, q_split, kv_len_lo,
+                              kv_len_hi, 0, out, out_lo, lse, status, OutScatter{}, stream);
 }
 
 extern "C" int moddit_sparse_attn_fwd_scatter(const void* q, const void* k, const void* v, int dtype, int BH, int N,
@@ -1026,7 +1055,7 @@ extern "C" int moddit_sparse_attn_fwd_scatter(const void* q, const void* k, cons
   OutScatter sc = {};
   if (int rc = scatter_to(&sc, peer_out, n_peers, N, head_base)) return rc;
   return sparse_attn_dispatch(q, k, v, dtype, BH, N, D, counts, entries, order, Hm, softmax_scale, q_split, kv_len_lo,
-                              kv_len_hi, 0, nullptr, lse, status, sc, stream);
+                              kv_len_hi, 0, nullptr, nullptr, lse, status, sc, stream);
 }
 
 extern "C" int moddit_sparse_attn_fwd_beside(const void* q, const void* k, const void* v, int dtype, int BH, int N, int D,
@@ -1040,5 +1069,5 @@ extern "C" int moddit_sparse_attn_fwd_beside(const void* q, const void* k, const
   if (peer_out != nullptr)
     if (int rc = scatter_to(&sc, peer_out, n_peers, N, head_base)) return rc;
   return sparse_attn_dispatch(q, k, v, dtype, BH, N, D, counts, entries, order, Hm, softmax_scale, q_split, kv_len_lo,
-                              kv_len_hi, pairs_beside, out, lse, status, sc, stream);
+                              kv_len_hi, pairs_beside, out, nullptr, lse, status, sc, stream);
 }

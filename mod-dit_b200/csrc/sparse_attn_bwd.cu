@@ -801,8 +801,8 @@ __global__ void __launch_bounds__(kThreads, 1) sparse_attn_bwd_kernel(
 // Row statistics: one group of D / 8 threads per row.  Rows past N and rows that attend to nothing get -inf, so that their
 // probabilities are zero whatever the scores are.
 template <int D, bool kBF16>
-__global__ void __launch_bounds__(256) bwd_stats_kernel(const void* __restrict__ out, const void* __restrict__ dout,
-                                                        const float* __restrict__ lse, int N, int npad,
+__global__ void __launch_bounds__(256) bwd_stats_kernel(const void* __restrict__ out, const void* __restrict__ lo,
+                                                        const void* __restrict__ dout, const float* __restrict__ lse, int N, int npad,
                                                         float* __restrict__ nlse, float* __restrict__ ndelta) {
   constexpr int kTpr = D / 8;
   const int bh = blockIdx.y;
@@ -812,19 +812,17 @@ __global__ void __launch_bounds__(256) bwd_stats_kernel(const void* __restrict__
   if (row < N) {
     const int64_t at = (static_cast<int64_t>(bh) * N + row) * kTpr + c;
     const uint4 a = __ldg(static_cast<const uint4*>(out) + at), b = __ldg(static_cast<const uint4*>(dout) + at);
-    const uint32_t wa[4] = {a.x, a.y, a.z, a.w}, wb[4] = {b.x, b.y, b.z, b.w};
+    const uint4 r = lo ? __ldg(static_cast<const uint4*>(lo) + at) : make_uint4(0, 0, 0, 0);
+    const uint32_t wa[4] = {a.x, a.y, a.z, a.w}, wb[4] = {b.x, b.y, b.z, b.w}, wr[4] = {r.x, r.y, r.z, r.w};
+    auto floats = [](const uint32_t& w) {
+      if constexpr (kBF16) return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
+      else return __half22float2(*reinterpret_cast<const __half2*>(&w));
+    };
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      float2 x, y;
-      if constexpr (kBF16) {
-        x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&wa[i]));
-        y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&wb[i]));
-      } else {
-        x = __half22float2(*reinterpret_cast<const __half2*>(&wa[i]));
-        y = __half22float2(*reinterpret_cast<const __half2*>(&wb[i]));
-      }
-      sum = fmaf(x.x, y.x, sum);
-      sum = fmaf(x.y, y.y, sum);
+      const float2 x = floats(wa[i]), y = floats(wb[i]), z = floats(wr[i]);
+      sum = fmaf(x.x + z.x, y.x, sum);
+      sum = fmaf(x.y + z.y, y.y, sum);
     }
   }
 #pragma unroll
@@ -839,7 +837,7 @@ __global__ void __launch_bounds__(256) bwd_stats_kernel(const void* __restrict__
 }
 
 template <int D, bool kBF16>
-int launch(BwdArgs a, const void* out, const float* lse, int dtype, int BH, float* ws, cudaStream_t st) {
+int launch(BwdArgs a, const void* out, const void* lo, const float* lse, int dtype, int BH, float* ws, cudaStream_t st) {
   const int kv_rows = max(1, max(a.kvl_lo, a.kvl_hi));
   CUtensorMap tq, tk, tv, tdo;
   if (int rc = make_tmap_rows(&tq, a.q, dtype, BH, a.N, D, kBlock)) return rc;
@@ -851,7 +849,8 @@ int launch(BwdArgs a, const void* out, const float* lse, int dtype, int BH, floa
   if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem)) return rc;
   a.nlse = ws;
   a.ndelta = ws + static_cast<int64_t>(BH) * a.npad;
-  bwd_stats_kernel<D, kBF16><<<dim3(a.npad / (2048 / D), BH), 256, 0, st>>>(out, a.dout, lse, a.N, a.npad, ws, ws + static_cast<int64_t>(BH) * a.npad);
+  bwd_stats_kernel<D, kBF16><<<dim3(a.npad / (2048 / D), BH), 256, 0, st>>>(out, lo, a.dout, lse, a.N, a.npad, ws,
+                                                                                  ws + static_cast<int64_t>(BH) * a.npad);
   MODDIT_CHECK_LAUNCH("bwd_stats_kernel");
   const int64_t blocks = static_cast<int64_t>(2 * a.ntiles + (a.ntiles & 1)) * BH;
   kernel<<<static_cast<unsigned>(blocks), kThreads, smem, st>>>(tq, tk, tv, tdo, a);
@@ -869,8 +868,8 @@ extern "C" size_t moddit_sparse_attn_bwd_workspace_bytes(int BH, int N) {
   return static_cast<size_t>(2) * BH * ceil_div(N, kTile) * kTile * sizeof(float);
 }
 
-extern "C" int moddit_sparse_attn_bwd(const void* q, const void* k, const void* v, const void* out, const void* dout,
-                                      const float* lse, int dtype, int BH, int N, int D, const int32_t* q_counts,
+extern "C" int moddit_sparse_attn_bwd(const void* q, const void* k, const void* v, const void* out, const void* out_lo,
+                                      const void* dout, const float* lse, int dtype, int BH, int N, int D, const int32_t* q_counts,
                                       const int32_t* q_entries, const int32_t* q_order, const int32_t* k_counts,
                                       const int32_t* k_entries, const int32_t* k_order, int Hm, float softmax_scale,
                                       int q_split, int kv_len_lo, int kv_len_hi, void* dq, void* dk, void* dv, void* workspace,
@@ -885,16 +884,16 @@ extern "C" int moddit_sparse_attn_bwd(const void* q, const void* k, const void* 
                    "sparse_attn_bwd: kv_len (%d, %d) outside [0, N=%d]", kv_len_lo, kv_len_hi, N);
   if (D != 64 && D != 128) return fail(MODDIT_E_UNSUPPORTED, "sparse_attn_bwd: head_dim must be 64 or 128, got %d", D);
   if (dtype != MODDIT_BF16 && dtype != MODDIT_FP16) return fail(MODDIT_E_ARG, "sparse_attn_bwd: unknown dtype %d", dtype);
-  const void* tensors[8] = {q, k, v, out, dout, dq, dk, dv};
+  if (N > kMaxBlocks * kBlock) return fail(MODDIT_E_UNSUPPORTED, "sparse_attn_bwd: N=%d exceeds %d", N, kMaxBlocks * kBlock);
+  if (static_cast<int64_t>(2 * ceil_div(N, kTile) + 1) * BH > (1ll << 31) - 1)
+    return fail(MODDIT_E_UNSUPPORTED, "sparse_attn_bwd: %d heads of %d rows are too many work items", BH, N);
+  const void* tensors[9] = {q, k, v, out, out_lo, dout, dq, dk, dv};
   for (const void* p : tensors)
     if (!aligned16(p)) return fail(MODDIT_E_ALIGN, "sparse_attn_bwd: all (BH, N, D) tensors must be 16-byte aligned");
   if (workspace == nullptr || workspace_bytes < moddit_sparse_attn_bwd_workspace_bytes(BH, N) || !aligned16(workspace))
     return fail(MODDIT_E_WORKSPACE, "sparse_attn_bwd: a 16-byte aligned workspace of %zu bytes is needed",
                 moddit_sparse_attn_bwd_workspace_bytes(BH, N));
   if (int rc = require_sm100()) return rc;
-  if (N > kMaxBlocks * kBlock) return fail(MODDIT_E_UNSUPPORTED, "sparse_attn_bwd: N=%d exceeds %d", N, kMaxBlocks * kBlock);
-  if (static_cast<int64_t>(2 * ceil_div(N, kTile) + 1) * BH > (1ll << 31) - 1)
-    return fail(MODDIT_E_UNSUPPORTED, "sparse_attn_bwd: %d heads of %d rows are too many work items", BH, N);
   BwdArgs a{};
   a.key_lists = Lists{k_counts, k_entries, k_order};
   a.query_lists = Lists{q_counts, q_entries, q_order};
@@ -907,6 +906,6 @@ extern "C" int moddit_sparse_attn_bwd(const void* q, const void* k, const void* 
   float* ws = static_cast<float*>(workspace);
   cudaStream_t st = as_stream(stream);
   if (D == 128)
-    return dtype == MODDIT_BF16 ? launch<128, true>(a, out, lse, dtype, BH, ws, st) : launch<128, false>(a, out, lse, dtype, BH, ws, st);
-  return dtype == MODDIT_BF16 ? launch<64, true>(a, out, lse, dtype, BH, ws, st) : launch<64, false>(a, out, lse, dtype, BH, ws, st);
+    return dtype == MODDIT_BF16 ? launch<128, true>(a, out, out_lo, lse, dtype, BH, ws, st) : launch<128, false>(a, out, out_lo, lse, dtype, BH, ws, st);
+  return dtype == MODDIT_BF16 ? launch<64, true>(a, out, out_lo, lse, dtype, BH, ws, st) : launch<64, false>(a, out, out_lo, lse, dtype, BH, ws, st);
 }

@@ -6,22 +6,25 @@ its selection is not differentiated.
 """
 from __future__ import annotations
 
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import ops
 
-__all__ = ["sparse_attention"]
+__all__ = ["sparse_attention", "qkv_prologue"]
 
 
 class _SparseAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lists, key_lists, limits, check_status):
-        out, lse = ops.sparse_attn_fwd(q, k, v, lists.counts, lists.entries, order=lists.order, return_lse=True,
-                                       check_status=check_status, **limits)
-        ctx.save_for_backward(q, k, v, out, lse, lists.counts, lists.entries, lists.order, key_lists.counts,
+        if not any(ctx.needs_input_grad[:3]):
+            return ops.sparse_attn_fwd(q, k, v, lists.counts, lists.entries, order=lists.order, check_status=check_status,
+                                       **limits)
+        out, lse, residual = ops.sparse_attn_fwd(q, k, v, lists.counts, lists.entries, order=lists.order,
+                                                 return_residual=True, check_status=check_status, **limits)
+        ctx.save_for_backward(q, k, v, out, lse, residual, lists.counts, lists.entries, lists.order, key_lists.counts,
                               key_lists.entries, key_lists.order)
         ctx.limits, ctx.check_status = limits, check_status
         return out
@@ -29,9 +32,10 @@ class _SparseAttention(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, lse, *lists = ctx.saved_tensors
+        q, k, v, out, lse, residual, *lists = ctx.saved_tensors
         grads = ops.sparse_attn_bwd(dout.contiguous(), q, k, v, out, lse, ops.TileLists(*lists[:3]),
-                                    ops.KeyLists(*lists[3:]), check_status=ctx.check_status, **ctx.limits)
+                                    ops.KeyLists(*lists[3:]), residual=residual, check_status=ctx.check_status,
+                                    **ctx.limits)
         return tuple(g if need else None for g, need in zip(grads, ctx.needs_input_grad)) + (None,) * 4
 
 
@@ -43,6 +47,71 @@ def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lists: o
 
     lists, key_lists: `ops.tile_lists` and `ops.key_lists` of the layer's mask; the other arguments are those of
     `ops.sparse_attn_fwd`.  Tensors that are not contiguous are copied.  What lies between the forward and the backward is
-    q, k, v, the output and 4 bytes per row."""
+    q, k, v, the output, what rounding took from it and 4 bytes per row."""
     limits = dict(softmax_scale=softmax_scale, q_split=q_split, kv_len_lo=kv_len_lo, kv_len_hi=kv_len_hi)
     return _SparseAttention.apply(q.contiguous(), k.contiguous(), v.contiguous(), lists, key_lists, limits, check_status)
+
+
+class _Prologue(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, fused, q_in, k_in, v_in, q_weight, q_bias, k_weight, k_bias, rope_cos, rope_sin, opts):
+        if fused is not None:
+            q_in, k_in, v_in = fused.split(fused.shape[-1] // 3, dim=-1)
+        (q, k, v), _ = ops.qkv_prologue(q_in, k_in, v_in, q_weight=q_weight, q_bias=q_bias, k_weight=k_weight, k_bias=k_bias,
+                                        rope_cos=rope_cos, rope_sin=rope_sin, **opts)
+        keep = opts["norm"] is not None
+        ctx.save_for_backward(fused if keep else None, q_in if keep and fused is None else None,
+                              k_in if keep and fused is None else None, q_weight, q_bias, k_weight, k_bias, rope_cos, rope_sin)
+        ctx.opts, ctx.fused, ctx.tokens = opts, fused is not None, q_in.shape[1]
+        ctx.set_materialize_grads(False)
+        return q, k, v
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *grads):
+        fused, q_in, k_in, q_weight, q_bias, k_weight, k_bias, rope_cos, rope_sin = ctx.saved_tensors
+        if fused is not None:
+            q_in, k_in, _ = fused.split(fused.shape[-1] // 3, dim=-1)
+        grads = [None if g is None else g.contiguous() for g in grads]
+        given = [g for g in grads if g is not None]
+        if not given:
+            return (None,) * 11
+        needs = ctx.needs_input_grad
+        if not ctx.fused:           # an input without a gradient costs nothing, unless its norm's parameters need theirs
+            wanted = (needs[1] or needs[4] or needs[5], needs[2] or needs[6] or needs[7], needs[3])
+            grads = [g if w else None for g, w in zip(grads, wanted)]
+            if all(g is None for g in grads):
+                return (None,) * 11
+        whole, out = None, None
+        if ctx.fused:
+            B, H, _, D = given[0].shape
+            whole = torch.empty(B, ctx.tokens, 3 * H * D, device=given[0].device, dtype=given[0].dtype)
+            out = whole.split(H * D, dim=-1)
+            for o, g in zip(out, grads):
+                if g is None:
+                    o.zero_()
+        dx, params = ops.qkv_prologue_bwd(*grads, q_in, k_in, q_weight=q_weight, q_bias=q_bias,
+                                          k_weight=k_weight, k_bias=k_bias, rope_cos=rope_cos, rope_sin=rope_sin,
+                                          n_tokens=ctx.tokens, out=out, **ctx.opts)
+        dx = (None, None, None) if ctx.fused else dx
+        return (whole, *dx, params["q_weight"], params["q_bias"], params["k_weight"], params["k_bias"], None, None, None)
+
+
+def qkv_prologue(q_in: Optional[torch.Tensor] = None, k_in: Optional[torch.Tensor] = None,
+                 v_in: Optional[torch.Tensor] = None, *, fused: Optional[torch.Tensor] = None, num_heads: int,
+                 norm: Optional[str] = None, q_weight: Optional[torch.Tensor] = None, q_bias: Optional[torch.Tensor] = None,
+                 k_weight: Optional[torch.Tensor] = None, k_bias: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                 rope_cos: Optional[torch.Tensor] = None, rope_sin: Optional[torch.Tensor] = None,
+                 rope_form: str = "elementwise", rope_range: Optional[Tuple[int, int]] = None):
+    """(q, k, v) of shape (B, H, S, D) as `ops.qkv_prologue` makes them, differentiable with respect to the projections and the
+    norm's parameters (the rotary tables are constants).
+
+    Either q_in, k_in and v_in, (B, S, H*D) each, or `fused`, a contiguous (B, S, 3*H*D) projection whose gradient is written
+    in one piece.  The other arguments are those of `ops.qkv_prologue`."""
+    if (fused is None) == (q_in is None) or (fused is None and (k_in is None or v_in is None)) or \
+            (fused is not None and (k_in is not None or v_in is not None)):
+        raise ValueError("qkv_prologue: either q_in, k_in and v_in or fused")
+    if fused is not None and (fused.dim() != 3 or not fused.is_contiguous() or fused.shape[-1] % (3 * num_heads)):
+        raise ValueError(f"fused must be a contiguous (B, S, 3 * {num_heads} * D) tensor")
+    opts = dict(num_heads=num_heads, norm=None if norm == "none" else norm, eps=eps, rope_form=rope_form, rope_range=rope_range)
+    return _Prologue.apply(fused, q_in, k_in, v_in, q_weight, q_bias, k_weight, k_bias, rope_cos, rope_sin, opts)

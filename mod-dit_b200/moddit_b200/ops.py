@@ -336,7 +336,7 @@ def qkv_prologue_bwd(dq: Optional[torch.Tensor], dk: Optional[torch.Tensor], dv:
     stride = _token_stride(present, (B, S, H * D), ref.dtype, dev, "inputs")
     width = H * D if norm == "rms_all_heads" else D
     for name, p in (("q_weight", q_weight), ("q_bias", q_bias), ("k_weight", k_weight), ("k_bias", k_bias)):
-        if p is not None and (p.dtype != ref.dtype or not p.is_contiguous() or p.device != dev or p.numel() != width):
+        if kind and p is not None and (p.dtype != ref.dtype or not p.is_contiguous() or p.device != dev or p.numel() != width):
             raise ValueError(f"{name} must be a contiguous {ref.dtype} tensor of {width} values on {dev}")
     if (rope_cos is None) != (rope_sin is None):
         raise ValueError("rope_cos and rope_sin go together")
@@ -352,9 +352,10 @@ def qkv_prologue_bwd(dq: Optional[torch.Tensor], dk: Optional[torch.Tensor], dv:
     if any(o is None for o in stores):
         raise ValueError("every gradient given needs an output buffer")
     out_stride = _token_stride(stores, (B, S, H * D), ref.dtype, dev, "output buffers")
-    params = {"q_weight": q_weight if dq is not None else None, "k_weight": k_weight if dk is not None else None,
-              "q_bias": q_bias if dq is not None else None, "k_bias": k_bias if dk is not None else None}
-    res = {name: None if p is None or not kind else torch.empty_like(p) for name, p in params.items()}
+    res = {"q_weight": None, "q_bias": None, "k_weight": None, "k_bias": None}
+    for name, p, g in (("q_weight", q_weight, dq), ("k_weight", k_weight, dk), ("q_bias", q_bias, dq), ("k_bias", k_bias, dk)):
+        if p is not None and g is not None and kind and (norm == "layer" or name.endswith("weight")):
+            res[name] = torch.empty_like(p)
     ws = None
     wsb = 0
     if any(r is not None for r in res.values()):
@@ -922,7 +923,10 @@ def raise_on_status(device) -> None:
 
 def post_status(device) -> None:
     """Queues a copy of the status words into pinned host memory behind the work already on the current stream
-    and records an event after it.  Costs no synchronisation; `check_posted_status` looks at the copy later."""
+    and records an event after it.  Costs no synchronisation; `check_posted_status` looks at the copy later.
+    While the stream is being captured it does nothing: an event of a captured graph cannot be asked."""
+    if torch.cuda.is_current_stream_capturing():
+        return
     device = torch.device(device)
     idx = device.index if device.index is not None else torch.cuda.current_device()
     slot = _POSTED.get(idx)
@@ -977,11 +981,13 @@ def sparse_attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, counts: t
                     softmax_scale: Optional[float] = None,
                     q_split: Optional[int] = None, kv_len_lo: Optional[int] = None,
                     kv_len_hi: Optional[int] = None, return_lse: bool = False, check_status=True,
-                    out: Optional[torch.Tensor] = None, scatter=None, pairs_beside: int = 0):
+                    out: Optional[torch.Tensor] = None, scatter=None, pairs_beside: int = 0,
+                    return_residual: bool = False):
     """Block-sparse attention forward of (B,H,N,D) tensors over the work lists from `tile_lists`.
 
     pairs_beside: work items (mask heads x query-tile pairs x batches) of other launches that run at the same time on
     other streams; same output, only the launch's shape takes them into account.
+    return_residual: (out, lse, residual) for a backward pass; the residual is what rounding took from the output.
     check_status: True reads the kernel's status words after the launch (synchronises); "deferred" queues an
     asynchronous copy of them (`post_status`) for a later `check_posted_status`; False does neither."""
     dev = _need_cuda(q, k, v, counts, entries)
@@ -998,7 +1004,9 @@ def sparse_attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, counts: t
                               or not order.is_contiguous() or order.device != dev):
         raise ValueError("order must be the contiguous int32 (Hm, npairs) tensor from tile_lists")
     scale = float(D ** -0.5 if softmax_scale is None else softmax_scale)
-    lse = torch.empty(B, H, N, device=dev, dtype=torch.float32) if return_lse else None
+    if return_residual and (scatter is not None or pairs_beside):
+        raise ValueError("return_residual: one launch with a local output only")
+    lse = torch.empty(B, H, N, device=dev, dtype=torch.float32) if return_lse or return_residual else None
     st = _status_words(dev)
     table, n_peers, head_base = None, 0, 0
     if scatter is not None:
@@ -1018,9 +1026,15 @@ def sparse_attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, counts: t
         elif scatter is not None:
             check(lib.moddit_sparse_attn_fwd_scatter(*args, table, n_peers, int(head_base), _ptr(lse), _ptr(st),
                                                      _stream(dev)), "moddit_sparse_attn_fwd_scatter")
+        elif return_residual:
+            residual = torch.empty_like(out)
+            check(lib.moddit_sparse_attn_fwd_residual(*args, _ptr(out), _ptr(residual), _ptr(lse), _ptr(st), _stream(dev)),
+                  "moddit_sparse_attn_fwd_residual")
         else:
             check(lib.moddit_sparse_attn_fwd(*args, _ptr(out), _ptr(lse), _ptr(st), _stream(dev)), "moddit_sparse_attn_fwd")
     _after_launch(dev, check_status)
+    if return_residual:
+        return out, lse, residual
     return (out, lse) if return_lse else out
 
 
@@ -1038,24 +1052,29 @@ def _need_lists(lists, rows: int, tiles: int, dev: torch.device, what: str) -> N
 def sparse_attn_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
                     lse: torch.Tensor, lists: TileLists, key_lists: KeyLists, *, softmax_scale: Optional[float] = None,
                     q_split: Optional[int] = None, kv_len_lo: Optional[int] = None, kv_len_hi: Optional[int] = None,
+                    residual: Optional[torch.Tensor] = None,
                     check_status=True) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Gradients (dq, dk, dv) of `sparse_attn_fwd` from the gradient `dout` of its output.
 
     q, k, v, the limits and the scale are the forward's, `out` and `lse` what it returned (`return_lse=True`), `lists`
-    and `key_lists` the results of `tile_lists` and `key_lists` for its mask.  The probabilities are computed again tile
+    and `key_lists` the results of `tile_lists` and `key_lists` for its mask.  `residual` (of `return_residual=True`) makes
+    the gradients of q and k of rows with nearly all of their weight on one key exact to 16 bits.  The probabilities are computed again tile
     by tile; the results are the same bits on every run.  check_status: as in `sparse_attn_fwd`."""
-    dev = _need_cuda(dout, q, k, v, out, lse)
+    rest = () if residual is None else (residual,)
+    dev = _need_cuda(dout, q, k, v, out, lse, *rest)
     if q.dim() != 4:
         raise ValueError("query, key, value, output and its gradient must be (B, H, N, D) tensors")
     dt = _qkv_dtype(q)
     shape, dtype = q.shape, q.dtype
-    for t in (k, v, out, dout):
+    for t in (k, v, out, dout, *rest):
         if t.shape != shape or t.dtype != dtype:
             raise ValueError("query, key, value, output and its gradient must have identical shapes and dtypes")
     B, H, N, D = shape
     if lse.shape != shape[:3] or lse.dtype != torch.float32:
         raise ValueError("lse must be the float32 (B, H, N) tensor that the forward returned")
     _need_contig(dout=dout, q=q, k=k, v=v, out=out, lse=lse)
+    if residual is not None:
+        _need_contig(residual=residual)
     nt = (N + 127) // 128
     _need_lists(lists, (nt + 1) // 2, nt, dev, "tile_lists")
     _need_lists(key_lists, nt, nt, dev, "key_lists")
@@ -1067,7 +1086,7 @@ def sparse_attn_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
     ws = torch.empty(wsb, device=dev, dtype=torch.uint8)
     with _entry("moddit_sparse_attn_bwd", dev):
         check(lib.moddit_sparse_attn_bwd(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(), lse.data_ptr(), dt, B * H, N, D,
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _addr(residual), dout.data_ptr(), lse.data_ptr(), dt, B * H, N, D,
             lists.counts.data_ptr(), lists.entries.data_ptr(), lists.order.data_ptr(), key_lists.counts.data_ptr(),
             key_lists.entries.data_ptr(), key_lists.order.data_ptr(), Hm,
             D ** -0.5 if softmax_scale is None else softmax_scale, N if q_split is None else q_split,
