@@ -324,7 +324,7 @@ __device__ __forceinline__ uint64_t advance(uint64_t desc, uint32_t bytes) {
 }
 
 constexpr int kMaxStages = 8;
-constexpr int kNumBarriers = 2 * kMaxStages + 10;
+constexpr int kNumBarriers = 2 * kMaxStages + 12;
 constexpr int kMaxBlocks = 7168;       // streamed blocks of a work item: 458,752 rows
 struct __align__(16) Control {
   float stats[kMaxStages][2][kBlock]; // key items: -lse * log2 e and -delta of the streamed query rows
@@ -352,7 +352,8 @@ struct Chains {
   static constexpr int kChunkBytes = kBlock * 128;
   static constexpr int kAcc0 = 256, kAcc1 = 320, kF = 384;
   static_assert(!kKeys || D == 64, "tensor memory holds two accumulators and the fixed tiles at D = 64 only");
-  enum { kFixed = 0, kSFull = 1, kDPFull = 3, kPDone = 5, kDSDone = 7, kFinal = 9, kFull = 10, kEmpty = kFull + kStages };
+  enum { kFixed = 0, kSFull = 1, kDPFull = 3, kPDone = 5, kDSDone = 7, kFinal = 9, kDPFree = 10, kFull = 12,
+         kEmpty = kFull + kStages };
 
   static __device__ __forceinline__ int arrivals(int i) {
     return i == kFixed ? 16 : (i >= kPDone && i < kFinal) ? 8 : 1;
@@ -384,7 +385,18 @@ struct Chains {
         for (int i = 0; i < 4096 && !ptx::mbar_try_wait(b.bar(kFull + m % kStages), (m / kStages) & 1); ++i) {}
   }
 
+  // Key items: one thread issues all products, which then run in the order of issue: acc1 += P(k) X1, S(k + 2),
+  // acc0 += dS(k - 1) X0, dP(k + 1).  Query items: the first products and the second ones have an issuing thread each.  A
+  // thread hands over an instruction about every 30 clocks and spends about 100 on a wait, at 64 columns the first are as long
+  // as their products take; on the other hand a buffer that is free when a product of the other thread is done costs a
+  // completion and a wait on top.  Two threads / one, dense 18,944 rows alone: query items at D = 128 194 / 206 us, at D = 64
+  // 162 / 160, key items (D = 64) 193 / 174.
   static __device__ __forceinline__ void issue(const Block& b, const BwdArgs& a) {
+    if constexpr (kKeys) issue_all(b, a);
+    else issue_first(b, a);
+  }
+
+  static __device__ __forceinline__ void issue_all(const Block& b, const BwdArgs& a) {
     constexpr uint32_t kIdescS = ptx::idesc_f16(128, kBlock, kBF16, false);
     constexpr uint32_t kIdescG = ptx::idesc_f16(128, D, kBF16, true);
     const uint32_t sX = ptx::smem_u32(b.smem);
@@ -427,7 +439,7 @@ struct Chains {
           ok = ptx::mbar_wait(b.bar(kPDone + (k & 1)), (k >> 1) & 1, b.abort_flag);
           if (!ok) { report(a.status, 3, 1, k); break; }
           ptx::tc_fence_after();
-          if (kKeys) second(0, k);
+          second(0, k);
           if (k + 2 < b.count) {
             ok = landed(k + 2);
             if (!ok) break;
@@ -443,6 +455,68 @@ struct Chains {
           if (k + 1 < b.count) first(1, k + 1);
         }
       }
+    }
+    ptx::tc_commit(b.bar(kFinal));
+  }
+
+  // First products of a query item: S(k) once the chain's scores have been read, dP(k - 1) once the chain's dS(k - 3) X0 is done.
+  static __device__ __forceinline__ void issue_first(const Block& b, const BwdArgs& a) {
+    constexpr uint32_t kIdescS = ptx::idesc_f16(128, kBlock, kBF16, false);
+    const uint64_t dx = ptx::smem_desc_sw128(ptx::smem_u32(b.smem), 16, 1024);      // K-major
+    if (b.count == 0) return;
+    bool ok = true;
+    auto wait = [&](int bar, uint32_t parity, int code, int k) {
+      ok = ok && ptx::mbar_wait(b.bar(bar), parity, b.abort_flag);
+      if (!ok) report(a.status, code, 1, k);
+      ptx::tc_fence_after();
+      return ok;
+    };
+    // which = 0: S = F0 X0^T, 1: dP = F1 X1^T
+    auto first = [&](int which, int k) {
+      const int c = k & 1;
+      const uint64_t b0 = advance(dx, (2 * (k % kStages) + which) * kBlockBytes);
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk)
+        ptx::mma_ts(b.tmem + which * 128 + c * 64, b.tmem + kF + which * (D / 2) + kk * 8,
+                    advance(b0, (kk / 4) * kChunkBytes + (kk % 4) * 32), kIdescS, kk > 0 ? 1u : 0u);
+      ptx::tc_commit(b.bar((which ? kDPFull : kSFull) + c));
+    };
+    if (!wait(kFixed, 0, 2, -1)) return;
+    for (int k = 0; k <= b.count; ++k) {
+      if (k < b.count) {
+        if (k >= 2 && !wait(kPDone + (k & 1), ((k - 2) >> 1) & 1, 3, k)) return;
+        if (!wait(kFull + k % kStages, (k / kStages) & 1, 2, k)) return;
+        first(0, k);
+      }
+      if (k >= 1) {
+        if (k >= 3 && !wait(kDPFree + ((k - 1) & 1), ((k - 3) >> 1) & 1, 4, k)) return;
+        first(1, k - 1);
+      }
+    }
+  }
+
+  // Second products of a query item: acc0 += dS X0.
+  static __device__ __forceinline__ void issue_second(const Block& b, const BwdArgs& a) {
+    if (kKeys) return;
+    constexpr uint32_t kIdescG = ptx::idesc_f16(128, D, kBF16, true);
+    const uint64_t dg = ptx::smem_desc_sw128(ptx::smem_u32(b.smem), kChunkBytes, 1024);       // MN-major
+    bool ok = true;
+    auto wait = [&](int bar, uint32_t parity, int code, int k) {
+      ok = ok && ptx::mbar_wait(b.bar(bar), parity, b.abort_flag);
+      if (!ok) report(a.status, code, 6, k);
+      ptx::tc_fence_after();
+      return ok;
+    };
+    for (int k = 0; k < b.count && ok; ++k) {
+      const int s = k % kStages;
+      if (!wait(kFull + s, (k / kStages) & 1, 2, k) || !wait(kDSDone + (k & 1), (k >> 1) & 1, 4, k)) break;
+      const uint64_t b0 = advance(dg, 2 * s * kBlockBytes);
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+        ptx::mma_ts(b.tmem + kAcc0, b.tmem + 128 + (k & 1) * 64 + (kk >> 1) * 32 + (kk & 1) * 8, advance(b0, kk * 2048), kIdescG,
+                    (k > 0 || kk > 0) ? 1u : 0u);
+      ptx::tc_commit(b.bar(kDPFree + (k & 1)));
+      ptx::tc_commit(b.bar(kEmpty + s));
     }
     ptx::tc_commit(b.bar(kFinal));
   }
@@ -603,6 +677,7 @@ struct Pairs {
     }
   }
 
+  static __device__ __forceinline__ void issue_second(const Block&, const BwdArgs&) {}      // one thread issues all products
   static __device__ __forceinline__ void issue(const Block& b, const BwdArgs& a) {
     constexpr uint32_t kIdescS = ptx::idesc_f16(128, 128, kBF16, false);
     constexpr uint32_t kIdescG = ptx::idesc_f16(128, D, kBF16, true);
@@ -786,6 +861,8 @@ __global__ void __launch_bounds__(kThreads, 1) sparse_attn_bwd_kernel(
     }
   } else if (warp == 1) {
     if (ptx::elect_one()) with_kind([&](auto kind) { kind.issue(b, a); });
+  } else if (warp == 3) {
+    if (ptx::elect_one()) with_kind([&](auto kind) { kind.issue_second(b, a); });
   } else if (warp >= 4) {
     with_kind([&](auto kind) { kind.compute(b, a, ctl, warp, lane); });
   }
