@@ -231,7 +231,12 @@ __device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, uint32_t* r) {
       : "memory");
 }
 // The same threads and rows with the two columns of a thread packed into one 32-bit column: registers 2 g (row i / 4) and
-// 2 g + 1 (row i / 4 + 8) of column group g.  Four groups of 16 lanes.
+// 2 g + 1 (row i / 4 + 8) of column group g.  Two or four groups of 16 lanes.
+__device__ __forceinline__ void tmem_st_16x2g(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x2.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+      "r"(r[3])
+      : "memory");
+}
 __device__ __forceinline__ void tmem_st_16x4g(uint32_t taddr, const uint32_t* r) {
   asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])

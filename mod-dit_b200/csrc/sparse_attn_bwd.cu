@@ -201,12 +201,13 @@ struct KeyRows {
     bool on;
     int split, lo, hi;
   };
-  // zeros in the masked places
-  __device__ __forceinline__ void clear(float (&v)[2][16], const Mask& m) {
+  // zeros in the masked places of column groups [g0, g1)
+  __device__ __forceinline__ void clear(float (&v)[2][16], const Mask& m, int g0, int g1) {
 #pragma unroll
     for (int g = 0; g < 4; ++g)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
+        if (g < g0 || g >= g1) continue;
         const int rows = 8 * g + 2 * static_cast<int>(threadIdx.x % 4) + i < m.split ? m.lo : m.hi;
 #pragma unroll
         for (int row = 0; row < 4; ++row) {
@@ -230,22 +231,36 @@ struct KeyRows {
 #pragma unroll
         for (int j = 0; j < 2; ++j) f(lh, 2 * g + j, g);
   }
-  // P, stored over the first half of the columns of S
+  // P of column groups [kG0, kG0 + kGs), stored over the first half of the columns of S
+  template <int kG0, int kGs>
   __device__ __forceinline__ void probabilities(uint32_t tS, uint64_t scale2, const float* nl, const Mask& m) {
-    uint64_t nl2[4];
 #pragma unroll
-    for (int g = 0; g < 4; ++g) nl2[g] = *reinterpret_cast<const uint64_t*>(nl + 8 * g + 2 * (threadIdx.x % 4));
-    pairs([&](int lh, int i, int g) {
-      float x0, x1;
-      ptx::unpack_f32x2(ptx::fma_f32x2(ptx::pack_f32x2(p[lh][2 * i], p[lh][2 * i + 1]), scale2, nl2[g]), x0, x1);
-      p[lh][2 * i] = ptx::ex2(x0);
-      p[lh][2 * i + 1] = ptx::ex2(x1);
-    });
-    if (m.on) clear(p, m);
-    uint32_t pk[2][8];
-    pairs([&](int lh, int i, int) { pk[lh][i] = pack2<kBF16>(p[lh][2 * i], p[lh][2 * i + 1]); });
-    ptx::tmem_st_16x4g(tS, pk[0]);
-    ptx::tmem_st_16x4g(tS + (16u << 16), pk[1]);
+    for (int g = kG0; g < kG0 + kGs; ++g) {
+      const uint64_t nl2 = *reinterpret_cast<const uint64_t*>(nl + 8 * g + 2 * (threadIdx.x % 4));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float* v = p[i >> 1] + 4 * g + 2 * (i & 1);
+        float x0, x1;
+        ptx::unpack_f32x2(ptx::fma_f32x2(ptx::pack_f32x2(v[0], v[1]), scale2, nl2), x0, x1);
+        v[0] = ptx::ex2(x0);
+        v[1] = ptx::ex2(x1);
+      }
+    }
+    if (m.on) clear(p, m, kG0, kG0 + kGs);
+    uint32_t pk[2][2 * kGs];
+#pragma unroll
+    for (int g = kG0; g < kG0 + kGs; ++g)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float* v = p[i >> 1] + 4 * g + 2 * (i & 1);
+        pk[i >> 1][2 * (g - kG0) + (i & 1)] = pack2<kBF16>(v[0], v[1]);
+      }
+#pragma unroll
+    for (int lh = 0; lh < 2; ++lh) {
+      const uint32_t to = tS + (static_cast<uint32_t>(16 * lh) << 16) + 4 * kG0;
+      if constexpr (kGs == 4) ptx::tmem_st_16x4g(to, pk[lh]);
+      else ptx::tmem_st_16x2g(to, pk[lh]);
+    }
   }
   __device__ __forceinline__ void scores_gradient(uint32_t tP, const float* nd, const Mask& m) {
     uint64_t nd2[4];
@@ -255,7 +270,7 @@ struct KeyRows {
     ptx::tmem_ld_16x32(tP, reinterpret_cast<uint32_t*>(d[0]));
     ptx::tmem_ld_16x32(tP + (16u << 16), reinterpret_cast<uint32_t*>(d[1]));
     ptx::tmem_ld_wait();
-    if (m.on) clear(d, m);            // what lies in a masked place may be anything
+    if (m.on) clear(d, m, 0, 4);         // what lies in a masked place may be anything
     uint32_t pk[2][8];
     pairs([&](int lh, int i, int g) {
       const uint64_t t = ptx::mul_f32x2(minus_delta<kBF16>(ptx::pack_f32x2(d[lh][2 * i], d[lh][2 * i + 1]), nd2[g]),
@@ -587,7 +602,7 @@ struct Chains {
         KeyRows<kBF16> x;
         const typename KeyRows<kBF16>::Mask m{b.row0 + kTile > kv_min, a.q_split - x0 - u * kCols, rows_lo, rows_hi};
         x.load(tS);
-        x.probabilities(tS, scale2, ctl->stats[s][0] + u * kCols, m);
+        x.template probabilities<0, 4>(tS, scale2, ctl->stats[s][0] + u * kCols, m);
         hand_over(b.bar(kPDone + c));
         ok = __all_sync(0xffffffffu, ptx::mbar_wait(b.bar(kDPFull + c), par, b.abort_flag));
         if (!ok) { if (lane == 0) report(a.status, 6, 2 + c, k); break; }
@@ -636,9 +651,9 @@ struct Pairs {
   static constexpr int kTileBytes = kTile * D * 2;
   static constexpr int kChunkBytes = kTile * 128;
   static constexpr int kHalfBytes = kBlock * 128;       // a block's rows of one 64-element chunk
-  enum { kFixed = 0, kSFull, kDPFull, kPDone, kDSDone, kFinal, kFull, kEmpty = kFull + kStages, kUsed = kEmpty + kStages };
+  enum { kFixed = 0, kSFull, kDPFull, kPLo, kPHi, kDSDone, kFinal, kFull, kEmpty = kFull + kStages, kUsed = kEmpty + kStages };
 
-  static __device__ __forceinline__ int arrivals(int i) { return (i == kPDone || i == kDSDone) ? 16 : 1; }
+  static __device__ __forceinline__ int arrivals(int i) { return (i >= kPLo && i <= kDSDone) ? 16 : 1; }
 
   static __device__ __forceinline__ void produce(const Block& b, const BwdArgs& a, const Control* ctl, const CUtensorMap* tf0,
                                                  const CUtensorMap* tf1, const CUtensorMap* tx0, const CUtensorMap* tx1) {
@@ -694,13 +709,13 @@ struct Pairs {
       }
       ptx::tc_commit(b.bar(kSFull + which));
     };
-    // which = 0: acc1 += P X1, 1: acc0 += dS X0; a warpgroup's 32 columns are two steps of 16
-    auto second = [&](int which, int s, uint32_t acc) {
+    // which = 0: acc1 += P X1, 1: acc0 += dS X0, steps kk0, kk0 + by, ... of 16 rows; a warpgroup's 32 columns are two steps
+    auto second = [&](int which, int s, uint32_t acc, int kk0, int by) {
       const uint64_t b0 = advance(dg, (2 * s + 1 - which) * kTileBytes);
 #pragma unroll
-      for (int kk = 0; kk < 8; ++kk)
+      for (int kk = kk0; kk < 8; kk += by)
         ptx::mma_ts(b.tmem + (which ? 256 : 384), b.tmem + which * 128 + (kk >> 1) * 32 + (kk & 1) * 8, advance(b0, kk * 2048),
-                    kIdescG, (acc || kk > 0) ? 1u : 0u);
+                    kIdescG, (acc || kk > kk0) ? 1u : 0u);
     };
     const int steps = (b.count + 1) / 2;
     bool ok = true;
@@ -713,10 +728,14 @@ struct Pairs {
     for (int n = 0; n < steps && ok; ++n) {
       const int s = n % kStages, s1 = (n + 1) % kStages;
       const bool next = n + 1 < steps;
-      ok = ptx::mbar_wait(b.bar(kPDone), n & 1, b.abort_flag);
+      ok = ptx::mbar_wait(b.bar(kPLo), n & 1, b.abort_flag);
       if (!ok) { report(a.status, 3, 1, n); break; }
       ptx::tc_fence_after();
-      second(0, s, n > 0);
+      second(0, s, n > 0, 0, 2);
+      ok = ptx::mbar_wait(b.bar(kPHi), n & 1, b.abort_flag);
+      if (!ok) { report(a.status, 3, 1, n); break; }
+      ptx::tc_fence_after();
+      second(0, s, 1u, 1, 2);
       if (next) {
         ok = ptx::mbar_wait(b.bar(kFull + s1), ((n + 1) / kStages) & 1, b.abort_flag);
         if (!ok) { report(a.status, 2, 1, n); break; }
@@ -726,7 +745,7 @@ struct Pairs {
       ok = ptx::mbar_wait(b.bar(kDSDone), n & 1, b.abort_flag);
       if (!ok) { report(a.status, 4, 1, n); break; }
       ptx::tc_fence_after();
-      second(1, s, n > 0);
+      second(1, s, n > 0, 0, 1);
       ptx::tc_commit(b.bar(kEmpty + s));
       if (next) first(1, s1);
     }
@@ -762,11 +781,14 @@ struct Pairs {
       const typename KeyRows<kBF16>::Mask m{b.row0 + kTile > kv_min, a.q_split - x0 - u * kCols, rows_lo, rows_hi};
       if (mine) {
         x.load(tS);
-        x.probabilities(tS, scale2, ctl->stats[2 * s + h][0] + u * kCols, m);
+        x.template probabilities<0, 2>(tS, scale2, ctl->stats[2 * s + h][0] + u * kCols, m);
+        hand_over(b.bar(kPLo));
+        x.template probabilities<2, 2>(tS, scale2, ctl->stats[2 * s + h][0] + u * kCols, m);
       } else {
         store_zeros(tS);
+        hand_over(b.bar(kPLo));
       }
-      hand_over(b.bar(kPDone));
+      hand_over(b.bar(kPHi));
       ok = __all_sync(0xffffffffu, ptx::mbar_wait(b.bar(kDPFull), n & 1, b.abort_flag));
       if (!ok) { if (lane == 0) report(a.status, 6, 2 + h, n); break; }
       ptx::tc_fence_after();
