@@ -90,12 +90,16 @@ __device__ __forceinline__ Item item_of(const BwdArgs& a) {
 // The streamed 64-row blocks of a work item, in list order, as (first row << 2) | halves: bit i of `halves` says that rows
 // [64 i, 64 i + 64) of the item keep the block.  A list entry names a streamed tile of 128 rows and its kept quarters; blocks
 // that start at or past `limit` are left out.  One warp writes them to shared memory and returns how many there are.
+// The first entries are asked for together with the count (a list has room for `room`).
 template <bool kKeys>
-__device__ __forceinline__ int expand(const int32_t* ent, int count, int shift, int limit, int32_t* blocks) {
+__device__ __forceinline__ int expand(const int32_t* ent, const int32_t* counts, int room, int shift, int limit, int32_t* blocks) {
   const int lane = threadIdx.x % 32;
+  int en_next = lane < room ? __ldg(ent + lane) : 0;
+  const int count = __ldg(counts);
   int n = 0;
   for (int e0 = 0; e0 < count; e0 += 32) {
-    const int en = e0 + lane < count ? __ldg(ent + e0 + lane) : 0;
+    const int en = en_next;
+    en_next = e0 + 32 + lane < count ? __ldg(ent + e0 + 32 + lane) : 0;
     const int fl = en >> shift, x0 = (en >> 8) * kTile;
     int bits[2];
     for (int half = 0; half < 2; ++half) {
@@ -323,6 +327,28 @@ __device__ __forceinline__ void store_rows(uint32_t t, bool any, bool in, float 
   }
 }
 
+// What an elementwise thread of an item with its fixed tiles in tensor memory reads while the block is set up: half of a row of
+// F0 (first 256 threads) or F1, zeros at and past `rows`, and for query items the row's statistics.
+template <int D>
+struct Fixed {
+  uint32_t v[D / 4];
+  float nl, nd;
+  __device__ __forceinline__ void load(const BwdArgs& a, bool keys, int bh, int row0, int rows) {
+    const int t = threadIdx.x - 128, f1 = t / 256, half = (t / 128) & 1, grow = row0 + t % 128;
+    const void* f = keys ? (f1 ? a.v : a.k) : (f1 ? a.dout : a.q);
+    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(f) +
+                                                      (static_cast<int64_t>(bh) * a.N + grow) * D * 2) + half * (D / 16);
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      const uint4 x = grow < rows ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
+      v[4 * i] = x.x; v[4 * i + 1] = x.y; v[4 * i + 2] = x.z; v[4 * i + 3] = x.w;
+    }
+    const int64_t at = static_cast<int64_t>(bh) * a.npad + grow;
+    nl = keys ? 0.f : a.nlse[at];
+    nd = keys ? 0.f : a.ndelta[at];
+  }
+};
+
 struct Block {                        // what all roles of a block know
   unsigned char* smem;                // 1024-byte aligned
   uint32_t tmem;
@@ -536,37 +562,20 @@ struct Chains {
     ptx::tc_commit(b.bar(kFinal));
   }
 
-  // Half of this thread's row of F0 or F1 into tensor memory; rows at and past `rows` are zero.
-  static __device__ __forceinline__ void load_fixed(const Block& b, const BwdArgs& a, const void* f, uint32_t to, int half,
-                                                    int grow, int rows) {
-    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(f) +
-                                                      (static_cast<int64_t>(b.bh) * a.N + grow) * D * 2) + half * (D / 16);
-    uint32_t v[D / 4];
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-      const uint4 x = grow < rows ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
-      v[4 * i] = x.x; v[4 * i + 1] = x.y; v[4 * i + 2] = x.z; v[4 * i + 3] = x.w;
-    }
-    if constexpr (D == 128) ptx::tmem_st32(to + half * 32, v);
-    else ptx::tmem_st16(to + half * 16, v);
-    hand_over(b.bar(kFixed));
-  }
-
-  static __device__ __forceinline__ void compute(const Block& b, const BwdArgs& a, const Control* ctl, int warp, int lane) {
+  static __device__ __forceinline__ void compute(const Block& b, const BwdArgs& a, const Control* ctl, const Fixed<D>& fixed, int warp,
+                                                 int lane) {
     const int c = (warp - 4) / 8;                 // chain
     const int u = ((warp - 4) / 4) & 1;           // half of its columns
     const int wq = warp % 4;                      // tensor-memory lane quarter
     const int grow = b.row0 + wq * 32 + lane;
     const uint32_t lane_base = static_cast<uint32_t>(wq * 32) << 16;
     const uint32_t tS = b.tmem + lane_base + c * 64 + u * kCols, tP = tS + 128;
-    const int kv_min = min(a.kvl_lo, a.kvl_hi), kv_max = max(a.kvl_lo, a.kvl_hi);
-    load_fixed(b, a, kKeys ? (c ? a.v : a.k) : (c ? a.dout : a.q), b.tmem + lane_base + kF + c * (D / 2), u, grow,
-               kKeys ? kv_max : a.N);
-    float nl = 0.f, nd = 0.f;
-    if (!kKeys) {
-      nl = a.nlse[static_cast<int64_t>(b.bh) * a.npad + grow];
-      nd = a.ndelta[static_cast<int64_t>(b.bh) * a.npad + grow];
-    }
+    const int kv_min = min(a.kvl_lo, a.kvl_hi);
+    const uint32_t tF = b.tmem + lane_base + kF + c * (D / 2) + u * (D / 4);
+    if constexpr (D == 128) ptx::tmem_st32(tF, fixed.v);
+    else ptx::tmem_st16(tF, fixed.v);
+    hand_over(b.bar(kFixed));
+    const float nl = fixed.nl, nd = fixed.nd;
     const int lim = grow < a.q_split ? a.kvl_lo : a.kvl_hi;
     int rows_lo = 0, rows_hi = 0;                 // key items: which of this thread's four rows lie below the limits
     if (kKeys)
@@ -752,7 +761,8 @@ struct Pairs {
     ptx::tc_commit(b.bar(kFinal));
   }
 
-  static __device__ __forceinline__ void compute(const Block& b, const BwdArgs& a, const Control* ctl, int warp, int lane) {
+  static __device__ __forceinline__ void compute(const Block& b, const BwdArgs& a, const Control* ctl, const Fixed<D>&, int warp,
+                                                 int lane) {
     const int h = (warp - 4) / 8;                 // which of the two streamed blocks
     const int u = ((warp - 4) / 4) & 1;           // half of its columns
     const int wq = warp % 4;
@@ -863,12 +873,13 @@ __global__ void __launch_bounds__(kThreads, 1) sparse_attn_bwd_kernel(
     ptx::tmem_relinquish();
     ptx::tc_fence_before();
   }
+  Fixed<D> fixed;
+  if (warp >= 4 && !(D == 128 && it.keys)) fixed.load(a, it.keys, b.bh, b.row0, it.keys ? kv_max : a.N);
   if (warp == 3) {
-    const int count = (it.keys && b.row0 >= kv_max) ? 0 : __ldg(l.counts + item);
     const int32_t* ent = l.entries + static_cast<int64_t>(item) * a.ntiles;
-    const int n = it.keys ? expand<true>(ent, count, 0, a.N, ctl->blocks)
-                          : expand<false>(ent, count, 4 * (it.pos & 1), kv_max, ctl->blocks);
-    if (lane == 0) ctl->count = n;
+    const int n = it.keys ? expand<true>(ent, l.counts + item, a.ntiles, 0, a.N, ctl->blocks)
+                          : expand<false>(ent, l.counts + item, a.ntiles, 4 * (it.pos & 1), kv_max, ctl->blocks);
+    if (lane == 0) ctl->count = (it.keys && b.row0 >= kv_max) ? 0 : n;      // keys that no row may see
   }
   __syncthreads();
   ptx::tc_fence_after();
@@ -886,7 +897,7 @@ __global__ void __launch_bounds__(kThreads, 1) sparse_attn_bwd_kernel(
   } else if (warp == 3) {
     if (ptx::elect_one()) with_kind([&](auto kind) { kind.issue_second(b, a); });
   } else if (warp >= 4) {
-    with_kind([&](auto kind) { kind.compute(b, a, ctl, warp, lane); });
+    with_kind([&](auto kind) { kind.compute(b, a, ctl, fixed, warp, lane); });
   }
 
   ptx::tc_fence_before();

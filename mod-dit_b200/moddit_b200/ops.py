@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes
 import os
 import threading
+import time
 from typing import Dict, Optional, Tuple
 
 import torch
@@ -921,14 +922,22 @@ def raise_on_status(device) -> None:
         raise _status_error(vals)
 
 
-def post_status(device) -> None:
+_LAST_POST: Dict[int, float] = {}      # device index -> when `post_status` last queued a copy
+
+
+def post_status(device, spacing: float = 0.0) -> None:
     """Queues a copy of the status words into pinned host memory behind the work already on the current stream
     and records an event after it.  Costs no synchronisation; `check_posted_status` looks at the copy later.
-    While the stream is being captured it does nothing: an event of a captured graph cannot be asked."""
+    While the stream is being captured it does nothing: an event of a captured graph cannot be asked.  `spacing`: nothing
+    either within so many seconds of the last copy - the words stay set, so a later copy reports them too."""
     if torch.cuda.is_current_stream_capturing():
         return
     device = torch.device(device)
     idx = device.index if device.index is not None else torch.cuda.current_device()
+    now = time.monotonic()
+    if spacing and now - _LAST_POST.get(idx, 0.0) < spacing:
+        return
+    _LAST_POST[idx] = now
     slot = _POSTED.get(idx)
     if slot is None:
         slot = [torch.zeros(4, dtype=torch.int32).pin_memory(), None]
@@ -969,9 +978,9 @@ def check_health(device) -> None:
             f"position={vals[3]}); the sparsity maps written since the last check are invalid")
 
 
-def _after_launch(dev, check_status) -> None:
+def _after_launch(dev, check_status, spacing: float = 0.0) -> None:
     if check_status == "deferred":
-        post_status(dev)
+        post_status(dev, spacing)
     elif check_status:
         raise_on_status(dev)
 
@@ -1092,5 +1101,6 @@ def sparse_attn_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
             D ** -0.5 if softmax_scale is None else softmax_scale, N if q_split is None else q_split,
             N if kv_len_lo is None else kv_len_lo, N if kv_len_hi is None else kv_len_hi, dq.data_ptr(), dk.data_ptr(),
             dv.data_ptr(), ws.data_ptr(), wsb, _status_words(dev).data_ptr(), _stream(dev)), "moddit_sparse_attn_bwd")
-    _after_launch(dev, check_status)
+    # the copy and its change of engines hold up a stream of short launches by some ten microseconds each
+    _after_launch(dev, check_status, spacing=1e-3)
     return dq, dk, dv
