@@ -36,8 +36,10 @@
 namespace moddit {
 namespace {
 
-constexpr int kThreads = 640;          // 4 control warps, 4 warpgroups
 constexpr int kCols = 32;              // streamed columns of a thread
+// 4 control warps, then warpgroups of elementwise work
+template <int D>
+constexpr int kThreads = D == 64 ? 512 : 640;
 constexpr int kTile = 128;             // rows of a work item
 constexpr int kBlock = 64;             // streamed rows that are kept or left out together
 constexpr float kLog2e = 1.4426950408889634f;
@@ -327,25 +329,30 @@ __device__ __forceinline__ void store_rows(uint32_t t, bool any, bool in, float 
   }
 }
 
-// What an elementwise thread of an item with its fixed tiles in tensor memory reads while the block is set up: half of a row of
-// F0 (first 256 threads) or F1, zeros at and past `rows`, and for query items the row's statistics.
+// What an elementwise thread of a query item reads while the block is set up: 32 words of a row of Q or dO (which end up in
+// tensor memory; at D = 64 two warpgroups have a row each, at D = 128 four half a row), zeros past the last row, and the row's
+// statistics.
 template <int D>
 struct Fixed {
-  uint32_t v[D / 4];
+  uint32_t v[32];
   float nl, nd;
-  __device__ __forceinline__ void load(const BwdArgs& a, bool keys, int bh, int row0, int rows) {
-    const int t = threadIdx.x - 128, f1 = t / 256, half = (t / 128) & 1, grow = row0 + t % 128;
-    const void* f = keys ? (f1 ? a.v : a.k) : (f1 ? a.dout : a.q);
-    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(f) +
-                                                      (static_cast<int64_t>(bh) * a.N + grow) * D * 2) + half * (D / 16);
+  static __device__ __forceinline__ int group() { return (static_cast<int>(threadIdx.x) - 128) / 128; }
+  static __device__ __forceinline__ int which() { return D == 64 ? group() : group() / 2; }
+  static __device__ __forceinline__ int part() { return D == 64 ? 0 : group() & 1; }
+  static __device__ __forceinline__ bool mine() { return which() < 2; }
+  __device__ __forceinline__ void load(const BwdArgs& a, int bh, int row0) {
+    const int grow = row0 + threadIdx.x % 128;
+    const int64_t at = static_cast<int64_t>(bh) * a.npad + grow;
+    nl = a.nlse[at];
+    nd = a.ndelta[at];
+    if (!mine()) return;
+    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(which() ? a.dout : a.q) +
+                                                      (static_cast<int64_t>(bh) * a.N + grow) * D * 2) + part() * 8;
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-      const uint4 x = grow < rows ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < 8; ++i) {
+      const uint4 x = grow < a.N ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
       v[4 * i] = x.x; v[4 * i + 1] = x.y; v[4 * i + 2] = x.z; v[4 * i + 3] = x.w;
     }
-    const int64_t at = static_cast<int64_t>(bh) * a.npad + grow;
-    nl = keys ? 0.f : a.nlse[at];
-    nd = keys ? 0.f : a.ndelta[at];
   }
 };
 
@@ -359,13 +366,21 @@ struct Block {                        // what all roles of a block know
   __device__ __forceinline__ uint32_t bar(int i) const { return bar0 + 8u * static_cast<uint32_t>(i); }
 };
 
+// Waits for a barrier's phase; most are complete when they are asked for (a complete one costs an issuing thread about 100 clocks
+// through try_wait).
+__device__ __forceinline__ bool await(const Block& b, const BwdArgs& a, int role, int bar, uint32_t parity, int code, int k) {
+  if (ptx::mbar_test(b.bar(bar), parity) || ptx::mbar_wait(b.bar(bar), parity, b.abort_flag)) return true;
+  report(a.status, code, role, k);
+  return false;
+}
+
 __device__ __forceinline__ uint64_t advance(uint64_t desc, uint32_t bytes) {
   // the start-address field (bits 0-13, units of 16 bytes) never carries out for shared-memory addresses
   return (desc & 0xffffffff00000000ull) | static_cast<uint32_t>(static_cast<uint32_t>(desc) + (bytes >> 4));
 }
 
 constexpr int kMaxStages = 8;
-constexpr int kNumBarriers = 2 * kMaxStages + 12;
+constexpr int kNumBarriers = 2 * kMaxStages + 18;
 constexpr int kMaxBlocks = 7168;       // streamed blocks of a work item: 458,752 rows
 struct __align__(16) Control {
   float stats[kMaxStages][2][kBlock]; // key items: -lse * log2 e and -delta of the streamed query rows
@@ -378,31 +393,54 @@ struct __align__(16) Control {
 
 // bytes of tiles in shared memory; behind them the control block, before them up to 1024 bytes of alignment
 template <int D>
-constexpr size_t kTilesBytes = static_cast<size_t>(D == 128 ? 192 : 128) * 1024;
+constexpr size_t kTilesBytes = static_cast<size_t>(D == 128 ? 192 : 160) * 1024;
 
 // ---------------------------------------------------------------------------------------------------------------
-// Two chains: warpgroups 2 c and 2 c + 1 take the streamed blocks c, c + 2, c + 4, ... through scores, dP and dS of its own, half a step
-// behind the other one, so that one has exponentials to do while the other one waits or packs.  The fixed tiles live in
-// tensor memory as A operands, which halves what the products read from shared memory.
-// Tensor memory: S_c [64 c, 64 c + 64), dP_c 128 + the same, acc0 [256, 256 + D), acc1 behind it (D = 64), F0, F1 from 384 on.
+// Chains: warpgroups of their own take every kC-th streamed block through scores, dP and dS of its own, a part of a step behind
+// the other chains, so that some have exponentials to do while the others wait or pack.
+//   D = 128 (query items)  two chains of two warpgroups, 32 columns a thread
+//   D = 64                 three chains of one warpgroup, 64 columns a thread: the waits and the latencies of a step are bound
+//                          here, not a unit, and a third chain hides more of them than a second warpgroup of a chain.
+// Fixed tiles live in tensor memory as A operands where there is room (query items), which halves what the first products read
+// from shared memory.
+// Tensor memory: S_c [64 c, 64 c + 64), then dP_c likewise, then the accumulators and F0, F1.
 template <int D, bool kBF16, bool kKeys>
 struct Chains {
+  static constexpr int kC = D == 64 ? 3 : 2;            // chains
+  static constexpr int kG = D == 64 ? 1 : 2;            // warpgroups of a chain
+  static constexpr int kU = 2 / kG;                     // units of kCols columns of a thread
   static constexpr int kStages = D == 128 ? 6 : 8;
   static constexpr int kBlockBytes = kBlock * D * 2;
+  static constexpr int kTileBytes = kTile * D * 2;
   static constexpr int kChunks = D / 64;
   static constexpr int kChunkBytes = kBlock * 128;
-  static constexpr int kAcc0 = 256, kAcc1 = 320, kF = 384;
-  static_assert(!kKeys || D == 64, "tensor memory holds two accumulators and the fixed tiles at D = 64 only");
-  enum { kFixed = 0, kSFull = 1, kDPFull = 3, kPDone = 5, kDSDone = 7, kFinal = 9, kDPFree = 10, kFull = 12,
-         kEmpty = kFull + kStages };
+  static constexpr int kStagesAt = kKeys ? 2 * kTileBytes : 0;
+  static constexpr int kDP = 64 * kC, kAcc0 = 128 * kC, kAcc1 = kAcc0 + 64, kF = kAcc0 + D;
+  static_assert(!kKeys || D == 64, "tensor memory holds two accumulators at D = 64 only");
+  static_assert((kKeys ? kAcc1 + 64 : kF + D) <= 512, "tensor memory");
+  static_assert(kStagesAt + 2 * kStages * kBlockBytes <= static_cast<int>(kTilesBytes<D>), "shared memory");
+  enum { kFixed = 0, kSFull = 1, kDPFull = kSFull + kC, kPDone = kDPFull + kC, kDSDone = kPDone + kC, kDPFree = kDSDone + kC,
+         kFinal = kDPFree + kC, kFull, kEmpty = kFull + kStages, kUsed = kEmpty + kStages };
+  static_assert(static_cast<int>(kUsed) <= kNumBarriers, "barriers");
 
-  static __device__ __forceinline__ int arrivals(int i) {
-    return i == kFixed ? 16 : (i >= kPDone && i < kFinal) ? 8 : 1;
+  static __device__ __forceinline__ int arrivals(int i) {               // one per warp, copy or commit
+    return i == kFixed ? (kKeys ? 1 : D == 64 ? 8 : 16) : (i >= kPDone && i < kDPFree) ? 4 * kG : 1;
   }
+  // a block's place in the barriers' phases
+  static __device__ __forceinline__ int chain(int k) { return k % kC; }
+  static __device__ __forceinline__ uint32_t phase(int k) { return (k / kC) & 1; }
 
-  static __device__ __forceinline__ void produce(const Block& b, const BwdArgs& a, const Control* ctl, const CUtensorMap* tx0,
-                                                 const CUtensorMap* tx1) {
-    const uint32_t sX = ptx::smem_u32(b.smem);
+  static __device__ __forceinline__ void produce(const Block& b, const BwdArgs& a, const Control* ctl, const CUtensorMap* tf0,
+                                                 const CUtensorMap* tf1, const CUtensorMap* tx0, const CUtensorMap* tx1) {
+    if (b.count == 0) return;
+    const uint32_t sF = ptx::smem_u32(b.smem), sX = sF + kStagesAt;
+    if (kKeys) {
+      ptx::mbar_expect_tx(b.bar(kFixed), 2 * kTileBytes);
+      for (int h = 0; h < 2; ++h) {
+        ptx::tma_load_3d(sF + h * kBlockBytes, tf0, b.bar(kFixed), 0, b.row0 + h * kBlock, b.bh);
+        ptx::tma_load_3d(sF + kTileBytes + h * kBlockBytes, tf1, b.bar(kFixed), 0, b.row0 + h * kBlock, b.bh);
+      }
+    }
     bool ok = true;
     int k = 0;
     for (; k < b.count; ++k) {
@@ -421,160 +459,123 @@ struct Chains {
         ptx::bulk_load(ptx::smem_u32(ctl->stats[s][1]), a.ndelta + at, kBlock * 4, b.bar(kFull + s));
       }
     }
-    if (!ok)        // give copies in flight a bounded time to land (their barriers may never be consumed)
+    if (!ok) {      // give copies in flight a bounded time to land (their barriers may never be consumed)
+      if (kKeys)
+        for (int i = 0; i < 4096 && !ptx::mbar_try_wait(b.bar(kFixed), 0); ++i) {}
       for (int m = max(0, k - kStages); m < k; ++m)
         for (int i = 0; i < 4096 && !ptx::mbar_try_wait(b.bar(kFull + m % kStages), (m / kStages) & 1); ++i) {}
+    }
   }
 
-  // Key items: one thread issues all products, which then run in the order of issue: acc1 += P(k) X1, S(k + 2),
-  // acc0 += dS(k - 1) X0, dP(k + 1).  Query items: the first products and the second ones have an issuing thread each.  A
+  // The products of block k.  which = 0: S = F0 X0^T, 1: dP = F1 X1^T
+  static __device__ __forceinline__ void first(const Block& b, int which, int k) {
+    constexpr uint32_t kIdesc = ptx::idesc_f16(128, kBlock, kBF16, false);
+    const uint32_t sF = ptx::smem_u32(b.smem);
+    const uint64_t b0 = ptx::smem_desc_sw128(sF + kStagesAt + (2 * (k % kStages) + which) * kBlockBytes, 16, 1024);      // K-major
+    const uint64_t a0 = ptx::smem_desc_sw128(sF + which * kTileBytes, 16, 1024);
+    const uint32_t d = b.tmem + which * kDP + chain(k) * 64;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      const uint64_t bk = advance(b0, (kk / 4) * kChunkBytes + (kk % 4) * 32);
+      if constexpr (kKeys) ptx::mma_ss(d, advance(a0, kk * 32), bk, kIdesc, kk > 0 ? 1u : 0u);
+      else ptx::mma_ts(d, b.tmem + kF + which * (D / 2) + kk * 8, bk, kIdesc, kk > 0 ? 1u : 0u);
+    }
+    ptx::tc_commit(b.bar((which ? kDPFull : kSFull) + chain(k)));
+  }
+  // which = 0: acc1 += P X1, 1: acc0 += dS X0
+  static __device__ __forceinline__ void second(const Block& b, int which, int k) {
+    constexpr uint32_t kIdesc = ptx::idesc_f16(128, D, kBF16, true);
+    const uint64_t b0 = ptx::smem_desc_sw128(ptx::smem_u32(b.smem) + kStagesAt + (2 * (k % kStages) + 1 - which) * kBlockBytes,
+                                             kChunkBytes, 1024);       // MN-major
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk)
+      ptx::mma_ts(b.tmem + (which ? kAcc0 : kAcc1), b.tmem + which * kDP + chain(k) * 64 + (kk >> 1) * 32 + (kk & 1) * 8,
+                  advance(b0, kk * 2048), kIdesc, (k > 0 || kk > 0) ? 1u : 0u);
+  }
+
+  // Key items: one thread issues all products, which then run in the order of issue: acc1 += P(k) X1, S(k + kC),
+  // acc0 += dS(k - 1) X0, dP(k - 1 + kC).  Query items: the first products and the second ones have an issuing thread each.  A
   // thread hands over an instruction about every 30 clocks and spends about 100 on a wait, at 64 columns the first are as long
   // as their products take; on the other hand a buffer that is free when a product of the other thread is done costs a
-  // completion and a wait on top.  Two threads / one, dense 18,944 rows alone: query items at D = 128 194 / 206 us, at D = 64
-  // 162 / 160, key items (D = 64) 193 / 174.
-  static __device__ __forceinline__ void issue(const Block& b, const BwdArgs& a) {
-    if constexpr (kKeys) issue_all(b, a);
-    else issue_first(b, a);
+  // completion and a wait on top.  Two threads / one, dense 18,944 rows alone, two chains: query items at D = 128 194 / 206 us,
+  // at D = 64 162 / 160, key items (D = 64) 193 / 174.
+  static __device__ __forceinline__ bool landed(const Block& b, const BwdArgs& a, int role, int k) {
+    return await(b, a, role, kFull + k % kStages, (k / kStages) & 1, 2, k);
+  }
+  // for what the elementwise warps have read from or written to tensor memory
+  static __device__ __forceinline__ bool wait(const Block& b, const BwdArgs& a, int role, int bar, uint32_t parity, int code, int k) {
+    const bool ok = await(b, a, role, bar, parity, code, k);
+    ptx::tc_fence_after();
+    return ok;
   }
 
-  static __device__ __forceinline__ void issue_all(const Block& b, const BwdArgs& a) {
-    constexpr uint32_t kIdescS = ptx::idesc_f16(128, kBlock, kBF16, false);
-    constexpr uint32_t kIdescG = ptx::idesc_f16(128, D, kBF16, true);
-    const uint32_t sX = ptx::smem_u32(b.smem);
-    const uint64_t dx = ptx::smem_desc_sw128(sX, 16, 1024);                // K-major
-    const uint64_t dg = ptx::smem_desc_sw128(sX, kChunkBytes, 1024);       // MN-major
-    // which = 0: S = F0 X0^T, 1: dP = F1 X1^T
-    auto first = [&](int which, int k) {
-      const int c = k & 1;
-      const uint64_t b0 = advance(dx, (2 * (k % kStages) + which) * kBlockBytes);
-#pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk)
-        ptx::mma_ts(b.tmem + which * 128 + c * 64, b.tmem + kF + which * (D / 2) + kk * 8,
-                    advance(b0, (kk / 4) * kChunkBytes + (kk % 4) * 32), kIdescS, kk > 0 ? 1u : 0u);
-      ptx::tc_commit(b.bar((which ? kDPFull : kSFull) + c));
-    };
-    // which = 0: acc1 += P X1, 1: acc0 += dS X0
-    auto second = [&](int which, int k) {
-      const uint64_t b0 = advance(dg, (2 * (k % kStages) + 1 - which) * kBlockBytes);
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk)
-        ptx::mma_ts(b.tmem + (which ? kAcc0 : kAcc1), b.tmem + which * 128 + (k & 1) * 64 + (kk >> 1) * 32 + (kk & 1) * 8, advance(b0, kk * 2048),
-                    kIdescG, (k > 0 || kk > 0) ? 1u : 0u);
-    };
-    auto landed = [&](int k) {
-      const bool ok = ptx::mbar_wait(b.bar(kFull + k % kStages), (k / kStages) & 1, b.abort_flag);
-      if (!ok) report(a.status, 2, 1, k);
-      ptx::tc_fence_after();
-      return ok;
-    };
-    if (b.count > 0) {
-      bool ok = ptx::mbar_wait(b.bar(kFixed), 0, b.abort_flag);
-      if (!ok) report(a.status, 2, 1, -1);
-      ptx::tc_fence_after();
-      for (int k = 0; k < 2 && ok && k < b.count; ++k) {
-        ok = landed(k);
-        if (ok) { first(0, k); first(1, k); }
+  static __device__ __forceinline__ void issue(const Block& b, const BwdArgs& a) {
+    if constexpr (kKeys) {
+      bool ok = b.count == 0 || wait(b, a, 1, kFixed, 0, 2, -1);
+      for (int k = 0; k < min(kC, b.count) && ok; ++k) {
+        ok = landed(b, a, 1, k);
+        if (ok) { first(b, 0, k); first(b, 1, k); }
       }
-      for (int k = 0; ok && k <= b.count; ++k) {
+      for (int k = 0; ok && k <= b.count && b.count > 0; ++k) {
         if (k < b.count) {
-          ok = ptx::mbar_wait(b.bar(kPDone + (k & 1)), (k >> 1) & 1, b.abort_flag);
-          if (!ok) { report(a.status, 3, 1, k); break; }
-          ptx::tc_fence_after();
-          second(0, k);
-          if (k + 2 < b.count) {
-            ok = landed(k + 2);
-            if (!ok) break;
-            first(0, k + 2);
+          if (!wait(b, a, 1, kPDone + chain(k), phase(k), 3, k)) break;
+          second(b, 0, k);
+          if (k + kC < b.count) {
+            if (!landed(b, a, 1, k + kC)) break;
+            first(b, 0, k + kC);
           }
         }
         if (k > 0) {
-          ok = ptx::mbar_wait(b.bar(kDSDone + ((k - 1) & 1)), ((k - 1) >> 1) & 1, b.abort_flag);
-          if (!ok) { report(a.status, 4, 1, k); break; }
-          ptx::tc_fence_after();
-          second(1, k - 1);
+          if (!wait(b, a, 1, kDSDone + chain(k - 1), phase(k - 1), 4, k)) break;
+          second(b, 1, k - 1);
           ptx::tc_commit(b.bar(kEmpty + (k - 1) % kStages));
-          if (k + 1 < b.count) first(1, k + 1);
+          if (k - 1 + kC < b.count) first(b, 1, k - 1 + kC);
+        }
+      }
+      ptx::tc_commit(b.bar(kFinal));
+    } else {
+      // S(k) once the chain's scores have been read, dP(k - 1) once the chain's last dS has been multiplied
+      if (b.count == 0 || !wait(b, a, 1, kFixed, 0, 2, -1)) return;
+      for (int k = 0; k <= b.count; ++k) {
+        if (k < b.count) {
+          if (k >= kC && !wait(b, a, 1, kPDone + chain(k), phase(k - kC), 3, k)) return;
+          if (!landed(b, a, 1, k)) return;
+          first(b, 0, k);
+        }
+        if (k >= 1) {
+          if (k - 1 >= kC && !wait(b, a, 1, kDPFree + chain(k - 1), phase(k - 1 - kC), 4, k)) return;
+          first(b, 1, k - 1);
         }
       }
     }
-    ptx::tc_commit(b.bar(kFinal));
   }
 
-  // First products of a query item: S(k) once the chain's scores have been read, dP(k - 1) once the chain's dS(k - 3) X0 is done.
-  static __device__ __forceinline__ void issue_first(const Block& b, const BwdArgs& a) {
-    constexpr uint32_t kIdescS = ptx::idesc_f16(128, kBlock, kBF16, false);
-    const uint64_t dx = ptx::smem_desc_sw128(ptx::smem_u32(b.smem), 16, 1024);      // K-major
-    if (b.count == 0) return;
-    bool ok = true;
-    auto wait = [&](int bar, uint32_t parity, int code, int k) {
-      ok = ok && ptx::mbar_wait(b.bar(bar), parity, b.abort_flag);
-      if (!ok) report(a.status, code, 1, k);
-      ptx::tc_fence_after();
-      return ok;
-    };
-    // which = 0: S = F0 X0^T, 1: dP = F1 X1^T
-    auto first = [&](int which, int k) {
-      const int c = k & 1;
-      const uint64_t b0 = advance(dx, (2 * (k % kStages) + which) * kBlockBytes);
-#pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk)
-        ptx::mma_ts(b.tmem + which * 128 + c * 64, b.tmem + kF + which * (D / 2) + kk * 8,
-                    advance(b0, (kk / 4) * kChunkBytes + (kk % 4) * 32), kIdescS, kk > 0 ? 1u : 0u);
-      ptx::tc_commit(b.bar((which ? kDPFull : kSFull) + c));
-    };
-    if (!wait(kFixed, 0, 2, -1)) return;
-    for (int k = 0; k <= b.count; ++k) {
-      if (k < b.count) {
-        if (k >= 2 && !wait(kPDone + (k & 1), ((k - 2) >> 1) & 1, 3, k)) return;
-        if (!wait(kFull + k % kStages, (k / kStages) & 1, 2, k)) return;
-        first(0, k);
-      }
-      if (k >= 1) {
-        if (k >= 3 && !wait(kDPFree + ((k - 1) & 1), ((k - 3) >> 1) & 1, 4, k)) return;
-        first(1, k - 1);
-      }
-    }
-  }
-
-  // Second products of a query item: acc0 += dS X0.
   static __device__ __forceinline__ void issue_second(const Block& b, const BwdArgs& a) {
-    if (kKeys) return;
-    constexpr uint32_t kIdescG = ptx::idesc_f16(128, D, kBF16, true);
-    const uint64_t dg = ptx::smem_desc_sw128(ptx::smem_u32(b.smem), kChunkBytes, 1024);       // MN-major
-    bool ok = true;
-    auto wait = [&](int bar, uint32_t parity, int code, int k) {
-      ok = ok && ptx::mbar_wait(b.bar(bar), parity, b.abort_flag);
-      if (!ok) report(a.status, code, 6, k);
-      ptx::tc_fence_after();
-      return ok;
-    };
-    for (int k = 0; k < b.count && ok; ++k) {
-      const int s = k % kStages;
-      if (!wait(kFull + s, (k / kStages) & 1, 2, k) || !wait(kDSDone + (k & 1), (k >> 1) & 1, 4, k)) break;
-      const uint64_t b0 = advance(dg, 2 * s * kBlockBytes);
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk)
-        ptx::mma_ts(b.tmem + kAcc0, b.tmem + 128 + (k & 1) * 64 + (kk >> 1) * 32 + (kk & 1) * 8, advance(b0, kk * 2048), kIdescG,
-                    (k > 0 || kk > 0) ? 1u : 0u);
-      ptx::tc_commit(b.bar(kDPFree + (k & 1)));
-      ptx::tc_commit(b.bar(kEmpty + s));
+    if constexpr (!kKeys) {
+      for (int k = 0; k < b.count; ++k) {
+        if (!landed(b, a, 6, k) || !wait(b, a, 6, kDSDone + chain(k), phase(k), 4, k)) break;
+        second(b, 1, k);
+        ptx::tc_commit(b.bar(kDPFree + chain(k)));
+        ptx::tc_commit(b.bar(kEmpty + k % kStages));
+      }
+      ptx::tc_commit(b.bar(kFinal));
     }
-    ptx::tc_commit(b.bar(kFinal));
   }
 
   static __device__ __forceinline__ void compute(const Block& b, const BwdArgs& a, const Control* ctl, const Fixed<D>& fixed, int warp,
                                                  int lane) {
-    const int c = (warp - 4) / 8;                 // chain
-    const int u = ((warp - 4) / 4) & 1;           // half of its columns
+    const int wg = (warp - 4) / 4;
+    const int c = wg / kG;                        // chain
+    const int u0 = wg % kG;                       // first unit of this thread
     const int wq = warp % 4;                      // tensor-memory lane quarter
     const int grow = b.row0 + wq * 32 + lane;
-    const uint32_t lane_base = static_cast<uint32_t>(wq * 32) << 16;
-    const uint32_t tS = b.tmem + lane_base + c * 64 + u * kCols, tP = tS + 128;
+    const uint32_t t = b.tmem + (static_cast<uint32_t>(wq * 32) << 16);
+    const uint32_t tS = t + c * 64 + u0 * kCols, tP = tS + kDP;
     const int kv_min = min(a.kvl_lo, a.kvl_hi);
-    const uint32_t tF = b.tmem + lane_base + kF + c * (D / 2) + u * (D / 4);
-    if constexpr (D == 128) ptx::tmem_st32(tF, fixed.v);
-    else ptx::tmem_st16(tF, fixed.v);
-    hand_over(b.bar(kFixed));
+    if (!kKeys && fixed.mine()) {
+      ptx::tmem_st32(t + kF + fixed.which() * (D / 2) + fixed.part() * 32, fixed.v);
+      hand_over(b.bar(kFixed));
+    }
     const float nl = fixed.nl, nd = fixed.nd;
     const int lim = grow < a.q_split ? a.kvl_lo : a.kvl_hi;
     int rows_lo = 0, rows_hi = 0;                 // key items: which of this thread's four rows lie below the limits
@@ -586,65 +587,71 @@ struct Chains {
       }
     const uint64_t scale2 = ptx::pack_f32x2(a.scale_log2, a.scale_log2);
     bool ok = true;
-    int next = b.blocks[c];           // read ahead; past the end it is not used
-    for (int k = c; k < b.count; k += 2) {
-      const int x0 = next >> 2, bits = next & 3;
-      next = b.blocks[k + 2];
-      const uint32_t par = (k >> 1) & 1;
-      const int s = k % kStages;
-      ok = ptx::mbar_wait(b.bar(kSFull + c), par, b.abort_flag);      // the statistics came with the operands
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) { if (lane == 0) report(a.status, 5, 2 + c, k); break; }
+    auto wait_all = [&](int bar, uint32_t parity, int code, int k) {
+      ok = __all_sync(0xffffffffu, ptx::mbar_wait(b.bar(bar), parity, b.abort_flag));
+      if (!ok && lane == 0) report(a.status, code, 2 + c, k);
       ptx::tc_fence_after();
-      const bool mine = (bits >> (wq >> 1)) & 1;
-      if (!mine) {                                // these rows keep nothing of the block
-        if (kKeys) store_zeros(tS);
+      return ok;
+    };
+    int next = b.blocks[c];           // read ahead; past the end it is not used
+    uint32_t par = 0;
+    for (int k = c; k < b.count; k += kC, par ^= 1) {
+      const int x0 = next >> 2, bits = next & 3;
+      next = b.blocks[k + kC];
+      const int s = k % kStages;
+      if (!wait_all(kSFull + c, par, 5, k)) break;      // the statistics came with the operands
+      if (!((bits >> (wq >> 1)) & 1)) {           // these rows keep nothing of the block
+        if (kKeys)
+          for (int u = 0; u < kU; ++u) store_zeros(tS + u * kCols);
         hand_over(b.bar(kPDone + c));
-        ok = __all_sync(0xffffffffu, ptx::mbar_wait(b.bar(kDPFull + c), par, b.abort_flag));
-        if (!ok) { if (lane == 0) report(a.status, 6, 2 + c, k); break; }
-        ptx::tc_fence_after();
-        store_zeros(tP);
+        if (!wait_all(kDPFull + c, par, 6, k)) break;
+        for (int u = 0; u < kU; ++u) store_zeros(tP + u * kCols);
         hand_over(b.bar(kDSDone + c));
         continue;
       }
       if constexpr (kKeys) {
-        KeyRows<kBF16> x;
-        const typename KeyRows<kBF16>::Mask m{b.row0 + kTile > kv_min, a.q_split - x0 - u * kCols, rows_lo, rows_hi};
-        x.load(tS);
-        x.template probabilities<0, 4>(tS, scale2, ctl->stats[s][0] + u * kCols, m);
+        KeyRows<kBF16> x[kU];
+        const float* stats = ctl->stats[s][0] + u0 * kCols;
+        typename KeyRows<kBF16>::Mask m{b.row0 + kTile > kv_min, a.q_split - x0 - u0 * kCols, rows_lo, rows_hi};
+#pragma unroll
+        for (int u = 0; u < kU; ++u) x[u].load(tS + u * kCols);
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+          x[u].template probabilities<0, 4>(tS + u * kCols, scale2, stats + u * kCols, m);
+          m.split -= kCols;
+        }
         hand_over(b.bar(kPDone + c));
-        ok = __all_sync(0xffffffffu, ptx::mbar_wait(b.bar(kDPFull + c), par, b.abort_flag));
-        if (!ok) { if (lane == 0) report(a.status, 6, 2 + c, k); break; }
-        ptx::tc_fence_after();
-        x.scores_gradient(tP, ctl->stats[s][1] + u * kCols, m);
+        if (!wait_all(kDPFull + c, par, 6, k)) break;
+        m.split += kU * kCols;
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+          x[u].scores_gradient(tP + u * kCols, stats + kBlock + u * kCols, m);
+          m.split -= kCols;
+        }
       } else {
-        QueryRows<kBF16> x;
-        const int below = lim - x0 - u * kCols;
-        x.load(tS);
+        QueryRows<kBF16> x[kU];
+        const int below = lim - x0 - u0 * kCols;
+#pragma unroll
+        for (int u = 0; u < kU; ++u) x[u].load(tS + u * kCols);
         ptx::tc_fence_before();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(b.bar(kPDone + c));      // P stays in registers: the next scores may overwrite these
-        x.probabilities(scale2, nl, below);
-        ok = __all_sync(0xffffffffu, ptx::mbar_wait(b.bar(kDPFull + c), par, b.abort_flag));
-        if (!ok) { if (lane == 0) report(a.status, 6, 2 + c, k); break; }
-        ptx::tc_fence_after();
-        x.scores_gradient(tP, nd, below);
+#pragma unroll
+        for (int u = 0; u < kU; ++u) x[u].probabilities(scale2, nl, below - u * kCols);
+        if (!wait_all(kDPFull + c, par, 6, k)) break;
+#pragma unroll
+        for (int u = 0; u < kU; ++u) x[u].scores_gradient(tP + u * kCols, nd, below - u * kCols);
       }
       hand_over(b.bar(kDSDone + c));
     }
-    if (ok) {
-      ok = __all_sync(0xffffffffu, ptx::mbar_wait(b.bar(kFinal), 0, b.abort_flag));
-      if (!ok && lane == 0) report(a.status, 7, 2 + c, -1);
+    if (!ok || !wait_all(kFinal, 0, 7, -1)) return;
+    // 32 columns of an accumulator at a time for each warpgroup
+    for (int unit = wg; unit < (kKeys ? 2 : 1) * (D / 32); unit += kC * kG) {
+      const int which = unit / (D / 32), col = unit % (D / 32) * 32;
+      const int64_t at = ((static_cast<int64_t>(b.bh) * a.N + grow) * D + col) * 2;
+      store_rows<kBF16, 32>(t + (which ? kAcc1 : kAcc0) + col, b.count > 0, grow < a.N, which ? (kBF16 ? 1.f : exp2f(-kHalfShift)) : a.scale,
+                            reinterpret_cast<uint4*>(static_cast<unsigned char*>(which ? a.dv : kKeys ? a.dk : a.dq) + at));
     }
-    if (!ok) return;
-    ptx::tc_fence_after();
-    const int64_t at = (static_cast<int64_t>(b.bh) * a.N + grow) * D * 2;
-    const int col = (2 * c + u) * (D / 4);
-    auto to = [&](void* g) { return reinterpret_cast<uint4*>(static_cast<unsigned char*>(g) + at + 2 * col); };
-    const bool in = grow < a.N;
-    const uint32_t t = b.tmem + lane_base + col;
-    store_rows<kBF16, D / 4>(t + kAcc0, b.count > 0, in, a.scale, to(kKeys ? a.dk : a.dq));
-    if (kKeys) store_rows<kBF16, D / 4>(t + kAcc1, b.count > 0, in, kBF16 ? 1.f : exp2f(-kHalfShift), to(a.dv));
   }
 };
 
@@ -729,30 +736,23 @@ struct Pairs {
     const int steps = (b.count + 1) / 2;
     bool ok = true;
     if (steps > 0) {
-      ok = ptx::mbar_wait(b.bar(kFixed), 0, b.abort_flag) && ptx::mbar_wait(b.bar(kFull), 0, b.abort_flag);
-      if (!ok) report(a.status, 2, 1, -1);
-      ptx::tc_fence_after();
+      ok = await(b, a, 1, kFixed, 0, 2, -1) && await(b, a, 1, kFull, 0, 2, -1);
       if (ok) { first(0, 0); first(1, 0); }
     }
     for (int n = 0; n < steps && ok; ++n) {
       const int s = n % kStages, s1 = (n + 1) % kStages;
       const bool next = n + 1 < steps;
-      ok = ptx::mbar_wait(b.bar(kPLo), n & 1, b.abort_flag);
-      if (!ok) { report(a.status, 3, 1, n); break; }
+      if (!await(b, a, 1, kPLo, n & 1, 3, n)) break;
       ptx::tc_fence_after();
       second(0, s, n > 0, 0, 2);
-      ok = ptx::mbar_wait(b.bar(kPHi), n & 1, b.abort_flag);
-      if (!ok) { report(a.status, 3, 1, n); break; }
+      if (!await(b, a, 1, kPHi, n & 1, 3, n)) break;
       ptx::tc_fence_after();
       second(0, s, 1u, 1, 2);
       if (next) {
-        ok = ptx::mbar_wait(b.bar(kFull + s1), ((n + 1) / kStages) & 1, b.abort_flag);
-        if (!ok) { report(a.status, 2, 1, n); break; }
-        ptx::tc_fence_after();
+        if (!await(b, a, 1, kFull + s1, ((n + 1) / kStages) & 1, 2, n)) break;
         first(0, s1);
       }
-      ok = ptx::mbar_wait(b.bar(kDSDone), n & 1, b.abort_flag);
-      if (!ok) { report(a.status, 4, 1, n); break; }
+      if (!await(b, a, 1, kDSDone, n & 1, 4, n)) break;
       ptx::tc_fence_after();
       second(1, s, n > 0, 0, 1);
       ptx::tc_commit(b.bar(kEmpty + s));
@@ -823,7 +823,7 @@ struct Pairs {
 };
 
 template <int D, bool kBF16>
-__global__ void __launch_bounds__(kThreads, 1) sparse_attn_bwd_kernel(
+__global__ void __launch_bounds__(kThreads<D>, 1) sparse_attn_bwd_kernel(
     const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
     const __grid_constant__ CUtensorMap tm_do, const __grid_constant__ BwdArgs a) {
   using Queries = Chains<D, kBF16, false>;
@@ -874,7 +874,7 @@ __global__ void __launch_bounds__(kThreads, 1) sparse_attn_bwd_kernel(
     ptx::tc_fence_before();
   }
   Fixed<D> fixed;
-  if (warp >= 4 && !(D == 128 && it.keys)) fixed.load(a, it.keys, b.bh, b.row0, it.keys ? kv_max : a.N);
+  if (warp >= 4 && !it.keys) fixed.load(a, b.bh, b.row0);
   if (warp == 3) {
     const int32_t* ent = l.entries + static_cast<int64_t>(item) * a.ntiles;
     const int n = it.keys ? expand<true>(ent, l.counts + item, a.ntiles, 0, a.N, ctl->blocks)
@@ -888,9 +888,10 @@ __global__ void __launch_bounds__(kThreads, 1) sparse_attn_bwd_kernel(
 
   if (warp == 0) {
     if (ptx::elect_one()) {
-      if (!it.keys) Queries::produce(b, a, ctl, &tm_k, &tm_v);
-      else if constexpr (D == 128) Pairs<kBF16>::produce(b, a, ctl, &tm_k, &tm_v, &tm_q, &tm_do);
-      else Chains<64, kBF16, true>::produce(b, a, ctl, &tm_q, &tm_do);
+      with_kind([&](auto kind) {
+        if (it.keys) kind.produce(b, a, ctl, &tm_k, &tm_v, &tm_q, &tm_do);
+        else kind.produce(b, a, ctl, nullptr, nullptr, &tm_k, &tm_v);
+      });
     }
   } else if (warp == 1) {
     if (ptx::elect_one()) with_kind([&](auto kind) { kind.issue(b, a); });
@@ -963,7 +964,7 @@ int launch(BwdArgs a, const void* out, const void* lo, const float* lse, int dty
                                                                                   ws + static_cast<int64_t>(BH) * a.npad);
   MODDIT_CHECK_LAUNCH("bwd_stats_kernel");
   const int64_t blocks = static_cast<int64_t>(2 * a.ntiles + (a.ntiles & 1)) * BH;
-  kernel<<<static_cast<unsigned>(blocks), kThreads, smem, st>>>(tq, tk, tv, tdo, a);
+  kernel<<<static_cast<unsigned>(blocks), kThreads<D>, smem, st>>>(tq, tk, tv, tdo, a);
   MODDIT_CHECK_LAUNCH("sparse_attn_bwd_kernel");
   return MODDIT_OK;
 }
