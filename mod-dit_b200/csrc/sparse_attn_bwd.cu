@@ -426,9 +426,16 @@ struct Chains {
   static __device__ __forceinline__ int arrivals(int i) {               // one per warp, copy or commit
     return i == kFixed ? (kKeys ? 1 : D == 64 ? 8 : 16) : (i >= kPDone && i < kDPFree) ? 4 * kG : 1;
   }
-  // a block's place in the barriers' phases
-  static __device__ __forceinline__ int chain(int k) { return k % kC; }
-  static __device__ __forceinline__ uint32_t phase(int k) { return (k / kC) & 1; }
+  // A block's stage and chain and the phases of their barriers, counted along: the issuing threads share their schedulers with
+  // busy warps, so every instruction between two products shows.
+  struct Place {
+    int s = 0, c = 0;
+    uint32_t stage_phase = 0, chain_phase = 0;
+    __device__ __forceinline__ void next() {
+      if (++s == kStages) { s = 0; stage_phase ^= 1; }
+      if (++c == kC) { c = 0; chain_phase ^= 1; }
+    }
+  };
 
   static __device__ __forceinline__ void produce(const Block& b, const BwdArgs& a, const Control* ctl, const CUtensorMap* tf0,
                                                  const CUtensorMap* tf1, const CUtensorMap* tx0, const CUtensorMap* tx1) {
@@ -467,30 +474,30 @@ struct Chains {
     }
   }
 
-  // The products of block k.  which = 0: S = F0 X0^T, 1: dP = F1 X1^T
-  static __device__ __forceinline__ void first(const Block& b, int which, int k) {
+  // The products of a block.  which = 0: S = F0 X0^T, 1: dP = F1 X1^T
+  static __device__ __forceinline__ void first(const Block& b, int which, const Place& p) {
     constexpr uint32_t kIdesc = ptx::idesc_f16(128, kBlock, kBF16, false);
     const uint32_t sF = ptx::smem_u32(b.smem);
-    const uint64_t b0 = ptx::smem_desc_sw128(sF + kStagesAt + (2 * (k % kStages) + which) * kBlockBytes, 16, 1024);      // K-major
-    const uint64_t a0 = ptx::smem_desc_sw128(sF + which * kTileBytes, 16, 1024);
-    const uint32_t d = b.tmem + which * kDP + chain(k) * 64;
+    const uint64_t b0 = advance(ptx::smem_desc_sw128(sF + kStagesAt + which * kBlockBytes, 16, 1024), 2 * p.s * kBlockBytes);
+    const uint64_t a0 = ptx::smem_desc_sw128(sF + which * kTileBytes, 16, 1024);      // both K-major
+    const uint32_t d = b.tmem + which * kDP + p.c * 64;
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
       const uint64_t bk = advance(b0, (kk / 4) * kChunkBytes + (kk % 4) * 32);
       if constexpr (kKeys) ptx::mma_ss(d, advance(a0, kk * 32), bk, kIdesc, kk > 0 ? 1u : 0u);
       else ptx::mma_ts(d, b.tmem + kF + which * (D / 2) + kk * 8, bk, kIdesc, kk > 0 ? 1u : 0u);
     }
-    ptx::tc_commit(b.bar((which ? kDPFull : kSFull) + chain(k)));
+    ptx::tc_commit(b.bar((which ? kDPFull : kSFull) + p.c));
   }
-  // which = 0: acc1 += P X1, 1: acc0 += dS X0
-  static __device__ __forceinline__ void second(const Block& b, int which, int k) {
+  // which = 0: acc1 += P X1, 1: acc0 += dS X0; acc: whether there is anything in the accumulator yet
+  static __device__ __forceinline__ void second(const Block& b, int which, const Place& p, uint32_t acc) {
     constexpr uint32_t kIdesc = ptx::idesc_f16(128, D, kBF16, true);
-    const uint64_t b0 = ptx::smem_desc_sw128(ptx::smem_u32(b.smem) + kStagesAt + (2 * (k % kStages) + 1 - which) * kBlockBytes,
-                                             kChunkBytes, 1024);       // MN-major
+    const uint64_t b0 = advance(ptx::smem_desc_sw128(ptx::smem_u32(b.smem) + kStagesAt + (1 - which) * kBlockBytes, kChunkBytes, 1024),
+                                2 * p.s * kBlockBytes);       // MN-major
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk)
-      ptx::mma_ts(b.tmem + (which ? kAcc0 : kAcc1), b.tmem + which * kDP + chain(k) * 64 + (kk >> 1) * 32 + (kk & 1) * 8,
-                  advance(b0, kk * 2048), kIdesc, (k > 0 || kk > 0) ? 1u : 0u);
+      ptx::mma_ts(b.tmem + (which ? kAcc0 : kAcc1), b.tmem + which * kDP + p.c * 64 + (kk >> 1) * 32 + (kk & 1) * 8,
+                  advance(b0, kk * 2048), kIdesc, kk > 0 ? 1u : acc);
   }
 
   // Key items: one thread issues all products, which then run in the order of issue: acc1 += P(k) X1, S(k + kC),
@@ -499,8 +506,8 @@ struct Chains {
   // as their products take; on the other hand a buffer that is free when a product of the other thread is done costs a
   // completion and a wait on top.  Two threads / one, dense 18,944 rows alone, two chains: query items at D = 128 194 / 206 us,
   // at D = 64 162 / 160, key items (D = 64) 193 / 174.
-  static __device__ __forceinline__ bool landed(const Block& b, const BwdArgs& a, int role, int k) {
-    return await(b, a, role, kFull + k % kStages, (k / kStages) & 1, 2, k);
+  static __device__ __forceinline__ bool landed(const Block& b, const BwdArgs& a, int role, const Place& p, int k) {
+    return await(b, a, role, kFull + p.s, p.stage_phase, 2, k);
   }
   // for what the elementwise warps have read from or written to tensor memory
   static __device__ __forceinline__ bool wait(const Block& b, const BwdArgs& a, int role, int bar, uint32_t parity, int code, int k) {
@@ -510,41 +517,56 @@ struct Chains {
   }
 
   static __device__ __forceinline__ void issue(const Block& b, const BwdArgs& a) {
+    if (b.count == 0) {
+      if (kKeys) ptx::tc_commit(b.bar(kFinal));
+      return;
+    }
+    if (!wait(b, a, 1, kFixed, 0, 2, -1)) return;
+    Place ahead, here, behind;        // blocks k + kC (whose first products are next), k and k - 1
     if constexpr (kKeys) {
-      bool ok = b.count == 0 || wait(b, a, 1, kFixed, 0, 2, -1);
-      for (int k = 0; k < min(kC, b.count) && ok; ++k) {
-        ok = landed(b, a, 1, k);
-        if (ok) { first(b, 0, k); first(b, 1, k); }
+      bool ok = true;
+      for (int k = 0; k < min(kC, b.count) && ok; ++k, ahead.next()) {
+        ok = landed(b, a, 1, ahead, k);
+        if (ok) { first(b, 0, ahead); first(b, 1, ahead); }
       }
-      for (int k = 0; ok && k <= b.count && b.count > 0; ++k) {
+      Place ahead_dp = ahead;
+      for (int k = 0; ok && k <= b.count; ++k) {
         if (k < b.count) {
-          if (!wait(b, a, 1, kPDone + chain(k), phase(k), 3, k)) break;
-          second(b, 0, k);
+          if (!wait(b, a, 1, kPDone + here.c, here.chain_phase, 3, k)) break;
+          second(b, 0, here, k > 0);
+          here.next();
           if (k + kC < b.count) {
-            if (!landed(b, a, 1, k + kC)) break;
-            first(b, 0, k + kC);
+            if (!landed(b, a, 1, ahead, k + kC)) break;
+            first(b, 0, ahead);
+            ahead.next();
           }
         }
         if (k > 0) {
-          if (!wait(b, a, 1, kDSDone + chain(k - 1), phase(k - 1), 4, k)) break;
-          second(b, 1, k - 1);
-          ptx::tc_commit(b.bar(kEmpty + (k - 1) % kStages));
-          if (k - 1 + kC < b.count) first(b, 1, k - 1 + kC);
+          if (!wait(b, a, 1, kDSDone + behind.c, behind.chain_phase, 4, k)) break;
+          second(b, 1, behind, k > 1);
+          ptx::tc_commit(b.bar(kEmpty + behind.s));
+          behind.next();
+          if (k - 1 + kC < b.count) {
+            first(b, 1, ahead_dp);
+            ahead_dp.next();
+          }
         }
       }
       ptx::tc_commit(b.bar(kFinal));
     } else {
-      // S(k) once the chain's scores have been read, dP(k - 1) once the chain's last dS has been multiplied
-      if (b.count == 0 || !wait(b, a, 1, kFixed, 0, 2, -1)) return;
+      // S(k) once the chain's scores have been read, dP(k - 1) once the chain's last dS has been multiplied: a chain's barriers
+      // are in the other phase of its last block then
       for (int k = 0; k <= b.count; ++k) {
         if (k < b.count) {
-          if (k >= kC && !wait(b, a, 1, kPDone + chain(k), phase(k - kC), 3, k)) return;
-          if (!landed(b, a, 1, k)) return;
-          first(b, 0, k);
+          if (k >= kC && !wait(b, a, 1, kPDone + here.c, here.chain_phase ^ 1, 3, k)) return;
+          if (!landed(b, a, 1, here, k)) return;
+          first(b, 0, here);
+          here.next();
         }
         if (k >= 1) {
-          if (k - 1 >= kC && !wait(b, a, 1, kDPFree + chain(k - 1), phase(k - 1 - kC), 4, k)) return;
-          first(b, 1, k - 1);
+          if (k - 1 >= kC && !wait(b, a, 1, kDPFree + behind.c, behind.chain_phase ^ 1, 4, k)) return;
+          first(b, 1, behind);
+          behind.next();
         }
       }
     }
@@ -552,11 +574,12 @@ struct Chains {
 
   static __device__ __forceinline__ void issue_second(const Block& b, const BwdArgs& a) {
     if constexpr (!kKeys) {
-      for (int k = 0; k < b.count; ++k) {
-        if (!landed(b, a, 6, k) || !wait(b, a, 6, kDSDone + chain(k), phase(k), 4, k)) break;
-        second(b, 1, k);
-        ptx::tc_commit(b.bar(kDPFree + chain(k)));
-        ptx::tc_commit(b.bar(kEmpty + k % kStages));
+      Place here;
+      for (int k = 0; k < b.count; ++k, here.next()) {
+        if (!landed(b, a, 6, here, k) || !wait(b, a, 6, kDSDone + here.c, here.chain_phase, 4, k)) break;
+        second(b, 1, here, k > 0);
+        ptx::tc_commit(b.bar(kDPFree + here.c));
+        ptx::tc_commit(b.bar(kEmpty + here.s));
       }
       ptx::tc_commit(b.bar(kFinal));
     }
