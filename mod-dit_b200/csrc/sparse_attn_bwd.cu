@@ -424,7 +424,9 @@ struct Chains {
   static_assert(static_cast<int>(kUsed) <= kNumBarriers, "barriers");
 
   static __device__ __forceinline__ int arrivals(int i) {               // one per warp, copy or commit
-    return i == kFixed ? (kKeys ? 1 : D == 64 ? 8 : 16) : (i >= kPDone && i < kDPFree) ? 4 * kG : 1;
+    if (i == kFixed) return kKeys ? 1 : D == 64 ? 8 : 16;
+    if (i >= kPDone && i < kDPFree) return 4 * kG;
+    return kKeys && (i == kFinal || i >= kEmpty) ? 2 : 1;               // key items: of both issuing threads
   }
   // A block's stage and chain and the phases of their barriers, counted along: the issuing threads share their schedulers with
   // busy warps, so every instruction between two products shows.
@@ -500,12 +502,6 @@ struct Chains {
                   advance(b0, kk * 2048), kIdesc, kk > 0 ? 1u : acc);
   }
 
-  // Key items: one thread issues all products, which then run in the order of issue: acc1 += P(k) X1, S(k + kC),
-  // acc0 += dS(k - 1) X0, dP(k - 1 + kC).  Query items: the first products and the second ones have an issuing thread each.  A
-  // thread hands over an instruction about every 30 clocks and spends about 100 on a wait, at 64 columns the first are as long
-  // as their products take; on the other hand a buffer that is free when a product of the other thread is done costs a
-  // completion and a wait on top.  Two threads / one, dense 18,944 rows alone, two chains: query items at D = 128 194 / 206 us,
-  // at D = 64 162 / 160, key items (D = 64) 193 / 174.
   static __device__ __forceinline__ bool landed(const Block& b, const BwdArgs& a, int role, const Place& p, int k) {
     return await(b, a, role, kFull + p.s, p.stage_phase, 2, k);
   }
@@ -516,46 +512,42 @@ struct Chains {
     return ok;
   }
 
-  static __device__ __forceinline__ void issue(const Block& b, const BwdArgs& a) {
-    if (b.count == 0) {
-      if (kKeys) ptx::tc_commit(b.bar(kFinal));
-      return;
+  // Two issuing threads.  Products of one thread run in the order of issue; a thread hands over an instruction about every 30
+  // clocks, spends up to 100 on a wait and shares its scheduler with busy warps, so one for everything is the bound.
+  // By sides: thread 0 has acc1 += P(k) X1 (key items) and S(k + kC), which overwrites that P; thread 1 has acc0 += dS(k) X0 and
+  // dP(k + kC), which overwrites that dS.  No column of tensor memory is shared.
+  // By kinds (query items at D = 64): thread 0 has the first products, thread 1 the second; dP(k + kC) then waits for the
+  // completion of dS(k) X0, but thread 0 fills both buffers as soon as either is free.
+  // Dense 18,944 rows alone, all by one thread / by sides / by kinds: key items at D = 64 171 / 167 / 193 us, query items at
+  // D = 64 160 / 158 / 147, at D = 128 201 / 183 / 189; key items at D = 128 (Pairs) 264 / 280 / -.  A third thread for dP alone:
+  // 156 and 199.
+  static __device__ __forceinline__ void issue_side(const Block& b, const BwdArgs& a, int side) {
+    const int role = side ? 6 : 1;
+    Place here, ahead;                // of blocks k and k + kC
+    bool ok = b.count == 0 || wait(b, a, role, kFixed, 0, 2, -1);
+    for (int k = 0; k < min(kC, b.count) && ok; ++k, ahead.next()) {
+      ok = landed(b, a, role, ahead, k);
+      if (ok) first(b, side, ahead);
     }
-    if (!wait(b, a, 1, kFixed, 0, 2, -1)) return;
-    Place ahead, here, behind;        // blocks k + kC (whose first products are next), k and k - 1
-    if constexpr (kKeys) {
-      bool ok = true;
-      for (int k = 0; k < min(kC, b.count) && ok; ++k, ahead.next()) {
-        ok = landed(b, a, 1, ahead, k);
-        if (ok) { first(b, 0, ahead); first(b, 1, ahead); }
+    for (int k = 0; k < b.count && ok; ++k, here.next(), ahead.next()) {
+      if (!wait(b, a, role, (side ? kDSDone : kPDone) + here.c, here.chain_phase, 3, k)) break;
+      if (kKeys || side) {
+        second(b, side, here, k > 0);
+        ptx::tc_commit(b.bar(kEmpty + here.s));
       }
-      Place ahead_dp = ahead;
-      for (int k = 0; ok && k <= b.count; ++k) {
-        if (k < b.count) {
-          if (!wait(b, a, 1, kPDone + here.c, here.chain_phase, 3, k)) break;
-          second(b, 0, here, k > 0);
-          here.next();
-          if (k + kC < b.count) {
-            if (!landed(b, a, 1, ahead, k + kC)) break;
-            first(b, 0, ahead);
-            ahead.next();
-          }
-        }
-        if (k > 0) {
-          if (!wait(b, a, 1, kDSDone + behind.c, behind.chain_phase, 4, k)) break;
-          second(b, 1, behind, k > 1);
-          ptx::tc_commit(b.bar(kEmpty + behind.s));
-          behind.next();
-          if (k - 1 + kC < b.count) {
-            first(b, 1, ahead_dp);
-            ahead_dp.next();
-          }
-        }
+      if (k + kC < b.count) {
+        if (!landed(b, a, role, ahead, k + kC)) break;
+        first(b, side, ahead);
       }
-      ptx::tc_commit(b.bar(kFinal));
-    } else {
-      // S(k) once the chain's scores have been read, dP(k - 1) once the chain's last dS has been multiplied: a chain's barriers
-      // are in the other phase of its last block then
+    }
+    if (kKeys || side) ptx::tc_commit(b.bar(kFinal));
+  }
+
+  static __device__ __forceinline__ void issue_kind(const Block& b, const BwdArgs& a, int kind) {
+    if (kind == 0) {
+      // a chain's barriers are in the other phase of its last block
+      if (b.count == 0 || !wait(b, a, 1, kFixed, 0, 2, -1)) return;
+      Place here, behind;             // blocks k and k - 1
       for (int k = 0; k <= b.count; ++k) {
         if (k < b.count) {
           if (k >= kC && !wait(b, a, 1, kPDone + here.c, here.chain_phase ^ 1, 3, k)) return;
@@ -569,11 +561,7 @@ struct Chains {
           behind.next();
         }
       }
-    }
-  }
-
-  static __device__ __forceinline__ void issue_second(const Block& b, const BwdArgs& a) {
-    if constexpr (!kKeys) {
+    } else {
       Place here;
       for (int k = 0; k < b.count; ++k, here.next()) {
         if (!landed(b, a, 6, here, k) || !wait(b, a, 6, kDSDone + here.c, here.chain_phase, 4, k)) break;
@@ -583,6 +571,11 @@ struct Chains {
       }
       ptx::tc_commit(b.bar(kFinal));
     }
+  }
+
+  static __device__ __forceinline__ void issue(const Block& b, const BwdArgs& a, int thread) {
+    if constexpr (!kKeys && D == 64) issue_kind(b, a, thread);
+    else issue_side(b, a, thread);
   }
 
   static __device__ __forceinline__ void compute(const Block& b, const BwdArgs& a, const Control* ctl, const Fixed<D>& fixed, int warp,
@@ -731,8 +724,8 @@ struct Pairs {
     }
   }
 
-  static __device__ __forceinline__ void issue_second(const Block&, const BwdArgs&) {}      // one thread issues all products
-  static __device__ __forceinline__ void issue(const Block& b, const BwdArgs& a) {
+  static __device__ __forceinline__ void issue(const Block& b, const BwdArgs& a, int thread) {
+    if (thread != 0) return;
     constexpr uint32_t kIdescS = ptx::idesc_f16(128, 128, kBF16, false);
     constexpr uint32_t kIdescG = ptx::idesc_f16(128, D, kBF16, true);
     const uint32_t sF = ptx::smem_u32(b.smem), sX = sF + 2 * kTileBytes;
@@ -917,9 +910,9 @@ __global__ void __launch_bounds__(kThreads<D>, 1) sparse_attn_bwd_kernel(
       });
     }
   } else if (warp == 1) {
-    if (ptx::elect_one()) with_kind([&](auto kind) { kind.issue(b, a); });
+    if (ptx::elect_one()) with_kind([&](auto kind) { kind.issue(b, a, 0); });
   } else if (warp == 3) {
-    if (ptx::elect_one()) with_kind([&](auto kind) { kind.issue_second(b, a); });
+    if (ptx::elect_one()) with_kind([&](auto kind) { kind.issue(b, a, 1); });
   } else if (warp >= 4) {
     with_kind([&](auto kind) { kind.compute(b, a, ctl, fixed, warp, lane); });
   }
