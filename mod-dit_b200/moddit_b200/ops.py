@@ -34,7 +34,7 @@ KERNELS_PER_CALL = {"moddit_pool_blocks": 1, "moddit_pooled_map": 1, "moddit_poo
                     # the stages of a prediction in one call: 3 + 2 + 3 (1 with the small solve) + 1 + 1 + 2
                     "moddit_predict_lines": 12, "moddit_predict_lines (small)": 10,
                     "moddit_mts_noalloc": 2, "moddit_copy_rows_dma": 0, "moddit_qkv_prologue": 1,
-                    "moddit_qkv_prologue_bwd": 2}
+                    "moddit_qkv_prologue_bwd": 2, "moddit_qkv_prologue_bwd (no parameters)": 1}
 
 
 def stage_timing(enable: bool, only=None, by_stage: bool = True) -> None:
@@ -362,7 +362,7 @@ def qkv_prologue_bwd(dq: Optional[torch.Tensor], dk: Optional[torch.Tensor], dv:
     if any(r is not None for r in res.values()):
         wsb = lib.moddit_qkv_prologue_bwd_workspace_bytes(B, S, H, D, kind)
         ws = torch.empty(wsb, device=dev, dtype=torch.uint8)
-    with _entry("moddit_qkv_prologue_bwd", dev):
+    with _entry("moddit_qkv_prologue_bwd" + ("" if wsb else " (no parameters)"), dev):
         check(lib.moddit_qkv_prologue_bwd(
             _addr(dq), _addr(dk), _addr(dv), _addr(inputs[0]), _addr(inputs[1]), dt, B, S, H, D, stride, kind, _addr(q_weight),
             _addr(k_weight), eps, _addr(rope_cos), _addr(rope_sin), _lib.ROPE_FORM[rope_form], lo, hi, N, src_row0,
@@ -1084,6 +1084,8 @@ def sparse_attn_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
     _need_contig(dout=dout, q=q, k=k, v=v, out=out, lse=lse)
     if residual is not None:
         _need_contig(residual=residual)
+    if not isinstance(key_lists, KeyLists) or isinstance(lists, KeyLists):
+        raise TypeError("lists must come from tile_lists and key_lists from key_lists")
     nt = (N + 127) // 128
     _need_lists(lists, (nt + 1) // 2, nt, dev, "tile_lists")
     _need_lists(key_lists, nt, nt, dev, "key_lists")

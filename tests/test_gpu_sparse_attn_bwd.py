@@ -143,3 +143,83 @@ def test_key_lists(ops, bs, N, H, density, limit):
             assert torch.equal(entries[h, t, :rows.numel()], (rows << 8) | bits[h, rows.long(), t])
     order = lists.order.cpu().flatten()
     assert torch.equal(order.sort().values, torch.arange(H * nt, dtype=torch.int32))
+
+
+def test_refusals(ops):
+    """What only a device call can tell: shapes, types, layouts and lists that do not belong together."""
+    q, k, v, dout = (t.cuda() for t in make(1, 2, 200, 64, torch.float16, 1))
+    mask = torch.ones(2, 2, 2, dtype=torch.bool, device="cuda")
+    lists, klists = ops.tile_lists(mask, 128, 200), ops.key_lists(mask, 128, 200)
+    out, lse = ops.sparse_attn_fwd(q, k, v, *lists, return_lse=True)
+    good = dict(dout=dout, q=q, k=k, v=v, out=out, lse=lse, lists=lists, key_lists=klists)
+
+    def refused(error, text, **kw):
+        with pytest.raises(error, match=text):
+            ops.sparse_attn_bwd(**{**good, **kw})
+
+    refused(ValueError, "identical shapes", dout=dout[:, :, :100].contiguous())
+    refused(ValueError, "identical shapes", v=v.bfloat16())
+    refused(ValueError, "identical shapes", residual=out.bfloat16())
+    refused(ValueError, "contiguous", dout=dout.transpose(1, 2).contiguous().transpose(1, 2))
+    refused(ValueError, "lse", lse=lse.half())
+    refused(ValueError, "lse", lse=lse[:, :1])
+    refused(TypeError, "float16 or bfloat16", **{n: good[n].float() for n in ("dout", "q", "k", "v", "out")})
+    refused(TypeError, "key_lists", lists=klists, key_lists=lists)
+    refused(TypeError, "key_lists", key_lists=lists)
+    refused(ValueError, "sequence length", key_lists=ops.key_lists(torch.ones(2, 3, 3, dtype=torch.bool, device="cuda"), 128, 300))
+    refused(ValueError, "one mask", key_lists=ops.key_lists(mask[:1], 128, 200))
+    refused(ValueError, "kv_len", kv_len_lo=201)
+    refused(ValueError, "softmax_scale", softmax_scale=-1.0)
+    refused(ValueError, "CUDA", lse=lse.cpu())
+    with pytest.raises(ValueError, match="one launch"):
+        ops.sparse_attn_fwd(q, k, v, *lists, return_residual=True, pairs_beside=4)
+    odd = torch.empty(q.numel() + 4, device="cuda", dtype=q.dtype)[4:].view(q.shape)      # 8 bytes off a 16-byte boundary
+    refused(RuntimeError, "aligned", q=odd)
+    wide = [torch.zeros(1, 2, 200, 96, device="cuda", dtype=torch.float16) for _ in range(5)]
+    refused(RuntimeError, "head_dim", **dict(zip(("dout", "q", "k", "v", "out"), wide)))
+    ops.sparse_attn_bwd(**good)
+
+
+def test_batches_share_a_mask_head_by_head(ops):
+    """Head bh of a batch of two uses mask head bh % Hm, with limits, at both head dimensions: each sample equals its own call."""
+    for D in (64, 128):
+        q, k, v, dout = (t.cuda() for t in make(2, 4, 450, D, torch.bfloat16, D))
+        mask = (torch.rand(2, 8, 8, generator=torch.Generator().manual_seed(3)) < 0.6).cuda()
+        lists, klists = ops.tile_lists(mask, 64, 450), ops.key_lists(mask, 64, 450)
+        kw = dict(q_split=300, kv_len_lo=448, kv_len_hi=401)
+        out, lse = ops.sparse_attn_fwd(q, k, v, *lists, order=lists.order, return_lse=True, **kw)
+        got = ops.sparse_attn_bwd(dout, q, k, v, out, lse, lists, klists, **kw)
+        for b in range(2):
+            for h in range(0, 4, 2):
+                part = [t[b:b + 1, h:h + 2].contiguous() for t in (dout, q, k, v, out, lse)]
+                want = ops.sparse_attn_bwd(*part, lists, klists, **kw)
+                assert all(torch.equal(g[b:b + 1, h:h + 2], w) for g, w in zip(got, want))
+
+
+def test_long_rows_of_few_blocks(ops):
+    """65,600 rows: lists of tiles far apart, a column that every row keeps and rows that keep everything, against the same
+    gradients of the kept blocks gathered into a short dense problem in 64 bits."""
+    N, D, bs = 65600, 128, 128
+    nb = (N + bs - 1) // bs
+    q, k, v, dout = (t.cuda() for t in make(1, 1, N, D, torch.bfloat16, 9))
+    mask = torch.zeros(1, nb, nb, dtype=torch.bool, device="cuda")
+    cols = [0, 17, 400, nb - 1]
+    mask[0, 300, cols] = True
+    mask[0, nb - 1, cols[1:]] = True
+    lists, klists = ops.tile_lists(mask, bs, N), ops.key_lists(mask, bs, N)
+    out, lse = ops.sparse_attn_fwd(q, k, v, *lists, return_lse=True)
+    dq, dk, dv = ops.sparse_attn_bwd(dout, q, k, v, out, lse, lists, klists)
+    rows = torch.cat([torch.arange(300 * bs, 301 * bs), torch.arange((nb - 1) * bs, N)])
+    keys = torch.cat([torch.arange(c * bs, min(N, (c + 1) * bs)) for c in cols])
+    keep = torch.ones(1, rows.numel(), keys.numel(), dtype=torch.bool)
+    keep[:, bs:, :bs] = False
+    pick = lambda t, i: t[:, :, i.to(t.device)].cpu()          # noqa: E731
+    args = (pick(q, rows), pick(k, keys), pick(v, keys), pick(dout, rows), keep, D ** -0.5, pick(out, rows), pick(lse, rows))
+    _, _, wq, wk, wv, sums = reference(*args)
+    check((pick(dq, rows), pick(dk, keys), pick(dv, keys)), (wq, wk, wv), sums, torch.bfloat16)
+    gone = torch.ones(N, dtype=torch.bool)
+    gone[rows] = False
+    assert (dq[:, :, gone.cuda()] == 0).all()
+    gone[:] = True
+    gone[keys] = False
+    assert (dk[:, :, gone.cuda()] == 0).all() and (dv[:, :, gone.cuda()] == 0).all()
