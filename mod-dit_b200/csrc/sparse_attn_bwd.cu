@@ -9,18 +9,25 @@
 //   query item  one tile of 128 queries, walks its key tiles: three products per tile
 //               S = Q K^T, dP = dO V^T, dQ += dS K
 // That is seven products where one pass over the pairs would need five; that pass would add every tile's 64 KB of float32 dQ
-// into memory with atomics (at 2,560 clocks of tensor pipe a tile about 25 bytes a clock and SM, and sums whose order varies).
+// into memory with atomics, in an order that varies, and at D = 128 has no tensor memory left for dQ.  Keeping dS for a product
+// of its own would take 32 KB per kept tile (12 GB for three heads of 115,456 tokens).
 //
-// Both kinds share one program: a block holds two fixed tiles (F0, F1 = K, V or Q, dO) and streams pairs of tiles
+// Both kinds work alike: a block holds two fixed tiles (F0, F1 = K, V or Q, dO) and streams blocks of 64 rows of two tensors
 // (X0, X1 = Q, dO or K, V):   S = F0 X0^T,  dP = F1 X1^T,  acc1 += P X1 (key items),  acc0 += dS X0.
 // P and dS stay in tensor memory, 16 bits wide, over the scores they came from, as the A operand of the second products;
 // X0 and X1 serve as K-major operands of the first products and as MN-major operands of the second from one copy in shared
-// memory.
-// Roles (20 warps): 0 TMA producer, 1 MMA issuer, 2 tensor-memory allocation, 3 the item's block list, 4-19 elementwise.
-// Tensor memory (512 columns): S [0,128) dP [128,256) acc0 [256,256+D) acc1 [384,384+D); P and dS overwrite columns
-// [64 h, 64 h + 32) of S and dP for column half h.
-// The issue order  acc1 += P(e) X1, S(e+1), acc0 += dS(e) X0, dP(e+1)  keeps the tensor pipe busy with the first two while
-// dS(e) is computed and with the other two while P(e+1) is.
+// memory.  A streamed block that neither half of the item's rows keeps is not fetched: at block size 64 a list of 128-row
+// tiles of which any quarter is kept would hold nearly twice the work (12 % of the blocks kept at random).
+// Roles: warp 0 TMA producer, 1 and 3 MMA issuers, 2 tensor-memory allocation, 3 first the item's block list, 4 and up
+// elementwise.
+//
+// Measured (B200; launch alone, clocks falling to 1.6 GHz at the power limit at D = 128): three heads of 115,456 tokens, block
+// 128, 15 % kept, D = 128 7.4 - 8.3 ms = 0.97 - 1.08 PFLOP/s on the five products of the kept pairs (58 - 65 % of the measured
+// burst rate, 1.35 - 1.5 PFLOP/s on the seven that run, about the rate a library product sustains); dense 24 x 4,096 543 us;
+// six heads of 45,104, block 64, D = 64 1.78 ms.  ncu, eight heads of 16,640 tokens at 25 %: tensor pipe 71 % at D = 128, 55 %
+// at D = 64, exponential unit 41 and 43 %.  What bounds it: at D = 128 power and the tensor pipe; at D = 64 the chain of waits
+// that a 64-column step is (scores, probabilities, dP, dS, products), of which tensor memory has room for three at a time.
+// From the first working version (one step at a time, 8 elementwise warps, 128-row tiles) 9.95 ms, 689 us and 4.36 ms.
 //
 // Sums are float32 in tensor memory; P and dS are rounded to the inputs' type once, for the second products.  P <= 1 falls
 // with the number of keys: for float16 it is held 2^8 times larger (its normal range then reaches 2^-22) and the factor is

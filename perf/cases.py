@@ -13,7 +13,7 @@ A case names a call (`kind`) and its sizes:
 
 The models are the three video transformers that `moddit_b200.synth.WORKLOADS` describes; query, key and value are its
 synthetic activations (positional locality, per-head mixture for wan), so masks have the density and the shape that the
-mask predictor finds on local attention.  Forward only: the framework has no backward pass.
+mask predictor finds on local attention.  Forward only; perf/operators.py has the backward pass.
 """
 import logging
 import math
