@@ -19,11 +19,14 @@ __all__ = ["sparse_attention", "qkv_prologue"]
 class _SparseAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lists, key_lists, limits, check_status):
-        if not any(ctx.needs_input_grad[:3]):
-            return ops.sparse_attn_fwd(q, k, v, lists.counts, lists.entries, order=lists.order, check_status=check_status,
-                                       **limits)
-        out, lse, residual = ops.sparse_attn_fwd(q, k, v, lists.counts, lists.entries, order=lists.order,
-                                                 return_residual=True, check_status=check_status, **limits)
+        wanted = any(ctx.needs_input_grad[:3])
+        res = ops.sparse_attn_fwd(q, k, v, lists.counts, lists.entries, order=lists.order, return_residual=wanted,
+                                  check_status=False if check_status == "deferred" else check_status, **limits)
+        if check_status == "deferred":
+            ops.post_status(q.device, spacing=ops.STATUS_SPACING)
+        if not wanted:
+            return res
+        out, lse, residual = res
         ctx.save_for_backward(q, k, v, out, lse, residual, lists.counts, lists.entries, lists.order, key_lists.counts,
                               key_lists.entries, key_lists.order)
         ctx.limits, ctx.check_status = limits, check_status
@@ -46,8 +49,9 @@ def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lists: o
     """Block-sparse attention of (B, H, N, D) float16 or bfloat16 tensors, differentiable with respect to q, k and v.
 
     lists, key_lists: `ops.tile_lists` and `ops.key_lists` of the layer's mask; the other arguments are those of
-    `ops.sparse_attn_fwd`.  Tensors that are not contiguous are copied.  What lies between the forward and the backward is
-    q, k, v, the output, what rounding took from it and 4 bytes per row."""
+    `ops.sparse_attn_fwd` ("deferred": status copies at most once a millisecond, see `ops.post_status`).  Tensors that are
+    not contiguous are copied.  What lies between the forward and the backward is q, k, v, the output, what rounding took from
+    it and 4 bytes per row."""
     limits = dict(softmax_scale=softmax_scale, q_split=q_split, kv_len_lo=kv_len_lo, kv_len_hi=kv_len_hi)
     return _SparseAttention.apply(q.contiguous(), k.contiguous(), v.contiguous(), lists, key_lists, limits, check_status)
 

@@ -923,6 +923,8 @@ def raise_on_status(device) -> None:
 
 
 _LAST_POST: Dict[int, float] = {}      # device index -> when `post_status` last queued a copy
+STATUS_SPACING = 1e-3                  # seconds between the copies that training calls queue: a copy and its change of engines
+                                       # hold up a stream of short launches by some ten microseconds
 
 
 def post_status(device, spacing: float = 0.0) -> None:
@@ -1103,6 +1105,5 @@ def sparse_attn_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
             D ** -0.5 if softmax_scale is None else softmax_scale, N if q_split is None else q_split,
             N if kv_len_lo is None else kv_len_lo, N if kv_len_hi is None else kv_len_hi, dq.data_ptr(), dk.data_ptr(),
             dv.data_ptr(), ws.data_ptr(), wsb, _status_words(dev).data_ptr(), _stream(dev)), "moddit_sparse_attn_bwd")
-    # the copy and its change of engines hold up a stream of short launches by some ten microseconds each
-    _after_launch(dev, check_status, spacing=1e-3)
+    _after_launch(dev, check_status, spacing=STATUS_SPACING)
     return dq, dk, dv
