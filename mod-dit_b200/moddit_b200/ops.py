@@ -1053,10 +1053,9 @@ def sparse_attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, counts: t
 # sparse backward
 # ---------------------------------------------------------------------------------------------
 
-def _need_lists(lists, rows: int, tiles: int, dev: torch.device, what: str) -> None:
-    Hm = lists.counts.shape[0]
+def _need_lists(lists, Hm: int, rows: int, tiles: int, dev: torch.device, what: str) -> None:
     for t, shape in ((lists.counts, (Hm, rows)), (lists.entries, (Hm, rows, tiles)), (lists.order, (Hm, rows))):
-        if t.dtype != torch.int32 or tuple(t.shape) != shape or t.device != dev or not t.is_contiguous():
+        if t.shape != shape or t.dtype != torch.int32 or t.device != dev or not t.is_contiguous():
             raise ValueError(f"the work lists do not match the sequence length and device (see {what})")
 
 
@@ -1088,12 +1087,11 @@ def sparse_attn_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
         _need_contig(residual=residual)
     if not isinstance(key_lists, KeyLists) or isinstance(lists, KeyLists):
         raise TypeError("lists must come from tile_lists and key_lists from key_lists")
-    nt = (N + 127) // 128
-    _need_lists(lists, (nt + 1) // 2, nt, dev, "tile_lists")
-    _need_lists(key_lists, nt, nt, dev, "key_lists")
-    Hm = lists.counts.shape[0]
+    nt, Hm = (N + 127) // 128, lists.counts.shape[0]
     if key_lists.counts.shape[0] != Hm:
         raise ValueError("tile_lists and key_lists must come from one mask")
+    _need_lists(lists, Hm, (nt + 1) // 2, nt, dev, "tile_lists")
+    _need_lists(key_lists, Hm, nt, nt, dev, "key_lists")
     dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
     wsb = lib.moddit_sparse_attn_bwd_workspace_bytes(B * H, N)
     ws = torch.empty(wsb, device=dev, dtype=torch.uint8)
