@@ -96,7 +96,7 @@ class _Prologue(torch.autograd.Function):
                     o.zero_()
         dx, params = ops.qkv_prologue_bwd(*grads, q_in, k_in, q_weight=q_weight, q_bias=q_bias,
                                           k_weight=k_weight, k_bias=k_bias, rope_cos=rope_cos, rope_sin=rope_sin,
-                                          n_tokens=ctx.tokens, out=out, **ctx.opts)
+                                          n_tokens=ctx.tokens, out=out, param_grads=any(needs[4:8]), **ctx.opts)
         dx = (None, None, None) if ctx.fused else dx
         return (whole, *dx, params["q_weight"], params["q_bias"], params["k_weight"], params["k_bias"], None, None, None)
 

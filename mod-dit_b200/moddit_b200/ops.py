@@ -150,8 +150,10 @@ def _ptr(t: Optional[torch.Tensor]):
     return ctypes.c_void_p(0 if t is None else t.data_ptr())
 
 
-def _stream(device: torch.device):
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+def _stream(device: torch.device) -> int:
+    # the handle itself: building a torch.cuda.Stream for it costs 2 us a call
+    index = device.index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
 def _need_cuda(*tensors: torch.Tensor) -> torch.device:
@@ -304,7 +306,7 @@ def qkv_prologue_bwd(dq: Optional[torch.Tensor], dk: Optional[torch.Tensor], dv:
                      k_bias: Optional[torch.Tensor] = None, eps: float = 1e-6, rope_cos: Optional[torch.Tensor] = None,
                      rope_sin: Optional[torch.Tensor] = None, rope_form: str = "elementwise",
                      rope_range: Optional[Tuple[int, int]] = None, src_row0: int = 0, n_tokens: Optional[int] = None,
-                     out: Optional[Tuple[Optional[torch.Tensor], ...]] = None):
+                     out: Optional[Tuple[Optional[torch.Tensor], ...]] = None, param_grads: bool = True):
     """Gradients of `qkv_prologue` (`moddit_qkv_prologue_bwd`).
 
     dq/dk/dv: (B, H, N, D) gradients of its outputs, any may be None; the tokens of this call are rows src_row0 to
@@ -312,33 +314,50 @@ def qkv_prologue_bwd(dq: Optional[torch.Tensor], dk: Optional[torch.Tensor], dv:
     forward's; q_in/k_in are needed where there is a norm.  S is that of q_in/k_in, else `n_tokens`, else the rest of the rows.
     `out`: buffers for the gradients of q_in, k_in and v_in (B, S, H*D), slices of one fused gradient included.
     Returns ((dq_in, dk_in, dv_in), {"q_weight", "q_bias", "k_weight", "k_bias"}): gradients of the parameters given
-    (each in its own dtype), None for the others."""
+    (each in its own dtype), None for the others and with `param_grads=False` (parameters that are not trained: nothing is
+    summed for them)."""
     grads = (dq, dk, dv)
     given = [t for t in grads if t is not None]
     if not given:
         raise ValueError("qkv_prologue_bwd: no gradient")
     dev = _need_cuda(*given)
     ref = given[0]
-    if ref.dim() != 4 or ref.shape[1] != num_heads:
+    shape, dtype = ref.shape, ref.dtype
+    if len(shape) != 4 or shape[1] != num_heads:
         raise ValueError(f"gradients must be (B, {num_heads}, N, D) tensors")
-    B, H, N, D = ref.shape
+    B, H, N, D = shape
     dt = _qkv_dtype(ref)
     for t in given:
-        if t.shape != ref.shape or t.dtype != ref.dtype or not t.is_contiguous():
+        if t.shape != shape or t.dtype != dtype or not t.is_contiguous():
             raise ValueError("dq, dk and dv must be contiguous tensors of one shape and dtype")
     kind = _lib.NORM_KIND[norm]
-    inputs = [x if kind and g is not None else None for x, g in ((q_in, dq), (k_in, dk))]
-    if kind and any(x is None and g is not None for x, g in zip(inputs, grads)):
-        raise ValueError("the gradient of a norm needs its input (q_in, k_in)")
-    present = [x for x in inputs if x is not None]
     if n_tokens is None:
         n_tokens = next((x.shape[1] for x in (q_in, k_in) if x is not None), N - src_row0)
     S = int(n_tokens)
-    stride = _token_stride(present, (B, S, H * D), ref.dtype, dev, "inputs")
-    width = H * D if norm == "rms_all_heads" else D
-    for name, p in (("q_weight", q_weight), ("q_bias", q_bias), ("k_weight", k_weight), ("k_bias", k_bias)):
-        if kind and p is not None and (p.dtype != ref.dtype or not p.is_contiguous() or p.device != dev or p.numel() != width):
-            raise ValueError(f"{name} must be a contiguous {ref.dtype} tensor of {width} values on {dev}")
+    tokens = (B, S, H * D)
+    inputs, stride = [None, None], H * D
+    if kind:
+        for i, (x, g) in enumerate(((q_in, dq), (k_in, dk))):
+            if g is not None:
+                if x is None:
+                    raise ValueError("the gradient of a norm needs its input (q_in, k_in)")
+                inputs[i] = x
+        stride = _token_stride([x for x in inputs if x is not None], tokens, dtype, dev, "inputs")
+    res = {"q_weight": None, "q_bias": None, "k_weight": None, "k_bias": None}
+    wsb, ws = 0, None
+    if kind:
+        width = H * D if norm == "rms_all_heads" else D
+        for name, p, g in (("q_weight", q_weight, dq), ("q_bias", q_bias, dq), ("k_weight", k_weight, dk), ("k_bias", k_bias, dk)):
+            if p is None:
+                continue
+            if p.dtype != dtype or not p.is_contiguous() or p.device != dev or p.numel() != width:
+                raise ValueError(f"{name} must be a contiguous {dtype} tensor of {width} values on {dev}")
+            if param_grads and g is not None and (norm == "layer" or name.endswith("weight")):
+                res[name] = torch.empty_like(p)
+                wsb = 1
+        if wsb:
+            wsb = lib.moddit_qkv_prologue_bwd_workspace_bytes(B, S, H, D, kind)
+            ws = torch.empty(wsb, device=dev, dtype=torch.uint8)
     if (rope_cos is None) != (rope_sin is None):
         raise ValueError("rope_cos and rope_sin go together")
     lo, hi = (0, S) if rope_range is None else rope_range
@@ -347,29 +366,23 @@ def qkv_prologue_bwd(dq: Optional[torch.Tensor], dk: Optional[torch.Tensor], dv:
         for t in (rope_cos, rope_sin):
             if t.dtype != torch.float32 or not t.is_contiguous() or t.shape != (hi - lo, cols) or t.device != dev:
                 raise ValueError(f"rotary tables must be contiguous float32 ({hi - lo}, {cols}) tensors on {dev}")
+    out_stride = H * D
     if out is None:
-        out = tuple(None if g is None else torch.empty(B, S, H * D, device=dev, dtype=ref.dtype) for g in grads)
-    stores = [o for o, g in zip(out, grads) if g is not None]
-    if any(o is None for o in stores):
-        raise ValueError("every gradient given needs an output buffer")
-    out_stride = _token_stride(stores, (B, S, H * D), ref.dtype, dev, "output buffers")
-    res = {"q_weight": None, "q_bias": None, "k_weight": None, "k_bias": None}
-    for name, p, g in (("q_weight", q_weight, dq), ("k_weight", k_weight, dk), ("q_bias", q_bias, dq), ("k_bias", k_bias, dk)):
-        if p is not None and g is not None and kind and (norm == "layer" or name.endswith("weight")):
-            res[name] = torch.empty_like(p)
-    ws = None
-    wsb = 0
-    if any(r is not None for r in res.values()):
-        wsb = lib.moddit_qkv_prologue_bwd_workspace_bytes(B, S, H, D, kind)
-        ws = torch.empty(wsb, device=dev, dtype=torch.uint8)
-    with _entry("moddit_qkv_prologue_bwd" + ("" if wsb else " (no parameters)"), dev):
+        out = tuple([None if g is None else torch.empty(tokens, device=dev, dtype=dtype) for g in grads])
+    else:
+        out = tuple(out)
+        stores = [o for o, g in zip(out, grads) if g is not None]
+        if len(out) != 3 or any(o is None for o in stores):
+            raise ValueError("every gradient given needs an output buffer")
+        out_stride = _token_stride(stores, tokens, dtype, dev, "output buffers")
+    to = [None if g is None else o.data_ptr() for o, g in zip(out, grads)]
+    with _entry("moddit_qkv_prologue_bwd" if wsb else "moddit_qkv_prologue_bwd (no parameters)", dev):
         check(lib.moddit_qkv_prologue_bwd(
             _addr(dq), _addr(dk), _addr(dv), _addr(inputs[0]), _addr(inputs[1]), dt, B, S, H, D, stride, kind, _addr(q_weight),
             _addr(k_weight), eps, _addr(rope_cos), _addr(rope_sin), _lib.ROPE_FORM[rope_form], lo, hi, N, src_row0,
-            _addr(out[0]) if dq is not None else None, _addr(out[1]) if dk is not None else None,
-            _addr(out[2]) if dv is not None else None, out_stride, _addr(res["q_weight"]), _addr(res["q_bias"]),
+            to[0], to[1], to[2], out_stride, _addr(res["q_weight"]), _addr(res["q_bias"]),
             _addr(res["k_weight"]), _addr(res["k_bias"]), _addr(ws), wsb, _stream(dev)), "moddit_qkv_prologue_bwd")
-    return tuple(out), res
+    return out, res
 
 
 def pooled_map(qbar: torch.Tensor, kbar: torch.Tensor, *, q_block_offset: int, k_block_offset: int,

@@ -287,3 +287,25 @@ def test_masked_places_hold_anything(mods):
     zero = ops.sparse_attn_bwd(dout, q, k, v, torch.zeros_like(out), torch.full_like(lse, -math.inf), lists, klists,
                                kv_len_lo=0, kv_len_hi=0)
     assert all((t == 0).all() for t in zero)
+
+
+@pytest.mark.parametrize("norm", ["rms_head", "rms_all_heads", "layer"])
+def test_frozen_norm_parameters(mods, norm):
+    """Parameters that are not trained get no gradient and change nothing about the inputs'."""
+    autograd, ops = mods
+    g = torch.Generator().manual_seed(31)
+    B, S, H, D = 2, 70, 3, 64
+    x = [torch.randn(B, S, H * D, generator=g).half().cuda().requires_grad_(True) for _ in range(3)]
+    width = H * D if norm == "rms_all_heads" else D
+    w = [torch.randn(width, generator=g).half().cuda().requires_grad_(True) for _ in range(2)]
+    dy = [torch.randn(B, H, S, D, generator=g).half().cuda() for _ in range(3)]
+
+    def step(weights):
+        return autograd.qkv_prologue(*x, num_heads=H, norm=norm, q_weight=weights[0], k_weight=weights[1])
+
+    want = torch.autograd.grad(step(w), x, dy)
+    got = torch.autograd.grad(step([t.detach() for t in w]), x, dy)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    dx, params = ops.qkv_prologue_bwd(*dy, x[0].detach(), x[1].detach(), num_heads=H, norm=norm, q_weight=w[0].detach(),
+                                      k_weight=w[1].detach(), param_grads=False)
+    assert all(torch.equal(a, b) for a, b in zip(dx, want)) and all(p is None for p in params.values())
