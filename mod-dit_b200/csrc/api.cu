@@ -52,7 +52,8 @@ int sm_count(int* sms) {
 }
 
 int ensure_dynamic_smem(const void* kernel, size_t bytes) {
-  if (bytes <= 48 * 1024) return MODDIT_OK;          // available without opting in
+  // A block has 48 KB without opting in, its kernel's static arrays among them; those are under 16 KB everywhere here.
+  if (bytes <= 32 * 1024) return MODDIT_OK;
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return fail(MODDIT_E_CUDA, "cudaGetDevice failed: %s", cudaGetErrorString(err));

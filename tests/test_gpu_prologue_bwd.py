@@ -99,6 +99,10 @@ CASES = [
     (1, 1000, 2, 128, None, "elementwise", 0, 1000, 0, False),
     (1, 50, 3, 64, None, None, 0, 0, 0, False),
     (1, 5000, 7, 64, "rms_head", "even_cos_odd_sin", 0, 4999, 0, False),
+    # wide tokens: their sums in shared memory and the kernel's own arrays pass 48 KB together, then each
+    (1, 19, 80, 128, "rms_all_heads", "pair", 0, 19, 0, False),
+    (1, 11, 192, 64, "rms_all_heads", "elementwise", 3, 9, 0, True),
+    (1, 10, 200, 128, "rms_all_heads", None, 0, 0, 0, False),
 ]
 
 
