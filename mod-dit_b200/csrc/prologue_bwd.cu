@@ -27,6 +27,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kRows = 2;                // rows per thread of an item of the per-head kernel
 constexpr int kStages = 5;              // heads of them in flight
+constexpr int kWide = 640;              // threads of the kernel with a piece of a whole token each
 
 template <typename T>
 struct Pair;
@@ -299,7 +300,8 @@ __global__ void __launch_bounds__(kThreads, 2) prologue_bwd_kernel(const __grid_
 // (from the L2), writes dx and adds to its columns' weight gradient, which lives in shared memory.  A piece lies at the same
 // columns of its head for all pieces of a lane or thread, so the rotary factors are read once a token: in the second part from
 // shared memory, where the first part's lanes have put them.
-// 8,640 tokens of 40 x 128: 179 us, 61 % of the measured copy bandwidth; bound by instructions and the two parts' latencies.
+// For tokens too wide for the kernel below.  8,640 tokens of 40 x 128: 172 us, 63 % of the measured copy bandwidth; bound by
+// instructions and the two parts' latencies.
 // Slower: a group's rows kept in shared memory between the parts, copied a group ahead (204 us with two blocks an SM, 257 with
 // one: block-wide sums and fewer warps), half as many tokens in flight with three or four blocks an SM (190 - 230).
 template <typename T, int D, bool kPair>
@@ -434,6 +436,206 @@ __global__ void __launch_bounds__(kThreads, 2) prologue_bwd_all_heads_kernel(con
   }
 }
 
+// The same for tokens of up to kWide pieces, in one pass over the rows: a thread has one piece of eight columns of every token of
+// its block, kept from the sums to dx in registers, with its columns' weights and weight gradient.  Two tokens at a time share
+// one block-wide sum of four values and one barrier.  The rows of the next kStages - 1 pairs of tokens are on their way into
+// places of the thread's own in shared memory, as in the per-head kernel, and with them the two tokens' rows of the rotary
+// tables, once a block.  Where q, k and v are all given, a block of q or k also copies one token of v per pair of its own:
+// copies want bytes, the sums want instructions.
+// 8,640 tokens of 40 x 128: 130 us, 5.5 TB/s, 83 % of the measured copy bandwidth; 260 instructions a piece, issued in 0.65 of
+// the cycles, are the other bound.  On the way: divisions and products for every pair's addresses, rotary rows loaded per thread
+// 170 us; those loaded a pair ahead 158 (spills where a table has a value a column); pointers moved on by additions 154; rotary
+// rows through shared memory 145; v beside q and k 137; q and k at once, half of the blocks each, 130.  Slower: two operations
+// an instruction on packed pairs (more registers: spills, 194 us against 158).
+template <typename T, int D, bool kPair>
+__global__ void __launch_bounds__(kWide, 1) prologue_bwd_tokens_kernel(const __grid_constant__ BwdArgs a) {
+  constexpr int kTpr = D / 8;
+  constexpr int kRow = kPair ? D / 2 : D;         // floats of a row of the rotary tables
+  constexpr int kChunks = 4 * kRow / 4;           // pieces of 16 bytes of two tokens' rows of both
+  extern __shared__ uint4 ring[];                 // [kStages][2][g, x][threads], then [kStages][2][cos, sin][kRow] floats
+  __shared__ float red[2][4][kWide / 32];         // [round & 1][x^2, g w x of the first token, of the second][warp]
+  const int which = blockIdx.y, threads = blockDim.x;
+  const T* __restrict__ g_in = static_cast<const T*>(a.g[which]);
+  const bool beside = a.g[0] && a.g[1] && a.g[2];   // the blocks of q and k copy a token of v each along with a pair of theirs
+  if (g_in == nullptr || (beside && which == 2)) return;
+  const bool normed = which < 2, turned = which < 2 && a.cos != nullptr;
+  const T* __restrict__ x_in = normed ? static_cast<const T*>(a.x[which]) : nullptr;
+  T* __restrict__ dx = static_cast<T*>(a.dx[which]);
+  const int W = a.H * D;
+  const bool has = threadIdx.x < W / 8;
+  const int p = has ? threadIdx.x : 0, c = p % kTpr;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = threads / 32;
+  const float inv_w = 1.f / static_cast<float>(W);
+  float w[8], dw[8] = {};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = 1.f;
+  if (normed && has && a.weight[which] != nullptr) unpack<T>(__ldg(static_cast<const uint4*>(a.weight[which]) + p), w);
+
+  // A block has every gridDim.x-th pair of tokens.  The pointers to where it reads (`ahead`) and writes (`at`) are moved on by
+  // additions, and made anew where the sample changes.
+  const int even = (a.S + 1) / 2 * 2, step = 2 * gridDim.x;
+  struct Place {
+    int b, s;
+    __device__ bool next(int step, int S) {       // true where the sample has changed
+      s += step;
+      if (s < S) return false;
+      do s -= S, ++b;
+      while (s >= S);
+      return true;
+    }
+  };
+  Place at{0, 0};
+  at.next(2 * blockIdx.x, even);
+  Place ahead = at;
+  const int64_t head = static_cast<int64_t>(p / kTpr) * a.N_out + a.src_row0;
+  const int64_t x_step = step * a.token_stride, d_step = step * a.out_stride;
+  auto g_at = [&](const Place& of) { return g_in + (static_cast<int64_t>(of.b) * a.H * a.N_out + head + of.s) * D + c * 8; };
+  auto x_at = [&](const Place& of) { return x_in + (static_cast<int64_t>(of.b) * a.S + of.s) * a.token_stride + p * 8; };
+  auto d_at = [&](const Place& of) { return dx + (static_cast<int64_t>(of.b) * a.S + of.s) * a.out_stride + p * 8; };
+  const T *gp = g_at(ahead), *xp = x_at(ahead);
+  T* dp = d_at(at);
+  const uint32_t mine = static_cast<uint32_t>(__cvta_generic_to_shared(ring + threadIdx.x)), apart = 16 * threads;
+  auto copy = [&](uint32_t to, const void* from, bool in) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(__cvta_generic_to_global(from)), "r"(in ? 16 : 0)
+                 : "memory");
+  };
+  const uint4* const tables = ring + kStages * 4 * threads;
+  const uint32_t tables_at = static_cast<uint32_t>(__cvta_generic_to_shared(tables));
+  auto turned_at = [&](int s) { return turned && s >= a.rope_lo && s < a.rope_hi; };
+  auto fetch = [&](int stage) {
+    if (ahead.b < a.B) {
+      if (turned)
+        for (int i = threadIdx.x; i < kChunks; i += threads) {
+          const int s = ahead.s + i / (kChunks / 2), piece = i % (kRow / 4);
+          const float* from = i / (kRow / 4) % 2 ? a.sin : a.cos;
+          const bool in = turned_at(s);
+          copy(tables_at + 16 * (stage * kChunks + i), in ? from + static_cast<int64_t>(s - a.rope_lo) * kRow + 4 * piece : from, in);
+        }
+      const uint32_t to = mine + stage * 4 * apart;
+      const bool two = ahead.s + 1 < a.S;
+      copy(to, gp, has);
+      copy(to + 2 * apart, two ? gp + D : gp, two && has);
+      if (normed) {
+        copy(to + apart, xp, has);
+        copy(to + 3 * apart, two ? xp + a.token_stride : xp, two && has);
+      }
+      if (ahead.next(step, even)) {
+        gp = g_at(ahead);
+        xp = x_at(ahead);
+      } else {
+        gp += step * D;
+        xp += x_step;
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  for (int j = 0; j < kStages - 1; ++j) fetch(j);
+  int stage = 0, round = 0;
+  auto turn_at = [&](int stage, int t) {
+    const float4* row = reinterpret_cast<const float4*>(tables + stage * kChunks + t * (kChunks / 2));
+    Turn f;
+    if constexpr (kPair) {
+      const float4 cs = row[c], sn = row[kRow / 4 + c];
+      const float cv[4] = {cs.x, cs.y, cs.z, cs.w}, sv[4] = {sn.x, sn.y, sn.z, sn.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f.cs[2 * i] = f.cs[2 * i + 1] = cv[i];
+        f.sn[2 * i] = f.sn[2 * i + 1] = sv[i];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        *reinterpret_cast<float4*>(f.cs + 4 * i) = row[2 * c + i];
+        *reinterpret_cast<float4*>(f.sn + 4 * i) = row[kRow / 4 + 2 * c + i];
+      }
+      if (a.rope_form == MODDIT_ROPE_EVEN_COS_ODD_SIN) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          f.cs[2 * i + 1] = f.cs[2 * i];
+          f.sn[2 * i] = f.sn[2 * i + 1];
+        }
+      }
+    }
+    return f;
+  };
+  // The tables' rows are copied by one thread and read by others: a round waits for the next round's copies before its barrier.
+  asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+  __syncthreads();
+  for (; at.b < a.B; round ^= 1) {
+    const int s0 = at.s;
+    T* const to = dp;
+    const bool copies = beside && has && s0 + which < a.S;
+    uint4 copied;
+    int64_t vrow = 0;
+    if (copies) {
+      copied = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.g[2]) + (static_cast<int64_t>(at.b) * a.H * a.N_out + head + s0 + which) * D + c * 8));
+      vrow = static_cast<int64_t>(at.b) * a.S + s0 + which;
+    }
+    if (at.next(step, even)) dp = d_at(at);
+    else dp += d_step;
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 3) : "memory");
+    const uint4* from = ring + stage * 4 * threads + threadIdx.x;
+    uint4 gv[2], xv[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      gv[t] = from[2 * t * threads];
+      if (normed) xv[t] = from[(2 * t + 1) * threads];
+    }
+    const int now = stage;
+    fetch(stage == 0 ? kStages - 1 : stage - 1);
+    stage = stage == kStages - 1 ? 0 : stage + 1;
+    if (normed) {
+      float g[2][8], sum[4] = {};
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        float x[8];
+        unpack<T>(gv[t], g[t]);
+        unpack<T>(xv[t], x);
+        if (turned_at(s0 + t)) turn_back(turn_at(now, t), g[t]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          sum[2 * t] = fmaf(x[i], x[i], sum[2 * t]);
+          sum[2 * t + 1] = fmaf(g[t][i] * w[i], x[i], sum[2 * t + 1]);
+        }
+      }
+      // four sums over the warp in six exchanges: eight lanes end with each of them
+      const bool up = lane & 16, odd = lane & 8;
+      const float s = (up ? sum[2] : sum[0]) + __shfl_xor_sync(0xffffffffu, up ? sum[0] : sum[2], 16);
+      const float d = (up ? sum[3] : sum[1]) + __shfl_xor_sync(0xffffffffu, up ? sum[1] : sum[3], 16);
+      const float part = lane_sum<8>((odd ? d : s) + __shfl_xor_sync(0xffffffffu, odd ? s : d, 8));
+      if (lane % 8 == 0) red[round][lane / 8][warp] = part;
+      __syncthreads();
+      float all = 0.f;
+      for (int j = lane % 8; j < warps; j += 8) all += red[round][lane / 8][j];
+      all = lane_sum<8>(all);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const float ss = __shfl_sync(0xffffffffu, all, 16 * t), sg = __shfl_sync(0xffffffffu, all, 16 * t + 8);
+        const float r = s0 + t < a.S ? rsqrtf(ss * inv_w + a.eps) : 0.f;     // a token past the end adds nothing, eps = 0 included
+        const float f = -r * r * (sg * inv_w);
+        float x[8];
+        unpack<T>(xv[t], x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float xr = x[i] * r;
+          dw[i] = fmaf(g[t][i], xr, dw[i]);
+          g[t][i] = fmaf(xr, f, r * (g[t][i] * w[i]));
+        }
+        gv[t] = pack8<T>(g[t]);
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+      if (has && s0 + t < a.S) *reinterpret_cast<uint4*>(to + t * a.out_stride) = gv[t];
+    if (copies) *reinterpret_cast<uint4*>(static_cast<T*>(a.dx[2]) + vrow * a.out_stride + p * 8) = copied;
+  }
+  if (normed && has && a.part[which] != nullptr) {
+    float4* to = reinterpret_cast<float4*>(a.part[which] + static_cast<int64_t>(blockIdx.x) * W + p * 8);
+    to[0] = make_float4(dw[0], dw[1], dw[2], dw[3]);
+    to[1] = make_float4(dw[4], dw[5], dw[6], dw[7]);
+  }
+}
+
 // Adds the rows of partial sums in index order: 32 columns a block, eight groups of rows.  y = tensor, z = weight, bias.
 struct SumArgs {
   const float* part[2];
@@ -463,13 +665,26 @@ __global__ void __launch_bounds__(kThreads) prologue_bwd_sums_kernel(const __gri
 // that many.
 constexpr int kBlocksPerHead = 296;
 constexpr int kBlocksAllHeads = 296;
+constexpr int kBlocksTokens = 148;                   // q's and k's half of them each where both are given
 constexpr int kMaxWidth = 48 * 1024;                 // values of a token: their sums lie in shared memory
 int heads_per_item(int B, int S, int H, int D) {
   const int64_t tiles = static_cast<int64_t>(B) * ceil_div(S, kRows * kThreads / (D / 8));
   const int chunks = static_cast<int>(std::min<int64_t>(H, (kBlocksPerHead + tiles - 1) / tiles));
   return ceil_div(H, chunks);
 }
-int blocks_for(int B, int S, int H, int D, int norm_kind) {
+// Tokens of up to kWide pieces are read once (a thread a piece), wider ones twice.  8,640 tokens of 40 x 128: 130 us once, 172
+// twice; 32,760 of 12 x 128: 148 and 235; 40,000 of 16 x 64: 128 and 233; 1,000 of 12 x 128 alike.
+bool one_pass(int H, int D) { return H <= kWide * 8 / D; }
+int token_threads(int H, int D) { return ceil_div(H * D / 8, 32) * 32; }
+constexpr size_t token_smem(int threads, int floats) { return sizeof(uint4) * kStages * (4 * threads + floats); }
+// as many blocks an SM as its registers and 227 KB of shared memory hold
+int token_blocks(int threads) {
+  return std::max(1, std::min(kWide / threads, static_cast<int>(226 * 1024 / (token_smem(threads, 128) + 2048))));
+}
+int blocks_for(int B, int S, int H, int D, int norm_kind, int tensors = 1) {
+  if (norm_kind == MODDIT_NORM_RMS_ALL_HEADS && one_pass(H, D))
+    return static_cast<int>(std::min<int64_t>(kBlocksTokens * token_blocks(token_threads(H, D)) / tensors,
+                                              static_cast<int64_t>(B) * ceil_div(S, 2)));
   if (norm_kind == MODDIT_NORM_RMS_ALL_HEADS)
     return static_cast<int>(std::min<int64_t>(kBlocksAllHeads, static_cast<int64_t>(B) * ceil_div(S, kThreads / 32)));
   return static_cast<int>(std::min<int64_t>(kBlocksPerHead, static_cast<int64_t>(B) * ceil_div(S, kRows * kThreads / (D / 8)) *
@@ -478,7 +693,13 @@ int blocks_for(int B, int S, int H, int D, int norm_kind) {
 
 template <typename T, int D, bool kPair>
 int launch_rows(const BwdArgs& a, int norm_kind, int blocks, cudaStream_t st) {
-  if (norm_kind == MODDIT_NORM_RMS_ALL_HEADS) {
+  if (norm_kind == MODDIT_NORM_RMS_ALL_HEADS && one_pass(a.H, D)) {
+    auto kernel = prologue_bwd_tokens_kernel<T, D, kPair>;
+    const int threads = token_threads(a.H, D);
+    const size_t smem = token_smem(threads, a.cos == nullptr ? 0 : kPair ? D / 2 : D);
+    if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem)) return rc;
+    kernel<<<dim3(blocks, 3), threads, smem, st>>>(a);
+  } else if (norm_kind == MODDIT_NORM_RMS_ALL_HEADS) {
     auto kernel = prologue_bwd_all_heads_kernel<T, D, kPair>;
     const size_t smem = sizeof(float) * a.H * D;
     if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem)) return rc;
@@ -577,7 +798,7 @@ extern "C" int moddit_qkv_prologue_bwd(const void* dq, const void* dk, const voi
                 moddit_qkv_prologue_bwd_workspace_bytes(B, S, H, D, norm_kind));
   if (int rc = require_sm100()) return rc;
 
-  const int blocks = blocks_for(B, S, H, D, norm_kind);
+  const int blocks = blocks_for(B, S, H, D, norm_kind, dq != nullptr && dk != nullptr ? 2 : 1);
   const int64_t per = static_cast<int64_t>(blocks) * (norm_kind == MODDIT_NORM_RMS_ALL_HEADS ? width : 2 * D);
   BwdArgs a{};
   SumArgs sums{};

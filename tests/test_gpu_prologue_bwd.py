@@ -103,6 +103,13 @@ CASES = [
     (1, 19, 80, 128, "rms_all_heads", "pair", 0, 19, 0, False),
     (1, 11, 192, 64, "rms_all_heads", "elementwise", 3, 9, 0, True),
     (1, 10, 200, 128, "rms_all_heads", None, 0, 0, 0, False),
+    # a token of eight pieces; the widest that is read once, an odd number of tokens and a rotated part; one wider
+    (3, 7, 1, 64, "rms_all_heads", "pair", 2, 6, 1, True),
+    (2, 331, 40, 128, "rms_all_heads", "elementwise", 5, 300, 0, False),
+    (2, 45, 41, 128, "rms_all_heads", "pair", 0, 45, 2, False),
+    # more pairs of tokens than blocks, a sample per round of them and several
+    (5, 1201, 9, 64, "rms_all_heads", "even_cos_odd_sin", 1, 1200, 3, False),
+    (300, 3, 2, 128, "rms_all_heads", "pair", 0, 3, 0, True),
 ]
 
 
@@ -164,3 +171,21 @@ def test_missing_parts(ops):
     both, _ = ops.qkv_prologue_bwd(dk, dk, dk, k, k, num_heads=2, norm="rms_head", k_weight=torch.ones(64, device="cuda", dtype=torch.bfloat16))
     assert torch.equal(both[1], dk_in) and torch.equal(both[0], dk_in)
     assert torch.equal(both[2], dk.transpose(1, 2).reshape(1, 40, 128))
+
+
+@pytest.mark.parametrize("H", [5, 41])
+def test_a_token_norm_of_some_tensors(ops, H):
+    """q, k and v share blocks where all are given: any of them alone gives the same bits of its gradient."""
+    g = torch.Generator().manual_seed(H)
+    B, S, D = 2, 51, 128
+    dy = [torch.randn(B, H, S, D, generator=g).half().cuda() for _ in range(3)]
+    x = [torch.randn(B, S, H * D, generator=g).half().cuda() for _ in range(2)]
+    w = [torch.randn(H * D, generator=g).half().cuda() for _ in range(2)]
+    kw = dict(num_heads=H, norm="rms_all_heads", q_weight=w[0], k_weight=w[1])
+    want, _ = ops.qkv_prologue_bwd(*dy, *x, **kw)
+    for keep in ((0,), (1,), (2,), (0, 1), (0, 2), (1, 2)):
+        some = [t if i in keep else None for i, t in enumerate(dy)]
+        got, params = ops.qkv_prologue_bwd(*some, *x, n_tokens=S, **kw)
+        for i in range(3):
+            assert got[i] is None if i not in keep else torch.equal(got[i], want[i])
+        assert (params["q_weight"] is None) == (0 not in keep) and (params["k_weight"] is None) == (1 not in keep)
