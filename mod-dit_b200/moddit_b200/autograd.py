@@ -20,6 +20,8 @@ class _SparseAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lists, key_lists, limits, check_status):
         wanted = any(ctx.needs_input_grad[:3])
+        if check_status == "deferred" and not torch.cuda.is_current_stream_capturing():
+            ops.check_posted_status(q.device)
         res = ops.sparse_attn_fwd(q, k, v, lists.counts, lists.entries, order=lists.order, return_residual=wanted,
                                   check_status=False if check_status == "deferred" else check_status, **limits)
         if check_status == "deferred":
@@ -49,8 +51,8 @@ def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lists: o
     """Block-sparse attention of (B, H, N, D) float16 or bfloat16 tensors, differentiable with respect to q, k and v.
 
     lists, key_lists: `ops.tile_lists` and `ops.key_lists` of the layer's mask; the other arguments are those of
-    `ops.sparse_attn_fwd` ("deferred": status copies at most once a millisecond, see `ops.post_status`).  Tensors that are
-    not contiguous are copied.  What lies between the forward and the backward is q, k, v, the output, what rounding took from
+    `ops.sparse_attn_fwd` ("deferred": a call raises for a kernel of an earlier step that gave up a wait, once the copy of its status
+    has arrived; copies are queued at most every `ops.STATUS_SPACING` seconds).  Tensors that are not contiguous are copied.  What lies between the forward and the backward is q, k, v, the output, what rounding took from
     it and 4 bytes per row."""
     limits = dict(softmax_scale=softmax_scale, q_split=q_split, kv_len_lo=kv_len_lo, kv_len_hi=kv_len_hi)
     return _SparseAttention.apply(q.contiguous(), k.contiguous(), v.contiguous(), lists, key_lists, limits, check_status)

@@ -309,3 +309,21 @@ def test_frozen_norm_parameters(mods, norm):
     dx, params = ops.qkv_prologue_bwd(*dy, x[0].detach(), x[1].detach(), num_heads=H, norm=norm, q_weight=w[0].detach(),
                                       k_weight=w[1].detach(), param_grads=False)
     assert all(torch.equal(a, b) for a, b in zip(dx, want)) and all(p is None for p in params.values())
+
+
+def test_a_later_step_reports_a_kernel_that_gave_up(mods):
+    """The status words of an earlier kernel, set here by hand, end a later step once their copy has arrived."""
+    autograd, ops = mods
+    q, k, v, dout, _, lists, klists = layer(mods, 40)
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    want = torch.autograd.grad(autograd.sparse_attention(*leaves, lists, klists), leaves, dout)
+    torch.cuda.synchronize()
+    ops.check_posted_status(q.device)
+    ops._status_words(q.device).copy_(torch.tensor([3, 1, 2, 0], dtype=torch.int32))
+    ops.post_status(q.device)
+    torch.cuda.synchronize()
+    with pytest.raises(Exception, match="bounded wait expired"):
+        autograd.sparse_attention(*leaves, lists, klists)
+    got = torch.autograd.grad(autograd.sparse_attention(*leaves, lists, klists), leaves, dout)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    ops.check_health(q.device)
