@@ -936,7 +936,7 @@ def raise_on_status(device) -> None:
 
 
 _LAST_POST: Dict[int, float] = {}      # device index -> when `post_status` last queued a copy
-STATUS_SPACING = 1e-3                  # seconds between the copies that training calls queue: a copy and its change of engines
+STATUS_SPACING = 1e-2                  # seconds between the copies that training calls queue: a copy and its change of engines
                                        # hold up a stream of short launches by some ten microseconds
 
 
@@ -1043,7 +1043,7 @@ def sparse_attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, counts: t
     args = (_ptr(q), _ptr(k), _ptr(v), _qkv_dtype(q), B * H, N, D, _ptr(counts), _ptr(entries), _ptr(order), Hm, scale,
             N if q_split is None else int(q_split), N if kv_len_lo is None else int(kv_len_lo),
             N if kv_len_hi is None else int(kv_len_hi))
-    with torch.cuda.device(dev), _timed("moddit_sparse_attn_fwd", dev):
+    with _entry("moddit_sparse_attn_fwd", dev):
         if pairs_beside:
             check(lib.moddit_sparse_attn_fwd_beside(*args, int(pairs_beside), _ptr(out), table, n_peers, int(head_base),
                                                     _ptr(lse), _ptr(st), _stream(dev)), "moddit_sparse_attn_fwd_beside")
