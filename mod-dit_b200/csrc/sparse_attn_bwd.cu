@@ -906,6 +906,7 @@ __global__ void __launch_bounds__(kThreads<D>, 1) sparse_attn_bwd_kernel(
   }
   __syncthreads();
   ptx::tc_fence_after();
+  asm volatile("griddepcontrol.wait;" ::: "memory");      // for the row statistics
   b.tmem = ctl->tmem_base;
   b.count = ctl->count;
 
@@ -938,6 +939,7 @@ template <int D, bool kBF16>
 __global__ void __launch_bounds__(256) bwd_stats_kernel(const void* __restrict__ out, const void* __restrict__ lo,
                                                         const void* __restrict__ dout, const float* __restrict__ lse, int N, int npad,
                                                         float* __restrict__ nlse, float* __restrict__ ndelta) {
+  asm volatile("griddepcontrol.launch_dependents;");      // the items may set themselves up meanwhile
   constexpr int kTpr = D / 8;
   const int bh = blockIdx.y;
   const int row = blockIdx.x * (256 / kTpr) + threadIdx.x / kTpr;
@@ -987,8 +989,19 @@ int launch(BwdArgs a, const void* out, const void* lo, const float* lse, int dty
                                                                                   ws + static_cast<int64_t>(BH) * a.npad);
   MODDIT_CHECK_LAUNCH("bwd_stats_kernel");
   const int64_t blocks = static_cast<int64_t>(2 * a.ntiles + (a.ntiles & 1)) * BH;
-  kernel<<<static_cast<unsigned>(blocks), kThreads<D>, smem, st>>>(tq, tk, tv, tdo, a);
-  MODDIT_CHECK_LAUNCH("sparse_attn_bwd_kernel");
+  // Launched beside the statistics: barriers, tensor memory and block lists are ready when these are.  2 heads of 4,096 at D = 128
+  // 59.3 -> 57.6 us, 1,200 rows 23.9 -> 22.9; the next launch of the stream still waits for all of it.
+  cudaLaunchAttribute beside{};
+  beside.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  beside.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned>(blocks));
+  config.blockDim = dim3(kThreads<D>);
+  config.dynamicSmemBytes = smem;
+  config.stream = st;
+  config.attrs = &beside;
+  config.numAttrs = 1;
+  MODDIT_CHECK_CUDA(cudaLaunchKernelEx(&config, kernel, tq, tk, tv, tdo, a));
   return MODDIT_OK;
 }
 
