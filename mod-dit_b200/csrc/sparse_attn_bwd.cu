@@ -1001,7 +1001,8 @@ int launch(BwdArgs a, const void* out, const void* lo, const float* lse, int dty
   config.stream = st;
   config.attrs = &beside;
   config.numAttrs = 1;
-  MODDIT_CHECK_CUDA(cudaLaunchKernelEx(&config, kernel, tq, tk, tv, tdo, a));
+  (void)cudaLaunchKernelEx(&config, kernel, tq, tk, tv, tdo, a);
+  MODDIT_CHECK_LAUNCH("sparse_attn_bwd_kernel");
   return MODDIT_OK;
 }
 
