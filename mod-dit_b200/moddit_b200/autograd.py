@@ -20,7 +20,7 @@ class _SparseAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lists, key_lists, limits, check_status):
         wanted = any(ctx.needs_input_grad[:3])
-        if check_status == "deferred" and not torch.cuda.is_current_stream_capturing():
+        if check_status == "deferred" and q.is_cuda and not torch.cuda.is_current_stream_capturing():
             ops.check_posted_status(q.device)
         res = ops.sparse_attn_fwd(q, k, v, lists.counts, lists.entries, order=lists.order, return_residual=wanted,
                                   check_status=False if check_status == "deferred" else check_status, **limits)
