@@ -280,10 +280,10 @@ def AttentionSparseEngine(query, key, value, mask, pre_defined_mask=None, video_
 
     Video query rows (index < video_token_num) see the keys below the valid length rounded up to 64, text
     rows see exactly the valid keys - the split the reference gets from its two third-party kernels.
-    One kernel launch covers both; the result is (B,H,S,D).  Where query, key or value require gradients the result is
-    differentiable with respect to them, the mask being a constant (not with `_scatter` or `_group_ready`).  When the mask is a stand-in that keeps every
-    block (a caller passing a mask of another shape, as the dense steps do), every row sees exactly the valid
-    keys, like the reference's dense branch (:268-276).  Whether a full-shape mask happens to be all true is
+    One kernel launch covers both; the result is (B,H,S,D).  Where query, key or value require gradients the
+    result is differentiable with respect to them, the mask being a constant (not with `_scatter` or
+    `_group_ready`).  When the mask is a stand-in that keeps every block (a caller passing a mask of another
+    shape, as the dense steps do), every row sees exactly the valid keys, like the reference's dense branch (:268-276).  Whether a full-shape mask happens to be all true is
     not looked up (the reference pays a host synchronisation per call for that): it goes down the sparse
     branch with the 64-rounded border.
     """

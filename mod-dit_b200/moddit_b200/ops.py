@@ -1081,8 +1081,10 @@ def sparse_attn_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
 
     q, k, v, the limits and the scale are the forward's, `out` and `lse` what it returned (`return_lse=True`), `lists`
     and `key_lists` the results of `tile_lists` and `key_lists` for its mask.  `residual` (of `return_residual=True`) makes
-    the gradients of q and k of rows with nearly all of their weight on one key exact to 16 bits.  The probabilities are computed again tile
-    by tile; the results are the same bits on every run.  check_status: as in `sparse_attn_fwd`."""
+    the gradients of q and k of rows with nearly all of their weight on one key exact to 16 bits.  The probabilities
+    are computed again tile by tile; the results are the same bits on every run.  Keys at and past the larger limit
+    are never read; all other rows have to be finite, those that attend to nothing among them.  check_status: as in
+    `sparse_attn_fwd`."""
     rest = () if residual is None else (residual,)
     dev = _need_cuda(dout, q, k, v, out, lse, *rest)
     if q.dim() != 4:
