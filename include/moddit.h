@@ -350,7 +350,8 @@ int moddit_sparse_attn_fwd_residual(const void* q, const void* k, const void* v,
  *   workspace : moddit_sparse_attn_bwd_workspace_bytes(BH, N) bytes of scratch, 16-byte aligned
  *   status    : as in the forward
  * Rows that attend to nothing (lse = -inf) and keys that no row attends to get zeros.  Keys at and past the larger limit are
- * never read; all other rows have to be finite, because a tile is multiplied whole where its mask keeps any of it.
+ * never read, nor are blocks of 64 queries that see no key; all other rows have to be finite, because a block is multiplied whole
+ * where the mask and the limits keep any of it.
  */
 size_t moddit_sparse_attn_bwd_workspace_bytes(int BH, int N);
 int moddit_sparse_attn_bwd(const void* q, const void* k, const void* v, const void* out, const void* out_lo,

@@ -1083,8 +1083,8 @@ def sparse_attn_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
     and `key_lists` the results of `tile_lists` and `key_lists` for its mask.  `residual` (of `return_residual=True`) makes
     the gradients of q and k of rows with nearly all of their weight on one key exact to 16 bits.  The probabilities
     are computed again tile by tile; the results are the same bits on every run.  Keys at and past the larger limit
-    are never read; all other rows have to be finite, those that attend to nothing among them.  check_status: as in
-    `sparse_attn_fwd`."""
+    are never read; all other rows have to be finite, but for whole blocks of 64 queries that see no key.
+    check_status: as in `sparse_attn_fwd`."""
     rest = () if residual is None else (residual,)
     dev = _need_cuda(dout, q, k, v, out, lse, *rest)
     if q.dim() != 4:

@@ -102,6 +102,11 @@ CASES = [
     (1, 2, 512, 128, 128, 1.0, 2, 300, 256, 129),
     (1, 1, 512, 64, 128, 1.0, 1, 0, 512, 65),
     (1, 1, 2048, 128, 128, 0.3, 1, None, None, None),
+    # limits far apart: first queries that see few or no keys, keys that only the last queries see, and the other way round
+    (1, 2, 900, 128, 64, 0.5, 2, 512, 256, 900),
+    (2, 2, 900, 64, 64, 0.5, 1, 448, 130, 900),
+    (1, 2, 900, 64, 128, 1.0, 2, 600, 0, 900),
+    (1, 2, 900, 128, 128, 1.0, 1, 700, 900, 0),
 ]
 
 
@@ -223,3 +228,18 @@ def test_long_rows_of_few_blocks(ops):
     gone[:] = True
     gone[keys] = False
     assert (dk[:, :, gone.cuda()] == 0).all() and (dv[:, :, gone.cuda()] == 0).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_rows_that_the_limits_leave_empty_hold_anything(ops, D):
+    """Blocks of 64 queries that see no key because of the limits are not multiplied: NaN there reaches nothing."""
+    N, split = 700, 320
+    q, k, v, dout = make(1, 2, N, D, torch.bfloat16, 77)
+    mask = torch.ones(2, 11, 11, dtype=torch.bool)
+    kw = dict(q_split=split, kv_len_lo=0, kv_len_hi=N)
+    _, _, want = run(ops, q, k, v, dout, mask, 64, **kw)
+    q[:, :, :split] = float("nan")
+    dout[:, :, :split] = float("inf")
+    out, lse, got = run(ops, q, k, v, dout, mask, 64, **kw)
+    assert (out[:, :, :split] == 0).all() and torch.isinf(lse[:, :, :split]).all()
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and (got[0][:, :, :split] == 0).all()
