@@ -125,7 +125,7 @@ __device__ __forceinline__ int expand(const int32_t* ent, const int32_t* counts,
   return n;
 }
 
-// Where the limits differ: leaves out of a list of `expand` the halves, and the blocks, in which no query may see a key, so that
+// Where the limits end in different blocks: leaves out of a list of `expand` the halves, and the blocks, in which no query may see a key, so that
 // what such rows hold is never multiplied.  A function of its own, called there only: inside `expand` it changed what the compiler
 // made of the rest (query items at D = 128 177 -> 183 us); like this nothing is slower.
 __device__ __noinline__ int visible(const BwdArgs& a, bool keys, int row0, int n, int32_t* blocks) {
@@ -925,7 +925,7 @@ __global__ void __launch_bounds__(kThreads<D>, 1) sparse_attn_bwd_kernel(
     int n = it.keys ? expand<true>(ent, l.counts + item, a.ntiles, 0, a.N, ctl->blocks)
                           : expand<false>(ent, l.counts + item, a.ntiles, 4 * (it.pos & 1), kv_max, ctl->blocks);
     n = (it.keys && b.row0 >= kv_max) ? 0 : n;    // keys that no row may see
-    if (a.kvl_lo != a.kvl_hi) n = visible(a, it.keys, b.row0, n, ctl->blocks);
+    if ((a.kvl_lo + kBlock - 1) / kBlock != (a.kvl_hi + kBlock - 1) / kBlock) n = visible(a, it.keys, b.row0, n, ctl->blocks);
     if (lane == 0) ctl->count = n;
   }
   __syncthreads();
