@@ -359,22 +359,18 @@ __device__ __forceinline__ void store_rows(uint32_t t, bool any, bool in, float 
 }
 
 // What an elementwise thread of a query item reads while the block is set up: 32 words of a row of Q or dO (which end up in
-// tensor memory; at D = 64 two warpgroups have a row each, at D = 128 four half a row), zeros past the last row, and the row's
-// statistics.
+// tensor memory; at D = 64 two warpgroups have a row each, at D = 128 four half a row), zeros past the last row.  Not the row's
+// statistics: the kernel that computes them may still be at work then.
 template <int D>
 struct Fixed {
   uint32_t v[32];
-  float nl, nd;
   static __device__ __forceinline__ int group() { return (static_cast<int>(threadIdx.x) - 128) / 128; }
   static __device__ __forceinline__ int which() { return D == 64 ? group() : group() / 2; }
   static __device__ __forceinline__ int part() { return D == 64 ? 0 : group() & 1; }
   static __device__ __forceinline__ bool mine() { return which() < 2; }
   __device__ __forceinline__ void load(const BwdArgs& a, int bh, int row0) {
-    const int grow = row0 + threadIdx.x % 128;
-    const int64_t at = static_cast<int64_t>(bh) * a.npad + grow;
-    nl = a.nlse[at];
-    nd = a.ndelta[at];
     if (!mine()) return;
+    const int grow = row0 + threadIdx.x % 128;
     const uint4* src = reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(which() ? a.dout : a.q) +
                                                       (static_cast<int64_t>(bh) * a.N + grow) * D * 2) + part() * 8;
 #pragma unroll
@@ -621,7 +617,12 @@ struct Chains {
       ptx::tmem_st32(t + kF + fixed.which() * (D / 2) + fixed.part() * 32, fixed.v);
       hand_over(b.bar(kFixed));
     }
-    const float nl = fixed.nl, nd = fixed.nd;
+    float nl = 0.f, nd = 0.f;                     // query items: the row's statistics, which are there since the wait for them
+    if (!kKeys) {
+      const int64_t at = static_cast<int64_t>(b.bh) * a.npad + grow;
+      nl = a.nlse[at];
+      nd = a.ndelta[at];
+    }
     const int lim = grow < a.q_split ? a.kvl_lo : a.kvl_hi;
     int rows_lo = 0, rows_hi = 0;                 // key items: which of this thread's four rows lie below the limits
     if (kKeys)
@@ -930,7 +931,7 @@ __global__ void __launch_bounds__(kThreads<D>, 1) sparse_attn_bwd_kernel(
   }
   __syncthreads();
   ptx::tc_fence_after();
-  asm volatile("griddepcontrol.wait;" ::: "memory");      // for the row statistics
+  asm volatile("griddepcontrol.wait;" ::: "memory");      // for the row statistics: nothing above may read them
   b.tmem = ctl->tmem_base;
   b.count = ctl->count;
 
@@ -1014,7 +1015,7 @@ int launch(BwdArgs a, const void* out, const void* lo, const float* lse, int dty
   MODDIT_CHECK_LAUNCH("bwd_stats_kernel");
   const int64_t blocks = static_cast<int64_t>(2 * a.ntiles + (a.ntiles & 1)) * BH;
   // Launched beside the statistics: barriers, tensor memory and block lists are ready when these are.  2 heads of 4,096 at D = 128
-  // 59.3 -> 57.6 us, 1,200 rows 23.9 -> 22.9; the next launch of the stream still waits for all of it.
+  // 58.8 -> 57.6 us, 1,200 rows 23.3 -> 22.7; the next launch of the stream still waits for all of it.
   cudaLaunchAttribute beside{};
   beside.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   beside.val.programmaticStreamSerializationAllowed = 1;
