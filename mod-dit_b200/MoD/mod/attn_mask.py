@@ -582,6 +582,7 @@ def _spargeattn_step(query, key, value, warmup_state):
     similar to one another (mean pairwise cosine similarity below state key `spargeattn_sim_threshold`; key
     rows relative to the mean key of the head) are not trusted to their mean: such a query block keeps every
     key block, such a key block is kept by every query block.  The default threshold 0 switches that test off.
+    The output is differentiable where the inputs ask for gradients, the mask a constant.
     Not taken over: the package's 8-bit quantisation of the products, its 128 x 64 block shape (the mask has
     the state's square block_size) and its skipping of small value products inside the kernel."""
     bs = warmup_state['block_size']
@@ -603,8 +604,11 @@ def _spargeattn_step(query, key, value, warmup_state):
     mask = _ops.select_topk_blocks(dark, count, row_full, col_keep)
     warmup_state['mask'] = mask
     lists = _ops.tile_lists(mask, bs, seq_len)
-    output = _ops.sparse_attn_fwd(query, key, value, lists.counts, lists.entries, order=lists.order,
-                                  check_status="deferred")
+    if _needs_grad(query, key, value):
+        output = _autograd.sparse_attention(query, key, value, lists, _ops.key_lists(mask, bs, seq_len))
+    else:
+        output = _ops.sparse_attn_fwd(query, key, value, lists.counts, lists.entries, order=lists.order,
+                                      check_status="deferred")
     return output, {'mode': 'warmup', 'mask': None}
 
 

@@ -1,0 +1,92 @@
+"""Gradients through the layer's own entry points: every kind of step gives, where its inputs ask for gradients, the output and the
+state of the same step without, bit for bit, and the gradients of `autograd.sparse_attention` under the mask that the step ran."""
+import logging
+import warnings
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+LOG = logging.getLogger("test")
+H, GRID, D, BS, TEXT = 2, (4, 16, 16), 64, 128, 128
+VIDEO = GRID[0] * GRID[1] * GRID[2]
+N = VIDEO + TEXT
+VALID = N - 37
+
+
+@pytest.fixture(scope="module")
+def mods():
+    import MoD.mod.attn_mask as am
+    from moddit_b200 import autograd, ops
+    return am, autograd, ops
+
+
+def inputs(step):
+    from moddit_b200 import synth
+    q, k, v = synth.make_qkv(heads=H, grid=GRID, head_dim=D, text_tokens=TEXT, seed=20 + step, device=torch.device("cuda"))
+    g = torch.Generator(device="cuda").manual_seed(step)
+    return q, k, v, torch.randn(q.shape, generator=g, device="cuda").to(q.dtype)
+
+
+def new_state(**extra):
+    from MoD.mod.state import create_adaptive_mask_state
+    state = create_adaptive_mask_state("hunyuan", H, VIDEO, TEXT, GRID[1] * GRID[2], GRID[0], warmup_steps=3, top_k=4, predict_T=3,
+                                       threshold=1e-3, block_size=BS, sparse_type=extra.pop("sparse_type", "mod-dit"))
+    state.update(extra)
+    return state
+
+
+def padding():
+    return (torch.arange(N) < VALID).unsqueeze(0).expand(N, N).contiguous().cuda()
+
+
+def wanted(mods, q, k, v, dout, mask, **limits):
+    """Gradients under a block mask; None stands for every block."""
+    am, autograd, ops = mods
+    if mask is None:
+        mask = torch.ones(1, (N + BS - 1) // BS, (N + BS - 1) // BS, dtype=torch.bool, device="cuda")
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    out = autograd.sparse_attention(*leaves, ops.tile_lists(mask, BS, N), ops.key_lists(mask, BS, N), **limits)
+    return out.detach(), torch.autograd.grad(out, leaves, dout)
+
+
+def holds_no_graph(value):
+    if torch.is_tensor(value):
+        return not value.requires_grad
+    if isinstance(value, dict):
+        return all(holds_no_graph(v) for v in value.values())
+    if isinstance(value, (list, tuple)):
+        return all(holds_no_graph(v) for v in value)
+    return True
+
+
+def both(mods, state, twin, step, **kw):
+    """One step with and one without gradients, each on a state of its own: (inputs, output, gradients)."""
+    am, _, _ = mods
+    q, k, v, dout = inputs(step)
+    plain, _ = am.SparseAttentionWithMap(q, k, v, twin, LOG, current_step=step, **kw)
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        out, _ = am.SparseAttentionWithMap(*leaves, state, LOG, current_step=step, **kw)
+    assert plain.grad_fn is None and out.requires_grad and torch.equal(out, plain)
+    with torch.no_grad():
+        assert holds_no_graph(state)
+    got = torch.autograd.grad(out, leaves, dout)
+    return (q, k, v, dout), out.detach(), got
+
+
+def same(got, want):
+    return all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+SPARSE = dict(q_split=VIDEO, kv_len_lo=(VALID + 63) // 64 * 64, kv_len_hi=VALID)
+
+
+@pytest.mark.parametrize("threshold", [0.0, 0.3])
+def test_spargeattn(mods, threshold):
+    state, twin = (new_state(sparse_type="spargeattn", spargeattn_sim_threshold=threshold) for _ in range(2))
+    x, out, got = both(mods, state, twin, 7)
+    assert torch.equal(state["mask"], twin["mask"])
+    want_out, want = wanted(mods, *x, state["mask"])
+    assert torch.equal(out, want_out) and same(got, want)
