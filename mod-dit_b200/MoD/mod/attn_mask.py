@@ -27,7 +27,8 @@ import torch
 from MoD.mod.cuda_lstsq import features_from_solution, solve_lstsq
 from MoD.mod.get_radial_mask import get_radial_mask
 from MoD.mod.state import is_warmup_complete
-from MoD.mod.triton_flash_sparsity import dense_attention_with_lse, flash_attn_with_sparsity_map
+from MoD.mod.triton_flash_sparsity import (attn_with_sparsity_map, dense_attention_with_lse,
+                                           flash_attn_with_sparsity_map)
 from moddit_b200 import _lib
 from moddit_b200 import autograd as _autograd
 from moddit_b200 import ops as _ops
@@ -65,14 +66,16 @@ def update_warmup(warmup_state: Dict, step: int, block_sparse_map: torch.Tensor)
 # ------------------------------------------------------------------------------------------------
 
 def compute_block_sparse_map_triton(query, key, value, warmup_state):
-    """Dense output and exact sparsity map (name kept from the reference, :252-263)."""
-    return flash_attn_with_sparsity_map(
-        query, key, value,
-        block_size=warmup_state['block_size'],
-        video_token_num=warmup_state['video_token_num'],
-        text_token_num=warmup_state['text_token_num'],
-        threshold=warmup_state['threshold'],
-        model_type=warmup_state['model_type'])
+    """Dense output and exact sparsity map (name kept from the reference, :252-263).  The output is differentiable where
+    the inputs ask for gradients; the map is a constant."""
+    how = dict(block_size=warmup_state['block_size'],
+               video_token_num=warmup_state['video_token_num'],
+               text_token_num=warmup_state['text_token_num'],
+               threshold=warmup_state['threshold'],
+               model_type=warmup_state['model_type'])
+    if _needs_grad(query, key, value):
+        return attn_with_sparsity_map(_dense_with_gradient, query, key, value, **how)
+    return flash_attn_with_sparsity_map(query, key, value, **how)
 
 
 compute_block_sparse_map = compute_block_sparse_map_triton
@@ -200,14 +203,19 @@ def _key_lists(mask: torch.Tensor, mask_heads: int, block_size: int, seq_len: in
     return _ops.key_lists(mask[:mask_heads], block_size, seq_len)       # lists of one head serve a mask that all heads share
 
 
-def _dense(query, key, value, kv_len: int):
-    """Dense attention over the first kv_len keys; differentiable where the inputs ask for gradients."""
-    if not _needs_grad(query, key, value):
-        return dense_attention_with_lse(query, key, value, kv_len=kv_len)[0]
+def _dense_with_gradient(query, key, value, softmax_scale=None, kv_len=None):
+    """`dense_attention_with_lse` with a differentiable output."""
     nb = (query.shape[2] + 127) // 128
     mask = torch.ones(1, nb, nb, device=query.device, dtype=torch.bool)
     return _autograd.sparse_attention(query, key, value, _ops.tile_lists(mask, 128, query.shape[2]),
-                                      _ops.key_lists(mask, 128, query.shape[2]), kv_len_lo=kv_len, kv_len_hi=kv_len)
+                                      _ops.key_lists(mask, 128, query.shape[2]), softmax_scale=softmax_scale,
+                                      kv_len_lo=kv_len, kv_len_hi=kv_len, return_lse=True)
+
+
+def _dense(query, key, value, kv_len: int):
+    """Dense attention over the first kv_len keys; differentiable where the inputs ask for gradients."""
+    attention = _dense_with_gradient if _needs_grad(query, key, value) else dense_attention_with_lse
+    return attention(query, key, value, kv_len=kv_len)[0]
 
 
 def _events(ready):
@@ -454,6 +462,8 @@ def SparseAttentionWithMap(
     once per group, each launch behind its own event, so the first group computes while the others still travel.
     `warmup_state['_head_groups'] = G` must be set so that the work lists are ordered group by group.
 
+    Every step's output is differentiable with respect to query, key and value where these require gradients (not
+    with `output_scatter`, which says so); masks, maps and features are constants.
     Steps warmup-2 and warmup-1 collect features (dense output); afterwards every predict_T-th step
     refreshes the map, the features and the mask (dense output) and all other steps run the block-sparse
     forward under the stored mask.  Returns (output (1,H,S,D), mask info) like the reference.

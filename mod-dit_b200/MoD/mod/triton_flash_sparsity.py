@@ -132,16 +132,24 @@ def flash_attn_with_sparsity_map(query, key, value, threshold, block_size, model
 
     Same contract as MoD/mod/triton_flash_sparsity.py:275-341.
     """
+    return attn_with_sparsity_map(dense_attention_with_lse, query, key, value, threshold, block_size, model_type,
+                                  video_token_num, text_token_num)
+
+
+def attn_with_sparsity_map(attention, query, key, value, threshold, block_size, model_type="hunyuan", video_token_num=0,
+                           text_token_num=0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """`flash_attn_with_sparsity_map` with its dense pass given: attention(query, key, value, softmax_scale) -> (O, LSE)."""
     threshold_value, video_block_num, q_video_offset, k_video_offset = _validate_inputs(
         query, key, value, threshold, block_size, model_type, video_token_num, text_token_num)
     D = query.shape[3]
     query, key, value = query.contiguous(), key.contiguous(), value.contiguous()
     sm_scale = D ** -0.5
-    out, lse = dense_attention_with_lse(query, key, value, sm_scale)
+    out, lse = attention(query, key, value, sm_scale)
     ln_thresh = math.log(threshold_value) if threshold_value > 0 else float("-inf")
-    sparsity_map = _compute_sparsity_map(
-        query, key, lse, softmax_scale=sm_scale, log_threshold=ln_thresh, q_video_offset=q_video_offset,
-        k_video_offset=k_video_offset, video_blocks=video_block_num, block_size=block_size)
+    with torch.no_grad():
+        sparsity_map = _compute_sparsity_map(
+            query, key, lse, softmax_scale=sm_scale, log_threshold=ln_thresh, q_video_offset=q_video_offset,
+            k_video_offset=k_video_offset, video_blocks=video_block_num, block_size=block_size)
     return out, sparsity_map
 
 

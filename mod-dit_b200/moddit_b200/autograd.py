@@ -18,44 +18,55 @@ __all__ = ["sparse_attention", "qkv_prologue"]
 
 class _SparseAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, lists, key_lists, limits, check_status):
+    def forward(ctx, q, k, v, lists, key_lists, limits, check_status, return_lse):
         wanted = any(ctx.needs_input_grad[:3])
         if check_status == "deferred" and q.is_cuda and not torch.cuda.is_current_stream_capturing():
             ops.check_posted_status(q.device)
         res = ops.sparse_attn_fwd(q, k, v, lists.counts, lists.entries, order=lists.order, return_residual=wanted,
-                                  check_status=False if check_status == "deferred" else check_status, **limits)
+                                  return_lse=return_lse, check_status=False if check_status == "deferred" else check_status,
+                                  **limits)
         if check_status == "deferred":
             ops.post_status(q.device, spacing=ops.STATUS_SPACING)
         if not wanted:
-            return res
+            return res if return_lse else (res, None)
         out, lse, residual = res
         ctx.save_for_backward(q, k, v, out, lse, residual, lists.counts, lists.entries, lists.order, key_lists.counts,
                               key_lists.entries, key_lists.order)
         ctx.limits, ctx.check_status = limits, check_status
-        return out
+        ctx.set_materialize_grads(False)
+        if not return_lse:
+            return out, None
+        ctx.mark_non_differentiable(lse)
+        return out, lse
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, dout):
+    def backward(ctx, dout, _):
+        if dout is None:
+            return (None,) * 8
         q, k, v, out, lse, residual, *lists = ctx.saved_tensors
         grads = ops.sparse_attn_bwd(dout.contiguous(), q, k, v, out, lse, ops.TileLists(*lists[:3]),
                                     ops.KeyLists(*lists[3:]), residual=residual, check_status=ctx.check_status,
                                     **ctx.limits)
-        return tuple(g if need else None for g, need in zip(grads, ctx.needs_input_grad)) + (None,) * 4
+        return tuple(g if need else None for g, need in zip(grads, ctx.needs_input_grad)) + (None,) * 5
 
 
 def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lists: ops.TileLists, key_lists: ops.KeyLists, *,
                      softmax_scale: Optional[float] = None, q_split: Optional[int] = None,
                      kv_len_lo: Optional[int] = None, kv_len_hi: Optional[int] = None,
-                     check_status="deferred") -> torch.Tensor:
+                     check_status="deferred", return_lse: bool = False):
     """Block-sparse attention of (B, H, N, D) float16 or bfloat16 tensors, differentiable with respect to q, k and v.
 
     lists, key_lists: `ops.tile_lists` and `ops.key_lists` of the layer's mask; the other arguments are those of
     `ops.sparse_attn_fwd` ("deferred": a call raises for a kernel of an earlier step that gave up a wait, once the copy of its status
-    has arrived; copies are queued at most every `ops.STATUS_SPACING` seconds).  Tensors that are not contiguous are copied.  What lies between the forward and the backward is q, k, v, the output, what rounding took from
-    it and 4 bytes per row."""
+    has arrived; copies are queued at most every `ops.STATUS_SPACING` seconds).  return_lse: (out, lse), lse a
+    constant.  Tensors that are not contiguous are copied.  What lies between the forward and the backward is q, k, v, the
+    output, what rounding took from it, 4 bytes per row and the work lists (of (N / 128)^2 entries of 4 bytes per mask head the
+    key lists, half as many the others)."""
     limits = dict(softmax_scale=softmax_scale, q_split=q_split, kv_len_lo=kv_len_lo, kv_len_hi=kv_len_hi)
-    return _SparseAttention.apply(q.contiguous(), k.contiguous(), v.contiguous(), lists, key_lists, limits, check_status)
+    out, lse = _SparseAttention.apply(q.contiguous(), k.contiguous(), v.contiguous(), lists, key_lists, limits, check_status,
+                                      return_lse)
+    return (out, lse) if return_lse else out
 
 
 class _Prologue(torch.autograd.Function):

@@ -90,3 +90,50 @@ def test_spargeattn(mods, threshold):
     assert torch.equal(state["mask"], twin["mask"])
     want_out, want = wanted(mods, *x, state["mask"])
     assert torch.equal(out, want_out) and same(got, want)
+
+
+@pytest.mark.parametrize("selector", ["topk_lines", "cumulative_mass"])
+def test_steps_of_the_exact_map(mods, selector):
+    """Dense, collecting, sparse and refreshing steps."""
+    state, twin = (new_state(selector=selector) for _ in range(2))
+    for step in range(8):
+        mask = state["mask"]
+        collects, refreshes = step in (1, 2), step in (5,)
+        x, out, got = both(mods, state, twin, step, pre_defined_mask=padding())
+        if step >= 2:
+            assert torch.equal(state["mask"], twin["mask"])
+        if step < 1:
+            want_out, want = wanted(mods, *x, None, kv_len_lo=VALID, kv_len_hi=VALID)
+        elif collects or refreshes:
+            want_out, want = wanted(mods, *x, None)
+        else:
+            want_out, want = wanted(mods, *x, mask, **SPARSE)
+        assert torch.equal(out, want_out) and same(got, want), step
+
+
+def test_radial(mods):
+    state, twin = (new_state(sparse_type="radial") for _ in range(2))
+    for step in (0, 3):
+        x, out, got = both(mods, state, twin, step)
+        want_out, want = wanted(mods, *x, None if step < 3 else state["mask"])
+        assert torch.equal(out, want_out) and same(got, want)
+
+
+def test_two_branches(mods):
+    """Both guidance branches of a collecting and a sparse step in one call."""
+    am, _, _ = mods
+    def states():
+        return [new_state() for _ in range(2)]
+    mine, twins = states(), states()
+    for step in (1, 2, 3):
+        pairs = [inputs(50 + 2 * step + i) for i in range(2)]
+        q, k, v, dout = (torch.cat([p[i] for p in pairs]) for i in range(4))
+        plain, _ = am.SparseAttentionWithMapCFG(q, k, v, twins, LOG, current_step=step)
+        leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+        mask = None if step < 3 else [s["mask"] for s in mine]
+        out, _ = am.SparseAttentionWithMapCFG(*leaves, mine, LOG, current_step=step)
+        assert torch.equal(out, plain)
+        got = torch.autograd.grad(out, leaves, dout)
+        for i, p in enumerate(pairs):
+            _, want = wanted(mods, *p, None if mask is None else mask[i])
+            assert same([t[i:i + 1] for t in got], want)
