@@ -289,8 +289,8 @@ def AttentionSparseEngine(query, key, value, mask, pre_defined_mask=None, video_
     Video query rows (index < video_token_num) see the keys below the valid length rounded up to 64, text
     rows see exactly the valid keys - the split the reference gets from its two third-party kernels.
     One kernel launch covers both; the result is (B,H,S,D).  Where query, key or value require gradients the
-    result is differentiable with respect to them, the mask being a constant (not with `_scatter` or
-    `_group_ready`).  When the mask is a stand-in that keeps every block (a caller passing a mask of another
+    result is differentiable with respect to them, the mask being a constant (not with `_scatter`; groups of heads run in
+    one launch then, behind the last group's arrival).  When the mask is a stand-in that keeps every block (a caller passing a mask of another
     shape, as the dense steps do), every row sees exactly the valid keys, like the reference's dense branch (:268-276).  Whether a full-shape mask happens to be all true is
     not looked up (the reference pays a host synchronisation per call for that): it goes down the sparse
     branch with the 64-rounded border.
@@ -311,13 +311,18 @@ def AttentionSparseEngine(query, key, value, mask, pre_defined_mask=None, video_
         valid = _valid_kv(pre_defined_mask, seq_len)
         border = valid if all_kept else min(seq_len, (valid + 63) // 64 * 64)
         fwd_kw = dict(q_split=video_token_num, kv_len_lo=border, kv_len_hi=valid)
-    if _group_ready is not None and len(_group_ready) > 1:
-        if query.shape[0] != 1 or lists.counts.shape[0] != query.shape[1]:
-            raise ValueError("head groups need a batch of one and one mask per head")
-        return _engine_by_head_groups(query, key, value, lists, _group_ready, _scatter, **fwd_kw)
+    grouped = _group_ready is not None and len(_group_ready) > 1
+    if grouped and (query.shape[0] != 1 or lists.counts.shape[0] != query.shape[1]):
+        raise ValueError("head groups need a batch of one and one mask per head")
     if _scatter is None and _needs_grad(query, key, value):
+        if grouped:                    # one launch behind every group's arrival, over lists in the order of one launch
+            for ev in _events(_group_ready):
+                torch.cuda.current_stream(query.device).wait_event(ev)
+            lists = _engine_lists(mask, block_size, seq_len)[0]
         return _autograd.sparse_attention(query, key, value, lists, _key_lists(mask, counts.shape[0], block_size, seq_len),
                                           **fwd_kw)
+    if grouped:
+        return _engine_by_head_groups(query, key, value, lists, _group_ready, _scatter, **fwd_kw)
     return _ops.sparse_attn_fwd(query, key, value, counts, entries, order=order, check_status="deferred",
                                 scatter=_scatter, **fwd_kw)
 

@@ -111,6 +111,51 @@ def test_steps_of_the_exact_map(mods, selector):
         assert torch.equal(out, want_out) and same(got, want), step
 
 
+@pytest.mark.parametrize("groups", [1, 2])
+def test_steps_of_the_pooled_map(mods, groups):
+    """Dense, collecting and sparse steps, with query, key and value complete or arriving in two groups of heads."""
+    extra = dict(score_producer="pooled")
+    kw = dict(pre_defined_mask=padding())
+    if groups > 1:
+        extra["_head_groups"] = groups
+        kw["head_group_ready"] = [torch.cuda.Event() for _ in range(groups)]
+        for e in kw["head_group_ready"]:
+            e.record()
+    state, twin = new_state(**extra), new_state(**extra)
+    for step in range(6):
+        x, out, got = both(mods, state, twin, step, **kw)
+        if step < 2:
+            want_out, want = wanted(mods, *x, None, kv_len_lo=VALID, kv_len_hi=VALID)
+        else:
+            assert torch.equal(state["mask"], twin["mask"])
+            want_out, want = wanted(mods, *x, state["mask"], **SPARSE)
+        assert torch.equal(out, want_out) and same(got, want), step
+
+
+def test_head_groups_arrive_before_the_gradient_path_reads(mods):
+    """The launch that is differentiable waits for every group's event, whatever the event's stream still does."""
+    am, _, ops = mods
+    q, k, v, dout = inputs(30)
+    mask = torch.rand(H, 9, 9, generator=torch.Generator().manual_seed(1)).lt(0.5).cuda()
+    want_out, want = wanted(mods, q, k, v, dout, mask)
+    late = [torch.zeros_like(t) for t in (q, k, v)]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    ready = [torch.cuda.Event() for _ in range(H)]
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20000000)                 # some ten milliseconds
+        for h, e in enumerate(ready):
+            for dst, src in zip(late, (q, k, v)):
+                dst[:, h].copy_(src[:, h])
+            e.record()
+    leaves = [t.requires_grad_(True) for t in late]
+    lists = ops.tile_lists(mask, BS, N, heads_per_group=1)
+    out = am.AttentionSparseEngine(*leaves, mask, block_size=BS, _lists=lists, _group_ready=ready)
+    got = torch.autograd.grad(out, leaves, dout)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want_out) and same(got, want)
+
+
 def test_radial(mods):
     state, twin = (new_state(sparse_type="radial") for _ in range(2))
     for step in (0, 3):
