@@ -19,6 +19,7 @@ Differences that are deliberate:
 """
 import logging
 import math
+import warnings
 import weakref
 from typing import Dict, List, Optional, Tuple
 
@@ -289,7 +290,7 @@ def AttentionSparseEngine(query, key, value, mask, pre_defined_mask=None, video_
     Video query rows (index < video_token_num) see the keys below the valid length rounded up to 64, text
     rows see exactly the valid keys - the split the reference gets from its two third-party kernels.
     One kernel launch covers both; the result is (B,H,S,D).  Where query, key or value require gradients the
-    result is differentiable with respect to them, the mask being a constant (not with `_scatter`; groups of heads run in
+    result is differentiable with respect to them, the mask being a constant (not with `_scatter`, which warns; groups of heads run in
     one launch then, behind the last group's arrival).  When the mask is a stand-in that keeps every block (a caller passing a mask of another
     shape, as the dense steps do), every row sees exactly the valid keys, like the reference's dense branch (:268-276).  Whether a full-shape mask happens to be all true is
     not looked up (the reference pays a host synchronisation per call for that): it goes down the sparse
@@ -321,6 +322,9 @@ def AttentionSparseEngine(query, key, value, mask, pre_defined_mask=None, video_
             lists = _engine_lists(mask, block_size, seq_len)[0]
         return _autograd.sparse_attention(query, key, value, lists, _key_lists(mask, counts.shape[0], block_size, seq_len),
                                           **fwd_kw)
+    if _needs_grad(query, key, value):
+        warnings.warn("query, key or value require gradients, but rows that are stored into peers' buffers have no gradient: "
+                      "call without the output scatter to train, or under torch.no_grad()", stacklevel=2)
     if grouped:
         return _engine_by_head_groups(query, key, value, lists, _group_ready, _scatter, **fwd_kw)
     return _ops.sparse_attn_fwd(query, key, value, counts, entries, order=order, check_status="deferred",

@@ -164,6 +164,25 @@ def test_radial(mods):
         assert torch.equal(out, want_out) and same(got, want)
 
 
+def test_output_that_goes_to_peers_says_that_it_has_no_gradient(mods):
+    """Rows stored into other tensors are not part of the graph: the call says so once its inputs ask for gradients."""
+    am, _, _ = mods
+    q, k, v, _ = inputs(40)
+    mask = torch.rand(H, 9, 9, generator=torch.Generator().manual_seed(2)).lt(0.5).cuda()
+    want = am.AttentionSparseEngine(q, k, v, mask, block_size=BS)
+    for ask in (False, True):
+        to = torch.zeros_like(q)
+        leaves = [t.clone().requires_grad_(ask) for t in (q, k, v)]
+        with warnings.catch_warnings(record=True) as seen:
+            warnings.simplefilter("always")
+            am.AttentionSparseEngine(*leaves, mask, block_size=BS, _scatter=([to.data_ptr()], 0))
+            with torch.no_grad():
+                am.AttentionSparseEngine(*leaves, mask, block_size=BS, _scatter=([to.data_ptr()], 0))
+        torch.cuda.synchronize()
+        assert torch.equal(to, want)
+        assert [str(w.message).count("no gradient") for w in seen] == [1] * ask
+
+
 def test_two_branches(mods):
     """Both guidance branches of a collecting and a sparse step in one call."""
     am, _, _ = mods
