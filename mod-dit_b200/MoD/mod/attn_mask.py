@@ -304,7 +304,9 @@ def AttentionSparseEngine(query, key, value, mask, pre_defined_mask=None, video_
     else:
         lists, all_kept = _engine_lists(mask, block_size, seq_len)
     counts, entries, order = lists.counts, lists.entries, lists.order
-    for ev in _events(_value_ready):   # inputs produced on another stream (e.g. still arriving from peers)
+    grouped = _group_ready is not None and len(_group_ready) > 1
+    # inputs produced on another stream (e.g. still arriving from peers); a single group is one more of them
+    for ev in _events(_value_ready) + (() if grouped else _events(_group_ready)):
         torch.cuda.current_stream(query.device).wait_event(ev)
     value = value.contiguous()
     fwd_kw = {}
@@ -312,7 +314,6 @@ def AttentionSparseEngine(query, key, value, mask, pre_defined_mask=None, video_
         valid = _valid_kv(pre_defined_mask, seq_len)
         border = valid if all_kept else min(seq_len, (valid + 63) // 64 * 64)
         fwd_kw = dict(q_split=video_token_num, kv_len_lo=border, kv_len_hi=valid)
-    grouped = _group_ready is not None and len(_group_ready) > 1
     if grouped and (query.shape[0] != 1 or lists.counts.shape[0] != query.shape[1]):
         raise ValueError("head groups need a batch of one and one mask per head")
     if _scatter is None and _needs_grad(query, key, value):

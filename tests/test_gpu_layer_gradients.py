@@ -201,3 +201,26 @@ def test_two_branches(mods):
         for i, p in enumerate(pairs):
             _, want = wanted(mods, *p, None if mask is None else mask[i])
             assert same([t[i:i + 1] for t in got], want)
+
+
+@pytest.mark.parametrize("ask", [False, True])
+def test_a_single_group_of_heads_is_waited_for(mods, ask):
+    """One event for all heads: rows that another stream still writes are read behind it, with and without gradients."""
+    am, _, ops = mods
+    q, k, v, dout = inputs(31)
+    mask = torch.rand(H, 9, 9, generator=torch.Generator().manual_seed(3)).lt(0.5).cuda()
+    want_out, want = wanted(mods, q, k, v, dout, mask)
+    late = [torch.zeros_like(t) for t in (q, k, v)]
+    lists = ops.tile_lists(mask, BS, N)
+    torch.cuda.synchronize()
+    side, ready = torch.cuda.Stream(), torch.cuda.Event()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20000000)
+        for dst, src in zip(late, (q, k, v)):
+            dst.copy_(src)
+        ready.record()
+    leaves = [t.requires_grad_(ask) for t in late]
+    out = am.AttentionSparseEngine(*leaves, mask, block_size=BS, _lists=lists, _group_ready=[ready])
+    got = torch.autograd.grad(out, leaves, dout) if ask else want
+    torch.cuda.synchronize()
+    assert torch.equal(out, want_out) and same(got, want)
