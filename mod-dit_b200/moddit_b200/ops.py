@@ -952,7 +952,6 @@ def post_status(device, spacing: float = 0.0) -> None:
     now = time.monotonic()
     if spacing and now - _LAST_POST.get(idx, 0.0) < spacing:
         return
-    _LAST_POST[idx] = now
     slot = _POSTED.get(idx)
     if slot is None:
         slot = [torch.zeros(4, dtype=torch.int32).pin_memory(), None]
@@ -963,6 +962,7 @@ def post_status(device, spacing: float = 0.0) -> None:
     ev = torch.cuda.Event()
     ev.record(torch.cuda.current_stream(device))
     slot[1] = ev
+    _LAST_POST[idx] = now
 
 
 def check_posted_status(device) -> None:
