@@ -936,7 +936,7 @@ def raise_on_status(device) -> None:
 
 
 _LAST_POST: Dict[int, float] = {}      # device index -> when `post_status` last queued a copy
-STATUS_SPACING = 1e-2                  # seconds between the copies that training calls queue: a copy and its change of engines
+STATUS_SPACING = 1e-2                  # seconds between the copies that steps under autograd queue: a copy and its change of engines
                                        # hold up a stream of short launches by some ten microseconds
 
 
@@ -993,9 +993,9 @@ def check_health(device) -> None:
             f"position={vals[3]}); the sparsity maps written since the last check are invalid")
 
 
-def _after_launch(dev, check_status, spacing: float = 0.0) -> None:
+def _after_launch(dev, check_status) -> None:
     if check_status == "deferred":
-        post_status(dev, spacing)
+        post_status(dev)
     elif check_status:
         raise_on_status(dev)
 
@@ -1118,5 +1118,5 @@ def sparse_attn_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
             D ** -0.5 if softmax_scale is None else softmax_scale, N if q_split is None else q_split,
             N if kv_len_lo is None else kv_len_lo, N if kv_len_hi is None else kv_len_hi, dq.data_ptr(), dk.data_ptr(),
             dv.data_ptr(), ws.data_ptr(), wsb, _status_words(dev).data_ptr(), _stream(dev)), "moddit_sparse_attn_bwd")
-    _after_launch(dev, check_status, spacing=STATUS_SPACING)
+    _after_launch(dev, check_status)
     return dq, dk, dv
