@@ -34,6 +34,10 @@ extern "C" {
 #define MODDIT_E_CUDA (-5)        /* a CUDA runtime/driver call failed (message has the detail) */
 #define MODDIT_E_DEVICE (-6)      /* device is not compute capability 10.x */
 
+/* what the gradients cover: rows of an attention problem, values of a token in a normalisation over all heads */
+#define MODDIT_ATTN_BWD_MAX_ROWS 458752
+#define MODDIT_TOKEN_NORM_BWD_MAX_WIDTH 49152
+
 /* layout codes for masks (token order of the sequence) — MoD/mod/triton_flash_sparsity.py:101-120 */
 #define MODDIT_LAYOUT_WAN 0       /* video only */
 #define MODDIT_LAYOUT_HUNYUAN 1   /* video first, then text */
@@ -349,7 +353,7 @@ int moddit_sparse_attn_fwd_residual(const void* q, const void* k, const void* v,
  *               the same mask (the orders may be NULL)
  *   workspace : moddit_sparse_attn_bwd_workspace_bytes(BH, N) bytes of scratch, 16-byte aligned
  *   status    : as in the forward
- * Rows that attend to nothing (lse = -inf) and keys that no row attends to get zeros.  Keys at and past the larger limit are
+ * Up to MODDIT_ATTN_BWD_MAX_ROWS rows.  Rows that attend to nothing (lse = -inf) and keys that no row attends to get zeros.  Keys at and past the larger limit are
  * never read, nor are blocks of 64 queries that see no key; all other rows have to be finite, because a block is multiplied whole
  * where the mask and the limits keep any of it.
  */
@@ -460,7 +464,7 @@ int moddit_qkv_prologue(const void* q_in, const void* k_in, const void* v_in, in
  *   dq_in,dk_in,dv_in : (B, S, H*D) results, out_stride elements between tokens (slices of one buffer are fine)
  *   dq_weight..dk_bias: null, or where the parameter's gradient goes (D values, H*D for MODDIT_NORM_RMS_ALL_HEADS), of `dtype`
  *   workspace : moddit_qkv_prologue_bwd_workspace_bytes(...) bytes, 16-byte aligned, only for parameter gradients
- * MODDIT_NORM_RMS_ALL_HEADS covers up to 49,152 values a token.  All other arguments as in moddit_qkv_prologue.
+ * MODDIT_NORM_RMS_ALL_HEADS covers up to MODDIT_TOKEN_NORM_BWD_MAX_WIDTH values a token.  All other arguments as in moddit_qkv_prologue.
  */
 size_t moddit_qkv_prologue_bwd_workspace_bytes(int B, int S, int H, int D, int norm_kind);
 int moddit_qkv_prologue_bwd(const void* dq, const void* dk, const void* dv, const void* q_in, const void* k_in, int dtype,

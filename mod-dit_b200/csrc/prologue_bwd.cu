@@ -666,7 +666,7 @@ __global__ void __launch_bounds__(kThreads) prologue_bwd_sums_kernel(const __gri
 constexpr int kBlocksPerHead = 296;
 constexpr int kBlocksAllHeads = 296;
 constexpr int kBlocksTokens = 148;                   // q's and k's half of them each where both are given
-constexpr int kMaxWidth = 48 * 1024;                 // values of a token: their sums lie in shared memory
+constexpr int kMaxWidth = MODDIT_TOKEN_NORM_BWD_MAX_WIDTH;       // values of a token: their sums lie in shared memory
 int heads_per_item(int B, int S, int H, int D) {
   const int64_t tiles = static_cast<int64_t>(B) * ceil_div(S, kRows * kThreads / (D / 8));
   const int chunks = static_cast<int>(std::min<int64_t>(H, (kBlocksPerHead + tiles - 1) / tiles));

@@ -1057,7 +1057,9 @@ extern "C" int moddit_sparse_attn_bwd(const void* q, const void* k, const void* 
                    "sparse_attn_bwd: kv_len (%d, %d) outside [0, N=%d]", kv_len_lo, kv_len_hi, N);
   if (D != 64 && D != 128) return fail(MODDIT_E_UNSUPPORTED, "sparse_attn_bwd: head_dim must be 64 or 128, got %d", D);
   if (dtype != MODDIT_BF16 && dtype != MODDIT_FP16) return fail(MODDIT_E_ARG, "sparse_attn_bwd: unknown dtype %d", dtype);
-  if (N > kMaxBlocks * kBlock) return fail(MODDIT_E_UNSUPPORTED, "sparse_attn_bwd: N=%d exceeds %d", N, kMaxBlocks * kBlock);
+  static_assert(kMaxBlocks * kBlock == MODDIT_ATTN_BWD_MAX_ROWS, "rows of a work item's block list");
+  if (N > MODDIT_ATTN_BWD_MAX_ROWS)
+    return fail(MODDIT_E_UNSUPPORTED, "sparse_attn_bwd: N=%d exceeds %d", N, MODDIT_ATTN_BWD_MAX_ROWS);
   if (static_cast<int64_t>(2 * ceil_div(N, kTile) + 1) * BH > (1ll << 31) - 1)
     return fail(MODDIT_E_UNSUPPORTED, "sparse_attn_bwd: %d heads of %d rows are too many work items", BH, N);
   const void* tensors[9] = {q, k, v, out, out_lo, dout, dq, dk, dv};

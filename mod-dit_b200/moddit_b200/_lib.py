@@ -114,6 +114,7 @@ for _name, (_res, _args) in SIGNATURES.items():
     _fn.argtypes = _args
 
 MODDIT_BF16, MODDIT_FP16 = 0, 1
+ATTN_BWD_MAX_ROWS, TOKEN_NORM_BWD_MAX_WIDTH = 458752, 49152
 NORM_KIND = {None: 0, "none": 0, "rms_head": 1, "rms_all_heads": 2, "layer": 3}
 ROPE_FORM = {"elementwise": 0, "even_cos_odd_sin": 1, "pair": 2}
 LAYOUT = {"wan": 0, "hunyuan": 1, "cogvideox": 2}

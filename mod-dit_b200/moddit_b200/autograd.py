@@ -11,15 +11,18 @@ from typing import Optional, Tuple
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import ops
+from . import _lib, ops
 
 __all__ = ["sparse_attention", "qkv_prologue"]
 
 
+def _builds_graph(*tensors: Optional[torch.Tensor]) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 class _SparseAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, lists, key_lists, limits, check_status, return_lse):
-        wanted = any(ctx.needs_input_grad[:3])
+    def forward(ctx, q, k, v, lists, key_lists, limits, check_status, return_lse, wanted):
         if check_status == "deferred" and q.is_cuda and not torch.cuda.is_current_stream_capturing():
             ops.check_posted_status(q.device)
         res = ops.sparse_attn_fwd(q, k, v, lists.counts, lists.entries, order=lists.order, return_residual=wanted,
@@ -43,7 +46,7 @@ class _SparseAttention(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout, _):
         if dout is None:
-            return (None,) * 8
+            return (None,) * 9
         q, k, v, out, lse, residual, *lists = ctx.saved_tensors
         deferred = ctx.check_status == "deferred"
         grads = ops.sparse_attn_bwd(dout.contiguous(), q, k, v, out, lse, ops.TileLists(*lists[:3]),
@@ -51,7 +54,7 @@ class _SparseAttention(torch.autograd.Function):
                                     check_status=False if deferred else ctx.check_status, **ctx.limits)
         if deferred:
             ops.post_status(q.device, spacing=ops.STATUS_SPACING)
-        return tuple(g if need else None for g, need in zip(grads, ctx.needs_input_grad)) + (None,) * 5
+        return tuple(g if need else None for g, need in zip(grads, ctx.needs_input_grad)) + (None,) * 6
 
 
 def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lists: ops.TileLists, key_lists: ops.KeyLists, *,
@@ -65,10 +68,16 @@ def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lists: o
     has arrived; copies are queued at most every `ops.STATUS_SPACING` seconds).  return_lse: (out, lse), lse a
     constant.  Tensors that are not contiguous are copied.  What lies between the forward and the backward is q, k, v, the
     output, what rounding took from it, 4 bytes per row and the work lists (of (N / 128)^2 entries of 4 bytes per mask head the
-    key lists, half as many the others)."""
+    key lists, half as many the others).
+
+    Where a graph is built, N is at most `_lib.ATTN_BWD_MAX_ROWS`."""
+    wanted = _builds_graph(q, k, v)
+    if wanted and q.dim() == 4 and q.shape[2] > _lib.ATTN_BWD_MAX_ROWS:
+        raise _lib.ModditError(f"gradients of the attention cover {_lib.ATTN_BWD_MAX_ROWS} rows, got {q.shape[2]}: run the "
+                               "forward alone under torch.no_grad()")
     limits = dict(softmax_scale=softmax_scale, q_split=q_split, kv_len_lo=kv_len_lo, kv_len_hi=kv_len_hi)
     out, lse = _SparseAttention.apply(q.contiguous(), k.contiguous(), v.contiguous(), lists, key_lists, limits, check_status,
-                                      return_lse)
+                                      return_lse, wanted)
     return (out, lse) if return_lse else out
 
 
@@ -127,11 +136,17 @@ def qkv_prologue(q_in: Optional[torch.Tensor] = None, k_in: Optional[torch.Tenso
     norm's parameters (the rotary tables are constants).
 
     Either q_in, k_in and v_in, (B, S, H*D) each, or `fused`, a contiguous (B, S, 3*H*D) projection whose gradient is written
-    in one piece.  The other arguments are those of `ops.qkv_prologue`."""
+    in one piece.  The other arguments are those of `ops.qkv_prologue`.  Where a graph is built, norm="rms_all_heads"
+    covers up to `_lib.TOKEN_NORM_BWD_MAX_WIDTH` values a token."""
     if (fused is None) == (q_in is None) or (fused is None and (k_in is None or v_in is None)) or \
             (fused is not None and (k_in is not None or v_in is not None)):
         raise ValueError("qkv_prologue: either q_in, k_in and v_in or fused")
     if fused is not None and (fused.dim() != 3 or not fused.is_contiguous() or fused.shape[-1] % (3 * num_heads)):
         raise ValueError(f"fused must be a contiguous (B, S, 3 * {num_heads} * D) tensor")
+    width = fused.shape[-1] // 3 if fused is not None else q_in.shape[-1]
+    if norm == "rms_all_heads" and width > _lib.TOKEN_NORM_BWD_MAX_WIDTH and \
+            _builds_graph(fused, q_in, k_in, v_in, q_weight, q_bias, k_weight, k_bias):
+        raise _lib.ModditError(f"gradients of a normalisation over all heads cover {_lib.TOKEN_NORM_BWD_MAX_WIDTH} values a "
+                               f"token, got {width}: run the forward alone under torch.no_grad()")
     opts = dict(num_heads=num_heads, norm=None if norm == "none" else norm, eps=eps, rope_form=rope_form, rope_range=rope_range)
     return _Prologue.apply(fused, q_in, k_in, v_in, q_weight, q_bias, k_weight, k_bias, rope_cos, rope_sin, opts)

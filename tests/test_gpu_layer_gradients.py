@@ -224,3 +224,20 @@ def test_a_single_group_of_heads_is_waited_for(mods, ask):
     got = torch.autograd.grad(out, leaves, dout) if ask else want
     torch.cuda.synchronize()
     assert torch.equal(out, want_out) and same(got, want)
+
+
+def test_without_a_graph_nothing_is_kept_for_one(mods, monkeypatch):
+    """Under no_grad the differentiable form is the forward alone, whatever its inputs would ask for."""
+    _, autograd, ops = mods
+    q, k, v, _ = inputs(60)
+    mask = torch.ones(1, 9, 9, dtype=torch.bool, device="cuda")
+    lists, klists = ops.tile_lists(mask, BS, N), ops.key_lists(mask, BS, N)
+    forward, kept = ops.sparse_attn_fwd, []
+    monkeypatch.setattr(ops, "sparse_attn_fwd", lambda *a, **kw: kept.append(kw["return_residual"]) or forward(*a, **kw))
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    with torch.no_grad():
+        out, lse = autograd.sparse_attention(*leaves, lists, klists, return_lse=True)
+    graph, graph_lse = autograd.sparse_attention(*leaves, lists, klists, return_lse=True)
+    assert kept == [False, True] and not out.requires_grad and graph.requires_grad and not graph_lse.requires_grad
+    assert torch.equal(out, graph) and torch.equal(lse, graph_lse)
+    assert torch.equal(autograd.sparse_attention(q, k, v, lists, klists), out)
