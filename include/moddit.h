@@ -353,6 +353,8 @@ int moddit_sparse_attn_fwd_residual(const void* q, const void* k, const void* v,
  *               the same mask (the orders may be NULL)
  *   workspace : moddit_sparse_attn_bwd_workspace_bytes(BH, N) bytes of scratch, 16-byte aligned
  *   status    : as in the forward
+ * float16: ds is held in float16 at its natural size, in steps of 2^-24 below 2^-14; a scaled loss keeps it above (17,000 keys: a
+ * dout of about 1 gives dq to its rounding, 0.02 to 0.08 %, 0.002 to 0.8 %).
  * Up to MODDIT_ATTN_BWD_MAX_ROWS rows.  Rows that attend to nothing (lse = -inf) and keys that no row attends to get zeros.  Keys at and past the larger limit are
  * never read, nor are blocks of 64 queries that see no key; all other rows have to be finite, because a block is multiplied whole
  * where the mask and the limits keep any of it.
