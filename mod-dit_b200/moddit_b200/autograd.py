@@ -48,12 +48,9 @@ class _SparseAttention(torch.autograd.Function):
         if dout is None:
             return (None,) * 9
         q, k, v, out, lse, residual, *lists = ctx.saved_tensors
-        deferred = ctx.check_status == "deferred"
         grads = ops.sparse_attn_bwd(dout.contiguous(), q, k, v, out, lse, ops.TileLists(*lists[:3]),
-                                    ops.KeyLists(*lists[3:]), residual=residual,
-                                    check_status=False if deferred else ctx.check_status, **ctx.limits)
-        if deferred:
-            ops.post_status(q.device, spacing=ops.STATUS_SPACING)
+                                    ops.KeyLists(*lists[3:]), residual=residual, check_status=ctx.check_status,
+                                    **ctx.limits)
         return tuple(g if need else None for g, need in zip(grads, ctx.needs_input_grad)) + (None,) * 6
 
 

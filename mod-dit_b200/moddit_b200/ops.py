@@ -936,7 +936,7 @@ def raise_on_status(device) -> None:
 
 
 _LAST_POST: Dict[int, float] = {}      # device index -> when `post_status` last queued a copy
-STATUS_SPACING = 1e-2                  # seconds between the copies that steps under autograd queue: a copy and its change of engines
+STATUS_SPACING = 1e-2                  # seconds between the copies that training calls queue: a copy and its change of engines
                                        # hold up a stream of short launches by some ten microseconds
 
 
@@ -993,9 +993,9 @@ def check_health(device) -> None:
             f"position={vals[3]}); the sparsity maps written since the last check are invalid")
 
 
-def _after_launch(dev, check_status) -> None:
+def _after_launch(dev, check_status, spacing: float = 0.0) -> None:
     if check_status == "deferred":
-        post_status(dev)
+        post_status(dev, spacing)
     elif check_status:
         raise_on_status(dev)
 
@@ -1075,8 +1075,8 @@ def _need_lists(lists, Hm: int, rows: int, tiles: int, dev: torch.device, what: 
 def sparse_attn_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
                     lse: torch.Tensor, lists: TileLists, key_lists: KeyLists, *, softmax_scale: Optional[float] = None,
                     q_split: Optional[int] = None, kv_len_lo: Optional[int] = None, kv_len_hi: Optional[int] = None,
-                    residual: Optional[torch.Tensor] = None,
-                    check_status=True) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+                    residual: Optional[torch.Tensor] = None, check_status=True,
+                    status_spacing: float = STATUS_SPACING) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Gradients (dq, dk, dv) of `sparse_attn_fwd` from the gradient `dout` of its output.
 
     q, k, v, the limits and the scale are the forward's, `out` and `lse` what it returned (`return_lse=True`), `lists`
@@ -1084,7 +1084,9 @@ def sparse_attn_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
     the gradients of q and k of rows with nearly all of their weight on one key exact to 16 bits.  The probabilities
     are computed again tile by tile; the results are the same bits on every run.  Keys at and past the larger limit
     are never read; all other rows have to be finite, but for whole blocks of 64 queries that see no key.
-    check_status: as in `sparse_attn_fwd`."""
+    check_status: as in `sparse_attn_fwd`, but "deferred" queues no copy of the status words within `status_spacing` seconds of
+    the last one.  A kernel that gave up is then reported by the next copy, of any call: the words stay set.  0 queues a copy
+    with every call, which a caller wants who looks with `check_posted_status` at this very call."""
     rest = () if residual is None else (residual,)
     dev = _need_cuda(dout, q, k, v, out, lse, *rest)
     if q.dim() != 4:
@@ -1118,5 +1120,5 @@ def sparse_attn_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
             D ** -0.5 if softmax_scale is None else softmax_scale, N if q_split is None else q_split,
             N if kv_len_lo is None else kv_len_lo, N if kv_len_hi is None else kv_len_hi, dq.data_ptr(), dk.data_ptr(),
             dv.data_ptr(), ws.data_ptr(), wsb, _status_words(dev).data_ptr(), _stream(dev)), "moddit_sparse_attn_bwd")
-    _after_launch(dev, check_status)
+    _after_launch(dev, check_status, spacing=status_spacing)
     return dq, dk, dv
