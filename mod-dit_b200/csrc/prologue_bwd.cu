@@ -8,8 +8,9 @@
 // from x, so the forward keeps nothing for this pass but its inputs.
 //
 // Bound: HBM.  Algorithmic bytes per token: q and k 3 * 2 * H * D each (g and x in, dx out), v 2 * 2 * H * D; the rotary
-// tables are fetched once for all heads.  57,728 tokens of 16 x 128 (one fused projection, rms per head) 320 us = 6.1 TB/s, 93 %
-// of the measured copy bandwidth; 2 x 45,104 of 30 x 64 (layer) 467 - 514 us = 5.4 - 5.9 TB/s.
+// tables are fetched once for all heads.  57,728 tokens of 16 x 128 (one fused projection, rms per head) 320 - 327 us = 6.0 - 6.1
+// TB/s, 91 - 93 % of the measured copy bandwidth; 2 x 45,104 of 30 x 64 (layer) 466 - 524 us = 5.3 - 6.0 TB/s; without a norm
+// 57,728 tokens of 16 x 128 242 us = 6.1 TB/s.
 //
 // Weight gradients are sums over all tokens.  Blocks are persistent: a thread keeps float32 sums for the eight columns it
 // always has, a block adds its threads' sums in shared memory and writes one row of partial sums, and a second kernel adds
@@ -300,8 +301,9 @@ __global__ void __launch_bounds__(kThreads, 2) prologue_bwd_kernel(const __grid_
 // (from the L2), writes dx and adds to its columns' weight gradient, which lives in shared memory.  A piece lies at the same
 // columns of its head for all pieces of a lane or thread, so the rotary factors are read once a token: in the second part from
 // shared memory, where the first part's lanes have put them.
-// For tokens too wide for the kernel below.  8,640 tokens of 40 x 128: 172 us, 63 % of the measured copy bandwidth; bound by
-// instructions and the two parts' latencies.
+// For tokens too wide for the kernel below.  8,192 tokens of 48 x 128 186 us, 67 % of the measured copy bandwidth; 4,096 of
+// 64 x 128 141 us, 58 %; 4,096 of 128 x 128 279 us, 59 %; bound by instructions and the two parts' latencies.  At 8,640 of 40 x
+// 128, which the kernel below has now, it took 172 us.
 // Slower: a group's rows kept in shared memory between the parts, copied a group ahead (204 us with two blocks an SM, 257 with
 // one: block-wide sums and fewer warps), half as many tokens in flight with three or four blocks an SM (190 - 230).
 template <typename T, int D, bool kPair>
@@ -442,7 +444,7 @@ __global__ void __launch_bounds__(kThreads, 2) prologue_bwd_all_heads_kernel(con
 // places of the thread's own in shared memory, as in the per-head kernel, and with them the two tokens' rows of the rotary
 // tables, once a block.  Where q, k and v are all given, a block of q or k also copies one token of v per pair of its own:
 // copies want bytes, the sums want instructions.
-// 8,640 tokens of 40 x 128: 130 us, 5.5 TB/s, 83 % of the measured copy bandwidth; 260 instructions a piece, issued in 0.65 of
+// 8,640 tokens of 40 x 128: 129 - 139 us, 5.1 - 5.5 TB/s, 78 - 84 % of the measured copy bandwidth; 260 instructions a piece, issued in 0.65 of
 // the cycles, are the other bound.  On the way: divisions and products for every pair's addresses, rotary rows loaded per thread
 // 170 us; those loaded a pair ahead 158 (spills where a table has a value a column); pointers moved on by additions 154; rotary
 // rows through shared memory 145; v beside q and k 137; q and k at once, half of the blocks each, 130.  Slower: two operations

@@ -9,8 +9,8 @@
 //   query item  one tile of 128 queries, walks its key tiles: three products per tile
 //               S = Q K^T, dP = dO V^T, dQ += dS K
 // That is seven products where one pass over the pairs would need five; that pass would add every tile's 64 KB of float32 dQ
-// into memory with atomics, in an order that varies, and at D = 128 has no tensor memory left for dQ.  Keeping dS for a product
-// of its own would take 32 KB per kept tile (12 GB for three heads of 115,456 tokens).
+// into memory with atomics, in an order that varies (tensor memory would have room for it, with 64 streamed rows at a time).
+// Keeping dS for a product of its own would take 32 KB per kept tile (12 GB for three heads of 115,456 tokens).
 //
 // Both kinds work alike: a block holds two fixed tiles (F0, F1 = K, V or Q, dO) and streams blocks of 64 rows of two tensors
 // (X0, X1 = Q, dO or K, V):   S = F0 X0^T,  dP = F1 X1^T,  acc1 += P X1 (key items),  acc0 += dS X0.
@@ -21,10 +21,11 @@
 // Roles: warp 0 TMA producer, 1 and 3 MMA issuers, 2 tensor-memory allocation, 3 first the item's block list, 4 and up
 // elementwise.
 //
-// Measured (B200; launch alone, clocks falling to 1.6 GHz at the power limit at D = 128): three heads of 115,456 tokens, block
-// 128, 15 % kept, D = 128 7.4 - 8.3 ms = 0.97 - 1.08 PFLOP/s on the five products of the kept pairs (58 - 65 % of the measured
-// burst rate, 1.35 - 1.5 PFLOP/s on the seven that run, about the rate a library product sustains); dense 24 x 4,096 543 us;
-// six heads of 45,104, block 64, D = 64 1.78 ms.  ncu, eight heads of 16,640 tokens at 25 %: tensor pipe 71 % at D = 128, 55 %
+// Measured (B200): three heads of 115,456 tokens, block 128, 15 % kept, D = 128 8.6 - 8.8 ms a call in a loop of calls = 0.91 -
+// 0.93 PFLOP/s on the five products of the kept pairs (55 - 56 % of the measured burst rate; 1.27 - 1.3 PFLOP/s on the seven that
+// run, 90 - 92 % of what a library product sustains); a few launches after a pause, before the clocks fall to 1.6 GHz at the power
+// limit, 7.4 - 7.5 ms.  Dense 24 x 4,096 545 us; six heads of 45,104, block 64, D = 64 1.78 ms after a pause, 2.04 - 2.09 in a
+// loop.  ncu, eight heads of 16,640 tokens at 25 %: tensor pipe 71 % at D = 128, 55 %
 // at D = 64, exponential unit 41 and 43 %.  What bounds it: at D = 128 power and the tensor pipe; at D = 64 the chain of waits
 // that a 64-column step is (scores, probabilities, dP, dS, products), of which tensor memory has room for three at a time.
 // From the first working version (one step at a time, 8 elementwise warps, 128-row tiles) 9.95 ms, 689 us and 4.36 ms.
