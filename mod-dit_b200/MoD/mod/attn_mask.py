@@ -297,7 +297,6 @@ def AttentionSparseEngine(query, key, value, mask, pre_defined_mask=None, video_
     branch with the 64-rounded border.
     """
     seq_len = query.shape[2]
-    query, key = query.contiguous(), key.contiguous()
     all_kept = False
     if _lists is not None:
         lists = _lists
@@ -305,10 +304,12 @@ def AttentionSparseEngine(query, key, value, mask, pre_defined_mask=None, video_
         lists, all_kept = _engine_lists(mask, block_size, seq_len)
     counts, entries, order = lists.counts, lists.entries, lists.order
     grouped = _group_ready is not None and len(_group_ready) > 1
-    # inputs produced on another stream (e.g. still arriving from peers); a single group is one more of them
-    for ev in _events(_value_ready) + (() if grouped else _events(_group_ready)):
+    # inputs produced on another stream (e.g. still arriving from peers); a single group is one more of them, and what has to
+    # be copied has to be there whole
+    whole = not grouped or not all(t.is_contiguous() for t in (query, key, value))
+    for ev in _events(_value_ready) + (_events(_group_ready) if whole else ()):
         torch.cuda.current_stream(query.device).wait_event(ev)
-    value = value.contiguous()
+    query, key, value = query.contiguous(), key.contiguous(), value.contiguous()
     fwd_kw = {}
     if pre_defined_mask is not None:
         valid = _valid_kv(pre_defined_mask, seq_len)
@@ -505,6 +506,9 @@ def SparseAttentionWithMap(
     pooled = warmup_state.get('score_producer', 'replay') == 'pooled'
     warmup_steps = warmup_state['warmup_steps']
     value_ready = kwargs.get('value_ready')
+    if not (query.is_contiguous() and key.is_contiguous()):        # the copies read rows that may still be arriving
+        for ev in _events(kwargs.get('qk_ready')) + _events(kwargs.get('head_group_ready')):
+            torch.cuda.current_stream(query.device).wait_event(ev)
     query, key = query.contiguous(), key.contiguous()
 
     if pooled:

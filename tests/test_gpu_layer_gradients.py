@@ -241,3 +241,40 @@ def test_without_a_graph_nothing_is_kept_for_one(mods, monkeypatch):
     assert kept == [False, True] and not out.requires_grad and graph.requires_grad and not graph_lse.requires_grad
     assert torch.equal(out, graph) and torch.equal(lse, graph_lse)
     assert torch.equal(autograd.sparse_attention(q, k, v, lists, klists), out)
+
+
+@pytest.mark.parametrize("way", ["value", "groups", "step", "step by groups"])
+@pytest.mark.parametrize("ask", [False, True])
+def test_copies_of_other_layouts_wait_for_the_rows(mods, way, ask):
+    """Query, key and value of (B, N, H, D) order are copied: behind the events that say that their rows are there."""
+    am, _, ops = mods
+    q, k, v, dout = inputs(32)
+    mask = torch.rand(H, 9, 9, generator=torch.Generator().manual_seed(4)).lt(0.5).cuda()
+    pools = tuple(ops.pool_blocks(t, BS) for t in (q, k))
+    by_groups = "groups" in way
+    state = new_state(score_producer="pooled", **(dict(_head_groups=H) if by_groups else {}))
+    if "step" in way:
+        am.SparseAttentionWithMap(q, k, v, state, LOG, current_step=1)           # collects
+    late = [torch.zeros(1, N, H, D, device="cuda", dtype=q.dtype) for _ in range(3)]
+    lists = ops.tile_lists(mask, BS, N, heads_per_group=1 if by_groups else None)
+    torch.cuda.synchronize()
+    side, ready = torch.cuda.Stream(), [torch.cuda.Event() for _ in range(H)]
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20000000)
+        for h, e in enumerate(ready):
+            for dst, src in zip(late, (q, k, v)):
+                dst[:, :, h].copy_(src[:, h])
+            e.record()
+    leaves = [t.transpose(1, 2).requires_grad_(ask) for t in late]
+    if way == "value":
+        out = am.AttentionSparseEngine(*leaves, mask, block_size=BS, _lists=lists, _value_ready=ready[-1])
+    elif way == "groups":
+        out = am.AttentionSparseEngine(*leaves, mask, block_size=BS, _lists=lists, _group_ready=ready)
+    else:
+        events = dict(head_group_ready=ready) if by_groups else dict(qk_ready=ready[-1])
+        out, _ = am.SparseAttentionWithMap(*leaves, state, LOG, current_step=2, pooled_qk=pools, **events)
+        mask = state["mask"]
+    got = torch.autograd.grad(out, leaves, dout) if ask else None
+    torch.cuda.synchronize()
+    want_out, want = wanted(mods, q, k, v, dout, mask)
+    assert torch.equal(out, want_out) and (not ask or same(got, want))
